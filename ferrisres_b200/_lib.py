@@ -112,6 +112,10 @@ SIGNATURES = {
     "ft_kv3_get_range": [_p, _p, _i64, _i64, _p, _p, _p],
     "ft_kv3_export_range": [_p, _p, _i64, _i64, _p, _p, _p, _p, _p],
     "ft_flash_decode_3bit": [_p, _p, _p, _i64, C.c_float, _p, _p],
+    "ft_flash_decode_3bit_weights": [_p, _p, _p, _i64, C.c_float, _p, _p, _i64, _p],
+    "ft_kv3_tree_decode": [_p, _p, _i64, _p, _i, _i64, _p, C.c_float, _p, _p],
+    "ft_kv_select_heavy": [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _p],
+    "ft_kv3_keep": [_p, _p, _i64, _i64, _p, _i64, _i64, _p],
     "ft_kvp_create": [_p, _i64, _i64, _i64, _i64, _i, C.c_uint64, _p],
     "ft_kvp_destroy": [_p],
     "ft_kvp_signs": [_p, _p],
@@ -121,6 +125,11 @@ SIGNATURES = {
     "ft_kvp_get_range": [_p, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "ft_kvp_export_range": [_p, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
     "ft_kvp_flash_decode": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, C.c_float, _p, _p],
+    "ft_kvp_flash_decode_weights": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, C.c_float, _p, _p,
+                                    _i64, _p],
+    "ft_kvp_tree_decode": [_p, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _p, C.c_float,
+                           _p, _p],
+    "ft_kvp_keep": [_p, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p],
 }
 _RESTYPE = {"ft_version": C.c_char_p, "ft_last_error_string": C.c_char_p,
             "ft_launch_counter": C.c_uint64}

@@ -62,52 +62,20 @@
 // D H / sqrt(128).
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <vector>
 
-#include "ft_internal.cuh"
+#include "ft_kv3.cuh"
 #include "ft_tc.cuh"
-
-struct ft_kv3 {
-  int device = 0;
-  int64_t batch = 0, kv_heads = 0, cap = 0;  // cap: slots per row, multiple of 32
-  int64_t head = 0, len = 0;                   // ring start slot, live positions
-  uint32_t* blocks = nullptr;  // [row][cap/32] block records
-  ft::Workspace part;  // split partials
-  int mode = 0;                // 0: the reference's min/max scheme, 1: mode T
-  float* signs = nullptr;      // mode T: the 128 rotation signs (device)
-  ft::Workspace rot;           // mode T: the rotated queries
-};
-
-// The page pool of the paged cache: page P holds 32 positions of every kv
-// head, record (P, h) at (P * kv_heads + h) * 3584 bytes -- the ring's record,
-// so the same kernels serve both.  The pool is storage only: which pages a
-// sequence owns, and in which order, is the caller's block table.
-struct ft_kvp {
-  int device = 0;
-  int64_t n_pages = 0, kv_heads = 0;
-  uint32_t* blocks = nullptr;
-  int mode = 0;
-  float* signs = nullptr;
-  ft::Workspace part, rot;
-};
 
 namespace ft {
 namespace {
 
-constexpr int kD = 128;                  // head dim = quantisation group
-constexpr int kRec = 48;                 // bytes of codes per vector
-constexpr int kBlk = 32;                 // slots per block
-constexpr int kBlkWords = kBlk * kRec / 4;  // 384
-constexpr int kBlkBytes = kBlk * kRec;   // 1536 (both K and V)
-constexpr int kMmBlkBytes = kBlk * 8;    // 256
 constexpr int kDecWarps = 4;             // compute warps = blocks per tile
 #ifndef FT_KV_STAGES
 #define FT_KV_STAGES 4
 #endif
 constexpr int kStages = FT_KV_STAGES;
-constexpr int kRecBytes = 2 * kBlkBytes + 2 * kMmBlkBytes;  // 3584: K | V | K min/max | V min/max
-constexpr int kRecWords = kRecBytes / 4;
-constexpr int kRecV = kBlkWords, kRecKmm = 2 * kBlkWords, kRecVmm = 2 * kBlkWords + 2 * kBlk;
 constexpr int kStageBytes = kDecWarps * kRecBytes;  // 14336
 constexpr int kWsmBytes = kDecWarps * 4 * 4 * kBlk;      // [warp][digit][head][8 words]
 constexpr int kQfBytes = 4 * 32 * 16;                    // q fragments [chunk][lane][16 B]
@@ -124,52 +92,6 @@ static_assert(kQdBytes <= kOsmBytes, "q digits are staged in the numerator area"
 #ifndef FT_KV_MIN_BLOCKS
 #define FT_KV_MIN_BLOCKS 3
 #endif
-
-__device__ __forceinline__ float load_act(const void* p, int64_t i, int bf16) {
-  return bf16 ? __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[i] << 16)
-              : static_cast<const float*>(p)[i];
-}
-
-// ---- layout maps (word indices within a 384-word block) ----
-// triple base word and quad of K code (slot s, dim d) / V code (slot s, dim d)
-__device__ __forceinline__ int k_triple(int s, int d) {
-  return (4 * (s & 7) + ((d >> 2) & 3)) * 12 + 3 * (s >> 3);
-}
-__device__ __forceinline__ int k_quad(int d) { return d >> 4; }
-__device__ __forceinline__ int k_elem(int s, int d) { return d & 3; }
-__device__ __forceinline__ int v_triple(int s, int d) {
-  return (4 * (d & 7) + (s & 3)) * 12 + 3 * (d >> 5);
-}
-__device__ __forceinline__ int v_quad(int s, int d) {
-  return 2 * (2 * ((d >> 4) & 1) + ((d >> 3) & 1)) + ((s >> 2) & 1);
-}
-__device__ __forceinline__ int v_elem(int s) { return s >> 3; }
-__device__ __forceinline__ int mm_index(int s) { return (s & 7) * 4 + (s >> 3); }
-
-__device__ __forceinline__ uint32_t triple_get(const uint32_t* t, int Q, int b) {
-  if (Q < 6) return (t[Q >> 1] >> (8 * b + 3 * (Q & 1))) & 7u;
-  return ((t[Q - 6] >> (8 * b + 6)) & 3u) | (((t[2] >> (8 * b + Q)) & 1u) << 2);
-}
-// writes code c at (Q, b) of a shared-memory triple; concurrent writers touch
-// disjoint bits
-__device__ __forceinline__ void triple_put(uint32_t* t, int Q, int b, uint32_t c) {
-  if (Q < 6) {
-    const int sh = 8 * b + 3 * (Q & 1);
-    atomicAnd(&t[Q >> 1], ~(7u << sh));
-    atomicOr(&t[Q >> 1], c << sh);
-  } else {
-    atomicAnd(&t[Q - 6], ~(3u << (8 * b + 6)));
-    atomicOr(&t[Q - 6], (c & 3u) << (8 * b + 6));
-    atomicAnd(&t[2], ~(1u << (8 * b + Q)));
-    atomicOr(&t[2], (c >> 2) << (8 * b + Q));
-  }
-}
-__device__ __forceinline__ uint32_t k_code(const uint32_t* blk, int s, int d) {
-  return triple_get(blk + k_triple(s, d), k_quad(d), k_elem(s, d));
-}
-__device__ __forceinline__ uint32_t v_code(const uint32_t* blk, int s, int d) {
-  return triple_get(blk + v_triple(s, d), v_quad(s, d), v_elem(s));
-}
 
 // ---------------------------------------------------------------- append --
 struct AppendParams {
@@ -188,18 +110,6 @@ struct AppendParams {
   int64_t tstride, n_pages;
   int* err;
 };
-
-// A page index read from a caller's block table, checked: out-of-range
-// entries are recorded in the error word (site `code`) and replaced by -1.
-__device__ __forceinline__ int64_t checked_page(const int32_t* table, int64_t idx,
-                                                int64_t n_pages, int* err, int code) {
-  const int32_t pg = table[idx];
-  if (pg < 0 || pg >= n_pages) {
-    if (err) atomicCAS(err, 0, code);
-    return -1;
-  }
-  return pg;
-}
 
 // Mode T constants: clip at 2.5 and the (min, max) factor 2.5 * 7/8 / sqrt(128).
 constexpr float kTClip = 2.5f;
@@ -504,6 +414,10 @@ struct DecodeParams {
   const int32_t* table;
   const int32_t* seq_lens;
   int64_t tstride, n_pages;
+  // decode with weights: the scores (log2 domain) of every q head at every
+  // slot of the logical blocks, [B][Hq][score_stride]
+  float* scores;
+  int64_t score_stride;
 };
 
 __device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -543,6 +457,8 @@ __device__ __forceinline__ float small_int_to_float(int d) {
   return __int_as_float(0x4B400000 + d) - 12582912.0f;
 }
 
+// kScores: the scores are also written out, for kv3_weights_kernel.
+template <bool kScores>
 __global__ void __launch_bounds__((kDecWarps + 1) * 32, FT_KV_MIN_BLOCKS)
     kv3_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -802,6 +718,11 @@ __global__ void __launch_bounds__((kDecWarps + 1) * 32, FT_KV_MIN_BLOCKS)
           }
         }
       }
+      if (kScores && r < nheads) {  // 8 lanes of a head write 32 contiguous bytes
+        float* sp = p.scores + ((b * p.Hq) + qh0 + r) * p.score_stride + (int64_t)j * kBlk + g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sp[8 * e] = s2[e];
+      }
       // ---- online softmax (head r): max over the block's 32 slots
       float mt = fmaxf(fmaxf(s2[0], s2[1]), fmaxf(s2[2], s2[3]));
 #pragma unroll
@@ -948,9 +869,9 @@ __global__ void __launch_bounds__((kDecWarps + 1) * 32, FT_KV_MIN_BLOCKS)
 
 // Merges the split partials of one (sequence, q head): thread = dim.
 // Mode T (signs != null): the rotated-domain output is rotated back.
-__global__ void kv3_combine_kernel(const float* __restrict__ part, int nsplit,
-                                   float* __restrict__ out, const float* __restrict__ signs) {
-  const int64_t bh = blockIdx.x;
+__device__ __forceinline__ void combine_head(const float* __restrict__ part, int nsplit,
+                                             float* __restrict__ out,
+                                             const float* __restrict__ signs, int64_t bh) {
   const int d = threadIdx.x;
   const float* pp = part + bh * nsplit * kPart;
   float M = -INFINITY;
@@ -973,74 +894,84 @@ __global__ void kv3_combine_kernel(const float* __restrict__ part, int nsplit,
   out[bh * kD + d] = r;
 }
 
+__global__ void kv3_combine_kernel(const float* __restrict__ part, int nsplit,
+                                   float* __restrict__ out, const float* __restrict__ signs) {
+  combine_head(part, nsplit, out, signs, blockIdx.x);
+}
+
+// Attention weight of every position, added to weights [B][Hkv][wstride]:
+// w[b, hk, s] += sum over the q heads of group hk of exp2(score - M) / l, with
+// (M, l) the softmax statistics that the split partials give.  Blocks x <
+// chunks take kWeightChunk positions each; the G blocks behind them merge the
+// outputs, so that a decode with weights is two launches like one without.
+constexpr int kWeightChunk = 1024;
+__global__ void __launch_bounds__(kD)
+    kv3_weights_kernel(const __grid_constant__ DecodeParams p, int nsplit, int chunks,
+                       float* __restrict__ weights, int64_t wstride, float* __restrict__ out,
+                       const float* __restrict__ signs) {
+  const int x = blockIdx.x;
+  const int64_t kvh = blockIdx.y, b = blockIdx.z;
+  const int64_t h0 = b * p.Hq + kvh * p.G;
+  if (x >= chunks) {
+    combine_head(p.part, nsplit, out, signs, h0 + (x - chunks));
+    return;
+  }
+  int64_t len = p.len;
+  if (p.table) {
+    len = p.seq_lens[b];  // the decode kernel reports a bad length
+    len = len < 0 ? 0 : (len > p.len ? p.len : len);
+  }
+  const int64_t first = (int64_t)x * kWeightChunk;
+  if (first >= len) return;
+  extern __shared__ float stat[];  // [G] M, then [G] 1 / l
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int h = warp; h < p.G; h += kD / 32) {
+    const float* pp = p.part + (h0 + h) * nsplit * kPart;
+    float M = -INFINITY;
+    for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, pp[s * kPart]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float l = 0.0f;
+    for (int s = lane; s < nsplit; s += 32) {
+      const float m = pp[s * kPart];
+      if (m != -INFINITY) l = fmaf(pp[s * kPart + 1], exp2f(m - M), l);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      stat[h] = M;
+      stat[p.G + h] = 1.0f / l;
+    }
+  }
+  __syncthreads();
+  float* w = weights + (b * p.Hkv + kvh) * wstride;
+  const float* sc = p.scores + h0 * p.score_stride + p.head_off;
+  const int64_t end = first + kWeightChunk < len ? first + kWeightChunk : len;
+  for (int64_t i = first + threadIdx.x; i < end; i += kD) {
+    float a = 0.0f;
+    for (int h = 0; h < p.G; ++h)
+      a = fmaf(exp2f(sc[h * p.score_stride + i] - stat[h]), stat[p.G + h], a);
+    w[i] += a;
+  }
+}
+
 // Opts the decode kernel into its dynamic shared memory (once per device) and
 // returns its resident CTAs per SM.
 int decode_occupancy(int device) {
   static int cached[64] = {0};
   if (device >= 0 && device < 64 && cached[device]) return cached[device];
-  cudaFuncSetAttribute(kv3_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem);
+  cudaFuncSetAttribute(kv3_decode_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       kDecSmem);
+  cudaFuncSetAttribute(kv3_decode_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       kDecSmem);
   int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kv3_decode_kernel,
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kv3_decode_kernel<false>,
                                                     (kDecWarps + 1) * 32, kDecSmem) != cudaSuccess ||
       occ < 1)
     occ = 1;
   if (device >= 0 && device < 64) cached[device] = occ;
   return occ;
 }
-
-// New ring of at least `need` slots; the live blocks are copied in logical
-// order, so the new head is head % 32.
-int grow(ft_kv3* c, int64_t need, cudaStream_t s) {
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  if (s) cudaStreamIsCapturing(s, &cs);
-  FT_CHECK(cs == cudaStreamCaptureStatusNone, FT_ERR_UNSUPPORTED,
-           "the 3-bit KV cache must grow but the stream is being captured");
-  int64_t ncap = c->cap * 2;
-  if (ncap < need + kBlk) ncap = need + kBlk;  // room for the head offset
-  ncap = round_up(ncap, kBlk);
-  const int64_t rows = c->batch * c->kv_heads, nbc = c->cap / kBlk, nnbc = ncap / kBlk;
-  uint32_t* blocks = nullptr;
-  cudaError_t e = cudaMalloc(&blocks, (size_t)(rows * nnbc) * kRecBytes);
-  if (e == cudaSuccess) e = cudaMemsetAsync(blocks, 0, (size_t)(rows * nnbc) * kRecBytes, s);
-  if (e != cudaSuccess) {
-    cudaFree(blocks);
-    return fail(e == cudaErrorMemoryAllocation ? FT_ERR_OOM : FT_ERR_GPU,
-                "3-bit KV cache growth to %lld slots failed: %s", (long long)ncap,
-                cudaGetErrorString(e));
-  }
-  const int64_t hb = c->head / kBlk;
-  const int64_t nlb = c->len == 0 ? 0 : (c->head % kBlk + c->len + kBlk - 1) / kBlk;
-  // runs of physical blocks: [hb, hb + n1) then [0, nlb - n1)
-  const int64_t n1 = nlb < nbc - hb ? nlb : nbc - hb;
-  const int64_t runs[2][3] = {{hb, 0, n1}, {0, n1, nlb - n1}};  // src block, dst block, count
-  const size_t rb = (size_t)kRecBytes;
-  for (const auto& run : runs) {
-    if (run[2] <= 0) continue;
-    FT_CUDA(cudaMemcpy2DAsync(reinterpret_cast<uint8_t*>(blocks) + run[1] * rb, nnbc * rb,
-                              reinterpret_cast<uint8_t*>(c->blocks) + run[0] * rb, nbc * rb,
-                              run[2] * rb, rows, cudaMemcpyDeviceToDevice, s));
-  }
-  FT_CUDA(cudaStreamSynchronize(s));
-  cudaFree(c->blocks);
-  c->blocks = blocks;
-  c->cap = ncap;
-  c->head = c->head % kBlk;
-  return FT_OK;
-}
-
-class DeviceScope {
- public:
-  explicit DeviceScope(int dev) : dev_(dev) {
-    cudaGetDevice(&prev_);
-    if (prev_ != dev) cudaSetDevice(dev);
-  }
-  ~DeviceScope() {
-    if (prev_ >= 0 && prev_ != dev_) cudaSetDevice(prev_);
-  }
-
- private:
-  int dev_ = 0, prev_ = -1;
-};
 
 int append_common(ft_kv3* c, int64_t n_pos, const AppendParams& proto, bool packed,
                   cudaStream_t s) {
@@ -1052,7 +983,7 @@ int append_common(ft_kv3* c, int64_t n_pos, const AppendParams& proto, bool pack
     const int64_t s0 = (c->head + c->len) % c->cap;
     const int64_t nblk = (s0 % kBlk + n_pos + kBlk - 1) / kBlk;
     if (c->len + n_pos > c->cap || nblk > c->cap / kBlk) {
-      const int rc = grow(c, c->len + n_pos, s);
+      const int rc = kv3_grow(c, c->len + n_pos, s);
       if (rc != FT_OK) return rc;
     }
   }
@@ -1096,6 +1027,12 @@ cudaError_t upload_signs(uint64_t seed, float** out) {
   return e;
 }
 
+template <class Cache>
+void free_workspaces(Cache* c) {
+  for (Workspace* w : {&c->part, &c->rot, &c->scores, &c->tree}) cudaFree(w->ptr);
+  for (void* p : c->retired) cudaFree(p);
+}
+
 RangeParams range_params(const ft_kv3* c, int64_t start, int64_t n) {
   RangeParams p{};
   p.B = c->batch;
@@ -1110,6 +1047,47 @@ RangeParams range_params(const ft_kv3* c, int64_t start, int64_t n) {
 }
 
 }  // namespace
+
+// New ring of at least `need` slots; the live blocks are copied in logical
+// order, so the new head is head % 32.
+int kv3_grow(ft_kv3* c, int64_t need, cudaStream_t s) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  if (s) cudaStreamIsCapturing(s, &cs);
+  FT_CHECK(cs == cudaStreamCaptureStatusNone, FT_ERR_UNSUPPORTED,
+           "the 3-bit KV cache must grow but the stream is being captured");
+  int64_t ncap = c->cap * 2;
+  if (ncap < need + kBlk) ncap = need + kBlk;  // room for the head offset
+  ncap = round_up(ncap, kBlk);
+  const int64_t rows = c->batch * c->kv_heads, nbc = c->cap / kBlk, nnbc = ncap / kBlk;
+  uint32_t* blocks = nullptr;
+  cudaError_t e = cudaMalloc(&blocks, (size_t)(rows * nnbc) * kRecBytes);
+  if (e == cudaSuccess) e = cudaMemsetAsync(blocks, 0, (size_t)(rows * nnbc) * kRecBytes, s);
+  if (e != cudaSuccess) {
+    cudaFree(blocks);
+    return fail(e == cudaErrorMemoryAllocation ? FT_ERR_OOM : FT_ERR_GPU,
+                "3-bit KV cache growth to %lld slots failed: %s", (long long)ncap,
+                cudaGetErrorString(e));
+  }
+  const int64_t hb = c->head / kBlk;
+  const int64_t nlb = c->len == 0 ? 0 : (c->head % kBlk + c->len + kBlk - 1) / kBlk;
+  // runs of physical blocks: [hb, hb + n1) then [0, nlb - n1)
+  const int64_t n1 = nlb < nbc - hb ? nlb : nbc - hb;
+  const int64_t runs[2][3] = {{hb, 0, n1}, {0, n1, nlb - n1}};  // src block, dst block, count
+  const size_t rb = (size_t)kRecBytes;
+  for (const auto& run : runs) {
+    if (run[2] <= 0) continue;
+    FT_CUDA(cudaMemcpy2DAsync(reinterpret_cast<uint8_t*>(blocks) + run[1] * rb, nnbc * rb,
+                              reinterpret_cast<uint8_t*>(c->blocks) + run[0] * rb, nbc * rb,
+                              run[2] * rb, rows, cudaMemcpyDeviceToDevice, s));
+  }
+  FT_CUDA(cudaStreamSynchronize(s));
+  cudaFree(c->blocks);
+  c->blocks = blocks;
+  c->cap = ncap;
+  c->head = c->head % kBlk;
+  return FT_OK;
+}
+
 }  // namespace ft
 
 using namespace ft;
@@ -1173,9 +1151,8 @@ int ft_kv3_destroy(ft_kv3* c) {
   DeviceScope scope(c->device);
   cudaDeviceSynchronize();
   cudaFree(c->blocks);
-  if (c->part.ptr) cudaFree(c->part.ptr);
   if (c->signs) cudaFree(c->signs);
-  if (c->rot.ptr) cudaFree(c->rot.ptr);
+  free_workspaces(c);
   delete c;
   return FT_OK;
 }
@@ -1274,39 +1251,25 @@ int ft_kv3_export_range(ft_ctx* ctx, const ft_kv3* c, int64_t start, int64_t end
 namespace ft {
 namespace {
 
-// Grows a workspace outside stream capture (a capture may only reuse it).
-int ensure_ws(Workspace& w, size_t need, cudaStream_t s, const char* what) {
-  if (w.bytes >= need) return FT_OK;
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  if (s) cudaStreamIsCapturing(s, &cs);
-  FT_CHECK(cs == cudaStreamCaptureStatusNone, FT_ERR_UNSUPPORTED,
-           "the %s buffer must grow but the stream is being captured", what);
-  if (w.ptr) {
-    FT_CUDA(cudaStreamSynchronize(s));
-    FT_CUDA(cudaFree(w.ptr));
-    w.ptr = nullptr;
-    w.bytes = 0;
-  }
-  FT_CUDA(cudaMalloc(&w.ptr, need));
-  w.bytes = need;
-  return FT_OK;
-}
-
 // Rotates q (mode T), picks the split of the slots, launches the decode and
 // the combine.  p carries the cache geometry (ring or paged); p.len is the
 // longest sequence.
-int launch_decode(ft_ctx* ctx, DecodeParams p, int64_t batch, int64_t kv_heads, int64_t q_heads,
-                  const float* signs, Workspace& part, Workspace& rot, const float* q_dev,
-                  float scale, float* out_dev, cudaStream_t s) {
+template <class Cache>
+int launch_decode(ft_ctx* ctx, Cache* c, DecodeParams p, int64_t batch, int64_t q_heads,
+                  const float* q_dev, float scale, float* out_dev, float* weights_dev,
+                  int64_t weights_stride, cudaStream_t s) {
+  const int64_t kv_heads = c->kv_heads;
+  const float* signs = c->signs;
   p.q = q_dev;
   if (signs) {
     // mode T: attention runs in the rotated domain
-    const int rc = ensure_ws(rot, (size_t)(batch * q_heads * kD) * 4, s, "rotated-query");
+    const int rc = ensure_ws(c->rot, (size_t)(batch * q_heads * kD) * 4, s, "rotated-query",
+                             c->retired);
     if (rc != FT_OK) return rc;
     kv3_rotate_kernel<<<(unsigned)(batch * q_heads), kD, 0, s>>>(
-        q_dev, static_cast<float*>(rot.ptr), signs, 0);
+        q_dev, static_cast<float*>(c->rot.ptr), signs, 0);
     FT_LAUNCH_CHECK();
-    p.q = static_cast<const float*>(rot.ptr);
+    p.q = static_cast<const float*>(c->rot.ptr);
   }
   p.Hq = q_heads;
   p.Hkv = kv_heads;
@@ -1339,12 +1302,29 @@ int launch_decode(ft_ctx* ctx, DecodeParams p, int64_t batch, int64_t kv_heads, 
   const int64_t nsplit = ceil_div(ntiles, best_per);
   FT_CHECK(nsplit <= 65535 && kv_heads * p.hgroups <= 65535 && batch <= 65535,
            FT_ERR_UNSUPPORTED, "decode grid too large");
-  const int rc = ensure_ws(part, (size_t)(batch * q_heads * nsplit * kPart) * 4, s,
-                           "decode partials");
+  const int rc = ensure_ws(c->part, (size_t)(batch * q_heads * nsplit * kPart) * 4, s,
+                           "decode partials", c->retired);
   if (rc != FT_OK) return rc;
-  p.part = static_cast<float*>(part.ptr);
+  p.part = static_cast<float*>(c->part.ptr);
   dim3 grid((unsigned)nsplit, (unsigned)(kv_heads * p.hgroups), (unsigned)batch);
-  kv3_decode_kernel<<<grid, (kDecWarps + 1) * 32, kDecSmem, s>>>(p);
+  if (weights_dev) {
+    p.score_stride = p.nlb * kBlk;
+    const int rs = ensure_ws(c->scores, (size_t)(batch * q_heads * p.score_stride) * 4, s,
+                             "decode scores", c->retired);
+    if (rs != FT_OK) return rs;
+    p.scores = static_cast<float*>(c->scores.ptr);
+    kv3_decode_kernel<true><<<grid, (kDecWarps + 1) * 32, kDecSmem, s>>>(p);
+    FT_LAUNCH_CHECK();
+    const int64_t chunks = ceil_div(p.len, kWeightChunk);
+    FT_CHECK(chunks + p.G < INT32_MAX && kv_heads <= 65535, FT_ERR_UNSUPPORTED,
+             "decode grid too large");
+    dim3 wgrid((unsigned)(chunks + p.G), (unsigned)kv_heads, (unsigned)batch);
+    kv3_weights_kernel<<<wgrid, kD, (unsigned)(2 * p.G * sizeof(float)), s>>>(
+        p, (int)nsplit, (int)chunks, weights_dev, weights_stride, out_dev, signs);
+    FT_LAUNCH_CHECK();
+    return FT_OK;
+  }
+  kv3_decode_kernel<false><<<grid, (kDecWarps + 1) * 32, kDecSmem, s>>>(p);
   FT_LAUNCH_CHECK();
   kv3_combine_kernel<<<(unsigned)(batch * q_heads), kD, 0, s>>>(p.part, (int)nsplit, out_dev,
                                                                   signs);
@@ -1357,8 +1337,8 @@ int launch_decode(ft_ctx* ctx, DecodeParams p, int64_t batch, int64_t kv_heads, 
 
 extern "C" {
 
-int ft_flash_decode_3bit(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads, float scale,
-                         float* out_dev, void* stream) {
+static int ring_decode(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads, float scale,
+                       float* out_dev, float* weights_dev, int64_t weights_stride, void* stream) {
   FT_CHECK(ctx && c && q_dev && out_dev, FT_ERR_SHAPE, "null argument");
   FT_CHECK(q_heads > 0 && q_heads % c->kv_heads == 0, FT_ERR_SHAPE,
            "q_heads (%lld) must be a multiple of kv_heads (%lld)", (long long)q_heads,
@@ -1373,8 +1353,23 @@ int ft_flash_decode_3bit(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_h
   p.head_blk = c->head / kBlk;
   p.len = c->len;
   p.blocks = c->blocks;
-  return launch_decode(ctx, p, c->batch, c->kv_heads, q_heads, c->signs, c->part, c->rot, q_dev,
-                       scale, out_dev, static_cast<cudaStream_t>(stream));
+  return launch_decode(ctx, c, p, c->batch, q_heads, q_dev, scale, out_dev, weights_dev,
+                       weights_stride, static_cast<cudaStream_t>(stream));
+}
+
+int ft_flash_decode_3bit(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads, float scale,
+                         float* out_dev, void* stream) {
+  return ring_decode(ctx, c, q_dev, q_heads, scale, out_dev, nullptr, 0, stream);
+}
+
+int ft_flash_decode_3bit_weights(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads,
+                                 float scale, float* out_dev, float* weights_dev,
+                                 int64_t weights_stride, void* stream) {
+  FT_CHECK(c && weights_dev, FT_ERR_SHAPE, "null argument");
+  FT_CHECK(weights_stride >= c->len, FT_ERR_SHAPE,
+           "weight rows of %lld entries do not hold %lld positions", (long long)weights_stride,
+           (long long)c->len);
+  return ring_decode(ctx, c, q_dev, q_heads, scale, out_dev, weights_dev, weights_stride, stream);
 }
 
 // ---- paged pool
@@ -1414,8 +1409,7 @@ int ft_kvp_destroy(ft_kvp* c) {
   DeviceScope scope(c->device);
   cudaFree(c->blocks);
   if (c->signs) cudaFree(c->signs);
-  if (c->part.ptr) cudaFree(c->part.ptr);
-  if (c->rot.ptr) cudaFree(c->rot.ptr);
+  free_workspaces(c);
   delete c;
   return FT_OK;
 }
@@ -1565,10 +1559,10 @@ int ft_kvp_export_range(ft_ctx* ctx, const ft_kvp* c, int64_t batch, const int32
   return FT_OK;
 }
 
-int ft_kvp_flash_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
+static int paged_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
                         int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
                         const float* q_dev, int64_t q_heads, float scale, float* out_dev,
-                        void* stream) {
+                        float* weights_dev, int64_t weights_stride, void* stream) {
   FT_CHECK(ctx && c && tables_dev && seq_lens_dev && q_dev && out_dev, FT_ERR_SHAPE,
            "null argument");
   FT_CHECK(q_heads > 0 && q_heads % c->kv_heads == 0, FT_ERR_SHAPE,
@@ -1589,8 +1583,29 @@ int ft_kvp_flash_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* ta
   p.seq_lens = seq_lens_dev;
   p.tstride = table_stride;
   p.n_pages = c->n_pages;
-  return launch_decode(ctx, p, batch, c->kv_heads, q_heads, c->signs, c->part, c->rot, q_dev,
-                       scale, out_dev, static_cast<cudaStream_t>(stream));
+  return launch_decode(ctx, c, p, batch, q_heads, q_dev, scale, out_dev, weights_dev,
+                       weights_stride, static_cast<cudaStream_t>(stream));
+}
+
+int ft_kvp_flash_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
+                        int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
+                        const float* q_dev, int64_t q_heads, float scale, float* out_dev,
+                        void* stream) {
+  return paged_decode(ctx, c, batch, tables_dev, table_stride, seq_lens_dev, max_seq_len, q_dev,
+                      q_heads, scale, out_dev, nullptr, 0, stream);
+}
+
+int ft_kvp_flash_decode_weights(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
+                                int64_t table_stride, const int32_t* seq_lens_dev,
+                                int64_t max_seq_len, const float* q_dev, int64_t q_heads,
+                                float scale, float* out_dev, float* weights_dev,
+                                int64_t weights_stride, void* stream) {
+  FT_CHECK(weights_dev, FT_ERR_SHAPE, "null argument");
+  FT_CHECK(weights_stride >= max_seq_len, FT_ERR_SHAPE,
+           "weight rows of %lld entries do not hold %lld positions", (long long)weights_stride,
+           (long long)max_seq_len);
+  return paged_decode(ctx, c, batch, tables_dev, table_stride, seq_lens_dev, max_seq_len, q_dev,
+                      q_heads, scale, out_dev, weights_dev, weights_stride, stream);
 }
 
 }  // extern "C"

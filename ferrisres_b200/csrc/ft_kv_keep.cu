@@ -1,0 +1,526 @@
+// Eviction from the 3-bit KV cache by accumulated attention weight, and the
+// compaction that moves the positions that stay.
+//
+// select_heavy, per (sequence, kv head): of the len positions the n_recent last
+// and the n_keep - n_recent heaviest of the others stay, listed in ascending
+// order; equal weights go to the lowest position, -0 equals 0 and NaN is
+// heavier than everything.  A sequence of at most n_keep positions stays whole.
+//
+// keep, per (sequence, kv head): position start + i := position idx[i], in
+// place, for i < count.  Any list with idx[i] >= start + i is allowed
+// (ascending lists are), so a position is never overwritten before a later one
+// reads it as long as lower positions are written no earlier than higher ones
+// are still to be read: see keep_kernel.
+#include <cooperative_groups.h>
+
+#include "ft_kv3.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace ft {
+namespace {
+
+// ---------------------------------------------------------------- select --
+struct SelectParams {
+  const float* w;      // [B][H] rows of wstride floats
+  float* w_out;        // [B][H] rows of wout_stride floats, or null
+  int32_t* idx;        // [B][H][n_keep]
+  const int32_t* lens;  // [B], or null: every sequence holds len
+  int64_t H, wstride, wout_stride;
+  int64_t len, n_keep, n_recent, out_len;
+  int* err;
+};
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelBins = 2048;
+constexpr int kSelKeys = 40960;  // keys held in shared memory; further ones are read again
+constexpr int kSelSmem = kSelBins * 4 + 4 * 64 * 4;
+
+// Order-preserving key of a weight: larger key = heavier.
+__device__ __forceinline__ uint32_t weight_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);  // -0 -> +0
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// One cluster per (sequence, kv head); each CTA takes a contiguous share of
+// the candidates.  Radix selection of the n-th largest key (11 + 11 + 10 bits,
+// histograms summed over the cluster through distributed shared memory), then
+// one ordered pass that ranks the kept positions.
+__global__ void __launch_bounds__(kSelThreads)
+    select_kernel(const __grid_constant__ SelectParams p, int cap) {
+  extern __shared__ uint32_t ssm[];
+  uint32_t* hist = ssm;              // this CTA's histogram
+  uint32_t* red = ssm + kSelBins;    // [64] warp sums
+  uint32_t* bc = red + 64;           // broadcast values and per-CTA counts
+  uint32_t* keys = bc + 192;         // [cap]
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int64_t row = blockIdx.x / C;
+  const int64_t b = row / p.H;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int64_t len = p.len;
+  if (p.lens) {
+    len = p.lens[b];
+    if (len < 0 || len > p.len) {
+      if (tid == 0) atomicCAS(p.err, 0, 1009);
+      len = len < 0 ? 0 : p.len;
+    }
+  }
+  const float* w = p.w + row * p.wstride;
+  float* wo = p.w_out ? p.w_out + row * p.wout_stride : nullptr;
+  int32_t* idx = p.idx + row * p.n_keep;
+  const int64_t kept = len < p.n_keep ? len : p.n_keep;
+  const int64_t gt0 = (int64_t)rank * kSelThreads + tid, gstep = (int64_t)C * kSelThreads;
+  // entries past the kept positions: no index, no weight
+  for (int64_t i = kept + gt0; i < p.n_keep; i += gstep) idx[i] = -1;
+  if (wo)
+    for (int64_t i = kept + gt0; i < p.out_len; i += gstep) wo[i] = 0.0f;
+  if (len <= p.n_keep) {  // uniform over the cluster
+    for (int64_t i = gt0; i < len; i += gstep) {
+      idx[i] = (int32_t)i;
+      if (wo) wo[i] = w[i];
+    }
+    return;
+  }
+  const int64_t cand = len - p.n_recent, heavy = p.n_keep - p.n_recent;  // 0 <= heavy < cand
+  for (int64_t i = gt0; i < p.n_recent; i += gstep) {
+    idx[heavy + i] = (int32_t)(cand + i);
+    if (wo) wo[heavy + i] = w[cand + i];
+  }
+  if (heavy == 0) return;
+  const int64_t share = (cand + C - 1) / C;
+  const int64_t lo = share * rank < cand ? share * rank : cand;
+  const int n = (int)((lo + share < cand ? lo + share : cand) - lo);
+  const float* wl = w + lo;
+  for (int i = tid; i < n && i < cap; i += kSelThreads) keys[i] = weight_key(wl[i]);
+  auto key_at = [&](int i) { return i < cap ? keys[i] : weight_key(wl[i]); };
+
+  uint32_t prefix = 0, pmask = 0;
+  uint32_t need = (uint32_t)heavy;  // still to be found among keys with this prefix
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const uint32_t bmask = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint32_t k = key_at(i);
+      if ((k & pmask) == prefix) atomicAdd(&hist[(k >> shift) & bmask], 1u);
+    }
+    cl.sync();
+    // thread t owns bins 4t .. 4t+3 of the cluster's histogram
+    uint32_t own[4] = {0, 0, 0, 0}, sum = 0;
+    for (int c = 0; c < C; ++c) {
+      const uint4 v = *reinterpret_cast<const uint4*>(cl.map_shared_rank(hist, c) + 4 * tid);
+      own[0] += v.x;
+      own[1] += v.y;
+      own[2] += v.z;
+      own[3] += v.w;
+    }
+    sum = own[0] + own[1] + own[2] + own[3];
+    // keys in bins above: suffix sums over the threads
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_down_sync(0xffffffffu, inc, o);
+      if (lane + o < 32) inc += u;
+    }
+    if (lane == 0) red[warp] = inc;
+    __syncthreads();
+    uint32_t above = inc - sum;
+    for (int k = warp + 1; k < kSelWarps; ++k) above += red[k];
+    if (above < need && need <= above + sum) {  // exactly one thread
+      int d = 3;
+      while (above + own[d] < need) above += own[d--];
+      bc[0] = (uint32_t)(4 * tid + d);
+      bc[1] = need - above;
+    }
+    cl.sync();  // also: every CTA has read the histograms before they are cleared
+    prefix |= bc[0] << shift;
+    pmask |= bmask << shift;
+    need = bc[1];
+  }
+  // prefix: the key of the lightest kept position; `need` positions that equal
+  // it stay.  Each warp takes a contiguous span of the CTA's share.
+  const int span = (n + kSelWarps - 1) / kSelWarps;
+  const int s0 = warp * span < n ? warp * span : n, s1 = s0 + span < n ? s0 + span : n;
+  uint32_t gt = 0, eq = 0;
+  for (int i = s0 + lane; i < s1; i += 32) {
+    const uint32_t k = key_at(i);
+    gt += k > prefix;
+    eq += k == prefix;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  if (lane == 0) {
+    red[warp] = gt;
+    red[32 + warp] = eq;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t a = 0, e = 0;
+    for (int k = 0; k < kSelWarps; ++k) {
+      a += red[k];
+      e += red[32 + k];
+    }
+    bc[2] = a;
+    bc[3] = e;
+  }
+  cl.sync();
+  uint32_t gt_before = 0, eq_before = 0;
+  for (int c = 0; c < rank; ++c) {
+    gt_before += cl.map_shared_rank(bc, c)[2];
+    eq_before += cl.map_shared_rank(bc, c)[3];
+  }
+  for (int k = 0; k < warp; ++k) {
+    gt_before += red[k];
+    eq_before += red[32 + k];
+  }
+  for (int i0 = s0; i0 < s1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t k = i < s1 ? key_at(i) : 0u;
+    const bool g = i < s1 && k > prefix, e = i < s1 && k == prefix;
+    const uint32_t bg = __ballot_sync(0xffffffffu, g), be = __ballot_sync(0xffffffffu, e);
+    const uint32_t below = (1u << lane) - 1u;
+    const uint32_t er = eq_before + __popc(be & below);
+    if (g || (e && er < need)) {
+      const uint32_t at = gt_before + __popc(bg & below) + (er < need ? er : need);
+      idx[at] = (int32_t)(lo + i);
+      if (wo) wo[at] = wl[i];
+    }
+    gt_before += __popc(bg);
+    eq_before += __popc(be);
+  }
+  cl.sync();  // no CTA leaves while another reads its counts
+}
+
+// ------------------------------------------------------------------ keep --
+struct KeepParams {
+  int64_t H, nbc, head_off, head_blk, len;
+  uint32_t* blocks;
+  const int32_t* idx;  // idx[b * ib + h * ih + i]
+  int64_t ib, ih;
+  int64_t start, count;        // ring; paged: count = the longest list
+  const int32_t* starts;       // paged: per sequence
+  const int32_t* counts;
+  const int32_t* seq_lens;
+  const int32_t* table;
+  int64_t tstride, n_pages;
+  int* err;
+};
+
+constexpr int kKeepWarps = 8;
+
+// One cluster per (sequence, kv head).  Rounds of (CTAs x warps) destination
+// blocks in ascending order: every warp gathers the 32 positions of its block
+// into registers, the cluster meets at a barrier, then the warps write.  A
+// round reads positions at or above its own first one and writes none above its
+// last, so what a later round reads is still in place and what this round reads
+// is read before the barrier.
+// Gathering one slot: its K codes are 4 triples (one a lane r, copied as they
+// are); its V codes are one byte lane of three words in each of 8 lanes and 4
+// triples, 6 bits of 8 x 3, which move to the byte and the half (a) of the
+// destination slot.  Bound by L1 and memory, a block of 3584 bytes in and out.
+__global__ void __launch_bounds__(32 * kKeepWarps, 2)
+    keep_kernel(const __grid_constant__ KeepParams p) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks();
+  const int64_t row = blockIdx.x / C;
+  const int64_t b = row / p.H, h = row % p.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, r = lane & 3;
+  int64_t start = p.start, count = p.count, len = p.len;
+  if (p.table) {
+    start = p.starts[b];
+    count = p.counts[b];
+    len = p.seq_lens[b];
+    // every length is bounded by the table, so that no page index leaves it
+    if (len < 0 || len > p.len || start < 0 || count < 0 || count > p.count ||
+        start + count > len) {
+      if (threadIdx.x == 0) atomicCAS(p.err, 0, 1010);
+      count = 0;
+    }
+  }
+  if (count == 0) return;  // uniform over the cluster
+  const int32_t* idx = p.idx + b * p.ib + h * p.ih;
+  const int64_t off = p.table ? 0 : p.head_off;
+  // record of logical block lb (positions off-shifted), null for a bad page
+  auto record = [&](int64_t lb) -> uint32_t* {
+    if (p.table) {
+      const int64_t pg = checked_page(p.table, b * p.tstride + lb, p.n_pages, p.err, 1011);
+      return pg < 0 ? nullptr : p.blocks + (pg * p.H + h) * kRecWords;
+    }
+    int64_t pb = p.head_blk + lb;
+    if (pb >= p.nbc) pb -= p.nbc;
+    return p.blocks + (row * p.nbc + pb) * kRecWords;
+  };
+  const int64_t blk0 = (start + off) / kBlk, blk1 = (start + count + off + kBlk - 1) / kBlk;
+  const int per = C * kKeepWarps;
+  const int me = (int)cl.block_rank() * kKeepWarps + warp;
+  for (int64_t first = blk0; first < blk1; first += per) {
+    const int64_t lb = first + me;
+    bool write = false;
+    uint32_t kd[12], vd[12];
+    float2 kmd = make_float2(0.0f, 0.0f), vmd = kmd;
+    uint32_t* dst = nullptr;
+    if (lb < blk1) {
+      dst = record(lb);
+      // lane u looks up the source of slot u: itself where the list does not reach
+      const int64_t pos = lb * kBlk + lane - off;
+      int64_t src = pos;
+      if (pos >= start && pos < start + count) {
+        const int64_t s = idx[pos - start];
+        if (s >= pos && s < len) src = s;
+        else atomicCAS(p.err, 0, 1012);  // would overwrite or leave the cache: skipped
+      }
+      const int64_t ss = src + off;
+      const bool moved = src != pos;
+      write = __any_sync(0xffffffffu, moved) && dst != nullptr;
+      if (write) {
+        const uint32_t* mine = moved ? record(ss / kBlk) : dst;
+        const bool bad = mine == nullptr;
+        if (bad) mine = dst;  // reported; the slot keeps what it holds
+        const int slot = bad ? lane : (int)(ss % kBlk);
+        const unsigned long long base = (unsigned long long)mine;
+        kmd = reinterpret_cast<const float2*>(mine + kRecKmm)[mm_index(slot)];
+        vmd = reinterpret_cast<const float2*>(mine + kRecVmm)[mm_index(slot)];
+        // K: lane (g, r) assembles the triples of slots g + 8e
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, g + 8 * e);
+          const int t = __shfl_sync(0xffffffffu, slot, g + 8 * e);
+          const uint32_t* k = rec + (4 * (t & 7) + r) * 12 + 3 * (t >> 3);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) kd[3 * e + i] = k[i];
+        }
+        // V: lane (g, r) assembles slots r + 4a + 8bb, byte bb of its words
+#pragma unroll
+        for (int i = 0; i < 12; ++i) vd[i] = 0;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int bb = 0; bb < 4; ++bb) {
+            const int u = r + 4 * a + 8 * bb;
+            const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, u);
+            const int t = __shfl_sync(0xffffffffu, slot, u);
+            const uint4* v4 =
+                reinterpret_cast<const uint4*>(rec + kRecV + (4 * g + (t & 3)) * 12);
+            uint32_t x[12];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+              const uint4 q = v4[i];
+              x[4 * i] = q.x;
+              x[4 * i + 1] = q.y;
+              x[4 * i + 2] = q.z;
+              x[4 * i + 3] = q.w;
+            }
+            const int sa = (t >> 2) & 1, sb = 8 * (t >> 3);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              // bytes of the three words; half a of a triple (quads 2j + a) is
+              // bits 0-2 (a = 0) or 3-5 (a = 1) of each byte, plus bits 6-7 of
+              // byte 0 or 1 and bit 6 or 7 of byte 2
+              const uint32_t y0 = x[3 * m] >> sb, y1 = x[3 * m + 1] >> sb, y2 = x[3 * m + 2] >> sb;
+              const int f = 3 * sa;
+              const uint32_t lo2 = ((sa ? y1 : y0) >> 6) & 3u, hi1 = (y2 >> (6 + sa)) & 1u;
+              uint32_t z0 = ((y0 >> f) & 7u) << (3 * a);
+              uint32_t z1 = ((y1 >> f) & 7u) << (3 * a);
+              const uint32_t z2 = (((y2 >> f) & 7u) << (3 * a)) | (hi1 << (6 + a));
+              if (a) z1 |= lo2 << 6;
+              else z0 |= lo2 << 6;
+              vd[3 * m] |= z0 << (8 * bb);
+              vd[3 * m + 1] |= z1 << (8 * bb);
+              vd[3 * m + 2] |= z2 << (8 * bb);
+            }
+          }
+      }
+    }
+    cl.sync();
+    if (write) {
+      uint4* k4 = reinterpret_cast<uint4*>(dst + lane * 12);
+      uint4* v4 = reinterpret_cast<uint4*>(dst + kRecV + lane * 12);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        k4[i] = make_uint4(kd[4 * i], kd[4 * i + 1], kd[4 * i + 2], kd[4 * i + 3]);
+        v4[i] = make_uint4(vd[4 * i], vd[4 * i + 1], vd[4 * i + 2], vd[4 * i + 3]);
+      }
+      reinterpret_cast<float2*>(dst + kRecKmm)[mm_index(lane)] = kmd;
+      reinterpret_cast<float2*>(dst + kRecVmm)[mm_index(lane)] = vmd;
+    }
+  }
+}
+
+// CTAs of a cluster (a power of two, at most 8) for `rows` rows of `units`
+// units of work, each CTA taking `per` units at a time: as many as keep every
+// SM busy, and none without work.
+int cluster_size(int num_sms, int64_t rows, int64_t units, int64_t per) {
+  int c = 1;
+  while (c < 8 && rows * c < 2 * num_sms && units > c * per) c *= 2;
+  return c;
+}
+
+template <class Kernel, class... Args>
+int launch_cluster(Kernel kernel, int64_t rows, int cluster, int threads, size_t smem,
+                   cudaStream_t s, Args... args) {
+  FT_CHECK(rows * cluster < INT32_MAX, FT_ERR_UNSUPPORTED, "too many (sequence, head) rows");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * cluster));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  FT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  FT_LAUNCH_CHECK();
+  return FT_OK;
+}
+
+int launch_keep(ft_ctx* ctx, const KeepParams& p, int64_t rows, cudaStream_t s) {
+  const int64_t blocks = ceil_div(p.count, kBlk) + 1;
+  const int c = cluster_size(ctx->num_sms, rows, blocks, kKeepWarps);
+  return launch_cluster(keep_kernel, rows, c, 32 * kKeepWarps, 0, s, p);
+}
+
+}  // namespace
+}  // namespace ft
+
+using namespace ft;
+
+extern "C" {
+
+int ft_kv_select_heavy(ft_ctx* ctx, int64_t batch, int64_t kv_heads, const float* weights_dev,
+                       int64_t weights_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
+                       int64_t n_keep, int64_t n_recent, int32_t* idx_dev, float* weights_out_dev,
+                       int64_t weights_out_stride, void* stream) {
+  FT_CHECK(ctx && weights_dev && idx_dev, FT_ERR_SHAPE, "null argument");
+  FT_CHECK(batch >= 0 && kv_heads > 0 && max_seq_len >= 0 && max_seq_len < INT32_MAX,
+           FT_ERR_SHAPE, "bad selection shape (batch %lld, %lld kv heads, %lld positions)",
+           (long long)batch, (long long)kv_heads, (long long)max_seq_len);
+  FT_CHECK(n_keep > 0 && n_recent >= 0 && n_recent <= n_keep && n_keep < INT32_MAX, FT_ERR_SHAPE,
+           "n_recent (%lld) must lie in [0, n_keep = %lld]", (long long)n_recent,
+           (long long)n_keep);
+  FT_CHECK(weights_stride >= max_seq_len, FT_ERR_SHAPE,
+           "weight rows of %lld entries do not hold %lld positions", (long long)weights_stride,
+           (long long)max_seq_len);
+  const int64_t kept = max_seq_len < n_keep ? max_seq_len : n_keep;
+  if (weights_out_dev) {
+    FT_CHECK(weights_out_stride >= kept, FT_ERR_SHAPE,
+             "weight rows of %lld entries do not hold %lld kept positions",
+             (long long)weights_out_stride, (long long)kept);
+    const int64_t rows = batch * kv_heads;
+    const uintptr_t a = (uintptr_t)weights_dev, o = (uintptr_t)weights_out_dev;
+    FT_CHECK(o + (size_t)(rows * weights_out_stride) * 4 <= a ||
+                 a + (size_t)(rows * weights_stride) * 4 <= o,
+             FT_ERR_SHAPE, "weights_out must not overlap weights");
+  }
+  if (batch == 0) return FT_OK;
+  DeviceScope scope(ctx->device);
+  SelectParams p{};
+  p.w = weights_dev;
+  p.w_out = weights_out_dev;
+  p.idx = idx_dev;
+  p.lens = seq_lens_dev;
+  p.H = kv_heads;
+  p.wstride = weights_stride;
+  p.wout_stride = weights_out_stride;
+  p.len = max_seq_len;
+  p.n_keep = n_keep;
+  p.n_recent = n_recent;
+  p.out_len = weights_out_stride;
+  p.err = ctx->err_word;
+  const int64_t rows = batch * kv_heads;
+  const int c = cluster_size(ctx->num_sms, rows, max_seq_len, 8 * kSelThreads);
+  // keys that do not fit shared memory are read from global memory again
+  const int64_t share = ceil_div(max_seq_len, c);
+  const int cap = (int)(share < kSelKeys ? share : kSelKeys);
+  const size_t smem = kSelSmem + (size_t)cap * 4;
+  static bool opted[64] = {false};  // once per device
+  if (ctx->device >= 64 || !opted[ctx->device]) {
+    FT_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kSelSmem + kSelKeys * 4));
+    if (ctx->device < 64) opted[ctx->device] = true;
+  }
+  return launch_cluster(select_kernel, rows, c, kSelThreads, smem,
+                        static_cast<cudaStream_t>(stream), p, cap);
+}
+
+int ft_kv3_keep(ft_ctx* ctx, ft_kv3* c, int64_t start, int64_t count, const int32_t* idx_dev,
+                int64_t idx_batch_stride, int64_t idx_head_stride, void* stream) {
+  FT_CHECK(ctx && c && (count == 0 || idx_dev), FT_ERR_SHAPE, "null argument");
+  FT_CHECK(start >= 0 && count >= 0 && start + count <= c->len, FT_ERR_SHAPE,
+           "%lld positions from %lld on do not come out of a cache of %lld", (long long)count,
+           (long long)start, (long long)c->len);
+  FT_CHECK(idx_batch_stride >= 0 && idx_head_stride >= 0, FT_ERR_SHAPE, "negative stride");
+  FT_CHECK(c->len < (int64_t)INT32_MAX, FT_ERR_UNSUPPORTED, "cache too long for 32-bit indices");
+  if (count > 0) {
+    DeviceScope scope(c->device);
+    // a full ring whose kept positions would end in the head's own block: two
+    // destination blocks would share one record, so the ring is laid out anew
+    if (c->head % kBlk + start + count > c->cap) {
+      const int rc = kv3_grow(c, c->len, static_cast<cudaStream_t>(stream));
+      if (rc != FT_OK) return rc;
+    }
+    KeepParams p{};
+    p.H = c->kv_heads;
+    p.nbc = c->cap / kBlk;
+    p.head_off = c->head % kBlk;
+    p.head_blk = c->head / kBlk;
+    p.len = c->len;
+    p.blocks = c->blocks;
+    p.idx = idx_dev;
+    p.ib = idx_batch_stride;
+    p.ih = idx_head_stride;
+    p.start = start;
+    p.count = count;
+    p.err = ctx->err_word;
+    const int rc =
+        launch_keep(ctx, p, c->batch * c->kv_heads, static_cast<cudaStream_t>(stream));
+    if (rc != FT_OK) return rc;
+  }
+  c->len = start + count;
+  return FT_OK;
+}
+
+int ft_kvp_keep(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
+                int64_t table_stride, const int32_t* seq_lens_dev, const int32_t* start_dev,
+                const int32_t* count_dev, int64_t max_count, const int32_t* idx_dev,
+                int64_t idx_batch_stride, int64_t idx_head_stride, void* stream) {
+  FT_CHECK(ctx && c && tables_dev && seq_lens_dev && start_dev && count_dev &&
+               (max_count == 0 || idx_dev),
+           FT_ERR_SHAPE, "null argument");
+  FT_CHECK(batch >= 0 && table_stride > 0 && max_count >= 0 &&
+               max_count <= table_stride * kBlk && table_stride < INT32_MAX / kBlk,
+           FT_ERR_SHAPE, "bad shape (batch %lld, %lld positions, table stride %lld)",
+           (long long)batch, (long long)max_count, (long long)table_stride);
+  FT_CHECK(idx_batch_stride >= 0 && idx_head_stride >= 0, FT_ERR_SHAPE, "negative stride");
+  if (batch == 0 || max_count == 0) return FT_OK;
+  DeviceScope scope(c->device);
+  KeepParams p{};
+  p.H = c->kv_heads;
+  p.nbc = 1;
+  p.len = table_stride * kBlk;
+  p.blocks = c->blocks;
+  p.idx = idx_dev;
+  p.ib = idx_batch_stride;
+  p.ih = idx_head_stride;
+  p.count = max_count;
+  p.starts = start_dev;
+  p.counts = count_dev;
+  p.seq_lens = seq_lens_dev;
+  p.table = tables_dev;
+  p.tstride = table_stride;
+  p.n_pages = c->n_pages;
+  p.err = ctx->err_word;
+  return launch_keep(ctx, p, batch * c->kv_heads, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

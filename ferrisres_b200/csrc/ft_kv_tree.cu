@@ -1,0 +1,739 @@
+// Attention of a tree of drafted tokens over the 3-bit KV cache (speculative
+// decoding).  The T <= 64 drafts of a sequence are its last T positions; draft
+// i sees every earlier position (the prefix, P = len - T of them) and the
+// drafts that its mask names:
+//     x[i, s] = scale * q[i] . k[s]   for s < P, or s >= P and bit s - P of mask[i]
+//     out[i]  = sum_s softmax(x[i])_s v[s],   0 for a draft that sees nothing,
+// with k, v = min + code * (max - min) / 7 as stored, and the GQA head map of
+// the single-token decode.  q and out are fp32 or bf16.
+//
+// Mathematics.  Rows of one kv head are its T * G queries (row = draft * G +
+// head in group).  q . k = min * sum(q) + (max - min)/7 * sum(q c): the codes
+// c = 0..7 go to the tensor cores as they are (a 3-bit field is the fp16
+// subnormal c * 2^-24, exact), q as fp16 hi + lo of q * 2^sh (sh puts the row's
+// absmax in [2^14, 2^15); hi alone holds a bf16 q exactly down to 2^-29 of the
+// absmax, hi + lo hold 22 bits of an fp32 q).  Likewise p . v = sum(p min) +
+// sum(p (max - min)/7 c), with w = p (max - min)/7 as fp16 (bf16 q: relative
+// rounding 2^-12, an eighth of the output's own) or fp16 hi + lo (fp32 q: 22
+// bits).  Softmax statistics, min terms and numerators are fp32.  The tensor
+// core truncates its fp32 sums, so it sums 32 positions at most; the blocks'
+// sums are added in fp32 with rounding to nearest.
+// The running reference of a row is M = max(x) - ew, 2^ew being the power of
+// two that keeps w = exp2(x - M) (max - min)/7 below 2^15: l, the min terms and
+// the numerator all carry that factor, so it needs no undoing.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ft_kv3.cuh"
+#include "ft_tc.cuh"
+
+namespace ft {
+namespace {
+
+constexpr int kMaxDraft = 64;       // bits of a mask word
+constexpr int kRows = 16;           // query rows per CTA (one MMA tile)
+constexpr int kTWarps = 4;          // compute warps = 32-slot blocks per tile
+constexpr int kTStages = 4;
+constexpr int kTStageBytes = kTWarps * kRecBytes;
+constexpr int kTPart = 2 + kD;      // partial record: M, l, numerator[128]
+constexpr int kTQfBytes = 8 * 32 * 16;  // q fragments of one term [k-step][lane][16 B]
+constexpr int kTOffQf = kTStages * kTStageBytes;
+constexpr int tree_off_info(int terms) { return kTOffQf + terms * kTQfBytes; }
+constexpr int tree_off_bars(int terms) { return tree_off_info(terms) + kRows * 16; }
+constexpr int tree_smem(int terms) { return tree_off_bars(terms) + 16 * kTStages; }
+constexpr int kTMergeBytes = kTWarps * kRows * (kD + 2) * 4;
+static_assert(kTMergeBytes <= kTStages * kTStageBytes, "the warps merge in the stage buffers");
+
+struct TreeParams {
+  const void* q;  // [B][T][Hq][128], fp32 or bf16
+  int q_bf16;
+  int64_t Hq, Hkv;
+  int G, T, rows, rgroups;  // rows = T * G per kv head, in groups of kRows
+  const uint64_t* mask;     // [B][T], or null: draft i sees drafts 0..i
+  int64_t nbc, head_off, head_blk, len;
+  int64_t nlb;        // logical 32-slot blocks covering the longest sequence
+  int64_t tiles_per;  // 128-slot tiles per split
+  float qk_log2;      // softmax scale * log2(e)
+  const uint32_t* blocks;
+  const float* signs;  // mode T rotation signs, or null
+  float* part;         // [B][Hkv][rows][nsplit][kTPart]
+  int* err;
+  const int32_t* table;  // paged pool, as the single-token decode
+  const int32_t* seq_lens;
+  int64_t tstride, n_pages;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// Codes of bytes (0, 2) (h = 0) or (1, 3) (h = 1) of quad Q of a triple, as two
+// fp16 subnormals c * 2^-24.
+template <int Q, int h>
+__device__ __forceinline__ uint32_t quad_half2(uint32_t w0, uint32_t w1, uint32_t w2) {
+  if (Q < 6) {
+    const uint32_t w = Q < 2 ? w0 : (Q < 4 ? w1 : w2);
+    return (w >> (3 * (Q & 1) + 8 * h)) & 0x00070007u;
+  }
+  if (Q == 6)
+    return ((w0 >> (6 + 8 * h)) & 0x00030003u) | ((w2 >> (4 + 8 * h)) & 0x00040004u);
+  return ((w1 >> (6 + 8 * h)) & 0x00030003u) | ((w2 >> (5 + 8 * h)) & 0x00040004u);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {  // a in the low half
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// Draft tokens of row R (0 <= R < rows): the mask bits of its draft.
+__device__ __forceinline__ uint64_t row_mask(const uint64_t* mask, int64_t b, int T, int t) {
+  const uint64_t all = T == 64 ? ~0ull : (1ull << T) - 1ull;
+  return (mask ? mask[b * T + t] : (2ull << t) - 1ull) & all;
+}
+
+// 128-point Walsh-Hadamard transform of the warp's vector, 4 elements a lane.
+__device__ __forceinline__ void warp_fwht128(float (&v)[4], int lane) {
+  float a = v[0] + v[1], b = v[0] - v[1], c = v[2] + v[3], d = v[2] - v[3];
+  v[0] = a + c;
+  v[1] = b + d;
+  v[2] = a - c;
+  v[3] = b - d;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float u = __shfl_xor_sync(0xffffffffu, v[j], o);
+      v[j] = (lane & o) ? u - v[j] : u + v[j];
+    }
+}
+
+// Query row (4 elements a lane), rotated in mode T; its sum, absmax and sh.
+__device__ __forceinline__ void load_q_row(const TreeParams& p, int64_t b, int64_t kvh, int R,
+                                           int lane, float (&v)[4], float* sum, int* sh) {
+  const int t = R / p.G;
+  const int64_t h = kvh * p.G + (R - t * p.G);
+  const int64_t at = ((b * p.T + t) * p.Hq + h) * kD + 4 * lane;
+  if (p.q_bf16) {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at);
+    v[0] = __uint_as_float(w.x << 16);
+    v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[2] = __uint_as_float(w.y << 16);
+    v[3] = __uint_as_float(w.y & 0xffff0000u);
+  } else {
+    const float4 w = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
+    v[0] = w.x;
+    v[1] = w.y;
+    v[2] = w.z;
+    v[3] = w.w;
+  }
+  if (p.signs) {
+    const float4 sg = reinterpret_cast<const float4*>(p.signs)[lane];
+    v[0] *= sg.x;
+    v[1] *= sg.y;
+    v[2] *= sg.z;
+    v[3] *= sg.w;
+    warp_fwht128(v, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= 0.08838834764831845f;  // 1 / sqrt(128)
+  }
+  float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  float s = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+  // amax * 2^sh in [2^14, 2^15); a non-finite row stays as it is and ends NaN
+  const int e = (int)((__float_as_uint(amax) >> 23) & 255u);
+  *sh = e == 255 ? 0 : min(14 + 127 - e, 120);
+  *sum = s;
+}
+
+// exponent e with v < 2^e for a finite v >= 0, held in [-85, 128]
+__device__ __forceinline__ int bound_exp(float v) {
+  const int e = (int)(__float_as_uint(v) >> 23) - 126;
+  return min(max(e, -85), 128);
+}
+
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <int kTerms>
+__global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
+    tree_decode_kernel(const __grid_constant__ TreeParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint4* qf = reinterpret_cast<const uint4*>(smem + kTOffQf);
+  float* qinfo = reinterpret_cast<float*>(smem + tree_off_info(kTerms));  // sum(q), then scale
+  uint64_t* qmask = reinterpret_cast<uint64_t*>(smem + tree_off_info(kTerms) + kRows * 8);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + tree_off_bars(kTerms));
+  const uint32_t full0 = tc::smem_u32(bars), empty0 = full0 + 8 * kTStages;
+
+  const int split = blockIdx.x;
+  const int64_t kvh = blockIdx.y / p.rgroups;
+  const int R0 = (int)(blockIdx.y % p.rgroups) * kRows;
+  const int64_t b = blockIdx.z;
+  const int64_t row = b * p.Hkv + kvh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, r = lane & 3;
+  int64_t len_b = p.len, nlb_b = p.nlb;
+  if (p.table) {
+    len_b = p.seq_lens[b];
+    if (len_b < 0 || len_b > p.len) {
+      if (tid == 0) atomicCAS(p.err, 0, 1007);
+      len_b = len_b < 0 ? 0 : p.len;
+    }
+    nlb_b = (len_b + kBlk - 1) / kBlk;
+  }
+  const int64_t ntiles_all = (nlb_b + kTWarps - 1) / kTWarps;
+  const int64_t t_begin = (int64_t)split * p.tiles_per;
+  int64_t t_end = t_begin + p.tiles_per;
+  if (t_end > ntiles_all) t_end = ntiles_all;
+  const int ntiles = t_end > t_begin ? (int)(t_end - t_begin) : 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < kTStages; ++s) {
+      tc::mbar_init(full0 + 8 * s, 1);
+      tc::mbar_init(empty0 + 8 * s, kTWarps);
+    }
+    tc::fence_barrier_init();
+  }
+  // q fragments: k-step Q covers dims 16Q .. 16Q+15, its k index 2r, 2r+1 being
+  // dims 4r, 4r+2 and 2r+8, 2r+9 dims 4r+1, 4r+3 (bytes 0, 2 and 1, 3 of a quad)
+  if (warp < kTWarps) {
+    uint32_t* qw = reinterpret_cast<uint32_t*>(smem + kTOffQf);
+    for (int i = warp; i < kRows; i += kTWarps) {
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+      int sh = 0;
+      if (R0 + i < p.rows) load_q_row(p, b, kvh, R0 + i, lane, v, &sum, &sh);
+      const float mul = pow2i(sh);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] *= mul;
+      const int at = ((lane >> 2) * 32 + (i & 7) * 4 + (lane & 3)) * 4 + (i >> 3);
+      const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
+      qw[at] = h0;
+      qw[at + 2] = h1;
+      if (kTerms == 2) {
+        const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+        qw[kTQfBytes / 4 + at] = pack_half2(v[0] - f0.x, v[2] - f0.y);
+        qw[kTQfBytes / 4 + at + 2] = pack_half2(v[1] - f1.x, v[3] - f1.y);
+      }
+      if (lane == 0) {
+        qinfo[i] = sum * p.qk_log2;
+        // undoes 2^sh and the codes' 2^-24 (sh <= 120, so the factor is >= 2^-96)
+        qinfo[kRows + i] = ldexpf(p.qk_log2, 24 - sh);
+        qmask[i] = R0 + i < p.rows ? row_mask(p.mask, b, p.T, (R0 + i) / p.G) : 0ull;
+      }
+    }
+  }
+  __syncthreads();
+
+  const uint32_t stage_base = tc::smem_u32(smem);
+  if (warp == kTWarps) {
+    // ------------------------------------------------------ producer warp --
+    if (lane == 0) {
+      bool ok = true;
+      int issued = 0;
+      int64_t pb = (p.head_blk + t_begin * kTWarps) % p.nbc;
+      for (int it = 0; it < ntiles && ok; ++it) {
+        const int s = it % kTStages;
+        if (it >= kTStages)
+          ok = tc::mbar_wait(empty0 + 8 * s, ((it / kTStages) - 1) & 1, p.err, 41);
+        if (!ok) break;
+        const int64_t j0 = (t_begin + it) * kTWarps;
+        const int nb = nlb_b - j0 < kTWarps ? (int)(nlb_b - j0) : kTWarps;
+        tc::mbar_arrive_expect_tx(full0 + 8 * s, nb * kRecBytes);
+        const uint32_t sb = stage_base + s * kTStageBytes;
+        if (p.table) {
+          for (int i = 0; i < nb; ++i) {  // a bad table entry reads page 0 and is reported
+            int64_t pg = checked_page(p.table, b * p.tstride + j0 + i, p.n_pages, p.err, 1008);
+            if (pg < 0) pg = 0;
+            tc::bulk_g2s(sb + i * kRecBytes, p.blocks + (pg * p.Hkv + kvh) * kRecWords, kRecBytes,
+                         full0 + 8 * s);
+          }
+        } else {
+          const int n1 = pb + nb <= p.nbc ? nb : (int)(p.nbc - pb);
+          tc::bulk_g2s(sb, p.blocks + (row * p.nbc + pb) * kRecWords, n1 * kRecBytes,
+                       full0 + 8 * s);
+          if (n1 < nb)
+            tc::bulk_g2s(sb + n1 * kRecBytes, p.blocks + row * p.nbc * kRecWords,
+                         (nb - n1) * kRecBytes, full0 + 8 * s);
+          pb += nb;
+          if (pb >= p.nbc) pb -= p.nbc;
+        }
+        ++issued;
+      }
+      // the copies of the last stages must land before the CTA may exit
+      for (int it = issued - kTStages < 0 ? 0 : issued - kTStages; it < issued; ++it)
+        tc::mbar_wait(full0 + 8 * (it % kTStages), (it / kTStages) & 1, p.err, 42);
+    }
+    return;
+  }
+
+  // -------------------------------------------------------- compute warps --
+  // rows g and g + 8 of the group (index h); slots r + 4a + 8bb + 16i of a block
+  const float qsum[2] = {qinfo[g], qinfo[g + 8]};
+  const float qscale[2] = {qinfo[kRows + g], qinfo[kRows + g + 8]};
+  float m_run[2] = {-INFINITY, -INFINITY}, Mref[2] = {-INFINITY, -INFINITY};
+  float wbound[2] = {0.0f, 0.0f};
+  float l_part[2] = {0.0f, 0.0f}, vm_part[2] = {0.0f, 0.0f};
+  int ew[2] = {0, 0};
+  float o[16][4];
+#pragma unroll
+  for (int n = 0; n < 16; ++n)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[n][c] = 0.0f;
+  bool ok = true;
+  // 32-bit slot arithmetic: the host keeps head_off + len below 2^31 - 64
+  const int nlb32 = (int)nlb_b, hoff = p.table ? 0 : (int)p.head_off, len32 = (int)len_b;
+  const int P = len32 - p.T;  // prefix length; negative: the first drafts do not exist
+  int j = (int)(t_begin * kTWarps) + warp;
+  for (int it = 0; it < ntiles; ++it, j += kTWarps) {
+    const int s = it % kTStages;
+    if (ok) ok = tc::mbar_wait(full0 + 8 * s, (it / kTStages) & 1, p.err, 43);
+    if (ok && j < nlb32) {
+      const uint32_t* rec =
+          reinterpret_cast<const uint32_t*>(smem + s * kTStageBytes + warp * kRecBytes);
+      // ---- scores.  Column n = g of tile (a, bb) is slot (g >> 1) + 4a + 8bb +
+      // 16 (g & 1), so that a lane's columns 2r, 2r+1 are the slots that its V
+      // words pair in one half2
+      float sc[2][2][4];
+      uint32_t kw[2][6];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint2* kp = reinterpret_cast<const uint2*>(rec + 12 * (4 * ((g >> 1) + 4 * a) + r) +
+                                                         6 * (g & 1));
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint2 x = kp[i];
+          kw[a][2 * i] = x.x;
+          kw[a][2 * i + 1] = x.y;
+        }
+#pragma unroll
+        for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[a][bb][c] = 0.0f;
+      }
+#define FT_TREE_KSTEP(Q)                                                                  \
+  {                                                                                       \
+    const uint4 ah = qf[(Q) * 32 + lane];                                                 \
+    uint4 al;                                                                             \
+    if (kTerms == 2) al = qf[(8 + (Q)) * 32 + lane];                                      \
+    _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) { \
+      const uint32_t b0 = quad_half2<Q, 0>(kw[a][3 * bb], kw[a][3 * bb + 1], kw[a][3 * bb + 2]); \
+      const uint32_t b1 = quad_half2<Q, 1>(kw[a][3 * bb], kw[a][3 * bb + 1], kw[a][3 * bb + 2]); \
+      mma_f16(sc[a][bb], ah, b0, b1);                                                     \
+      if (kTerms == 2) mma_f16(sc[a][bb], al, b0, b1);                                    \
+    }                                                                                     \
+  }
+      FT_TREE_KSTEP(0) FT_TREE_KSTEP(1) FT_TREE_KSTEP(2) FT_TREE_KSTEP(3)
+      FT_TREE_KSTEP(4) FT_TREE_KSTEP(5) FT_TREE_KSTEP(6) FT_TREE_KSTEP(7)
+#undef FT_TREE_KSTEP
+      // ---- x = scale * q . k in the log2 domain; vs, vn: (max - min)/7 and min of V
+      float vs[2][2][2], vn[2][2][2];  // [a][bb][i]
+      const float4* kmm = reinterpret_cast<const float4*>(rec + kRecKmm);
+      const float4* vmm = reinterpret_cast<const float4*>(rec + kRecVmm);
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 km = kmm[(r + 4 * a) * 2 + i], vm = vmm[(r + 4 * a) * 2 + i];
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb) {
+            const float kmin = bb ? km.z : km.x, kmax = bb ? km.w : km.y;
+            const float vmin = bb ? vm.z : vm.x, vmax = bb ? vm.w : vm.y;
+            const float ks = (kmax - kmin) * 0.14285714285714285f;
+            vs[a][bb][i] = (vmax - vmin) * 0.14285714285714285f;
+            vn[a][bb][i] = vmin;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              sc[a][bb][2 * h + i] =
+                  fmaf(kmin, qsum[h], ks * (sc[a][bb][2 * h + i] * qscale[h]));
+          }
+        }
+      const int base = j * kBlk - hoff;
+      // blocks of the prefix are seen whole; the others slot by slot
+      const bool part = base < 0 || base + kBlk > P;
+      float mt[2], vx[2];
+      if (!part) {
+        float v = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mt[h] = -INFINITY;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              v = fmaxf(v, vs[a][bb][i] < INFINITY ? vs[a][bb][i] : 0.0f);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) mt[h] = fmaxf(mt[h], sc[a][bb][2 * h + i]);
+            }
+        vx[0] = vx[1] = v;
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint64_t mask = qmask[g + 8 * h];
+          mt[h] = -INFINITY;
+          vx[h] = 0.0f;
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int bb = 0; bb < 2; ++bb)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int pos = base + r + 4 * a + 8 * bb + 16 * i;
+                const bool sees =
+                    pos >= 0 && pos < len32 && (pos < P || ((mask >> (pos - P)) & 1ull));
+                float& x = sc[a][bb][2 * h + i];
+                x = sees ? x : -INFINITY;
+                mt[h] = fmaxf(mt[h], x);
+                if (sees && vs[a][bb][i] < INFINITY) vx[h] = fmaxf(vx[h], vs[a][bb][i]);
+              }
+        }
+      }
+      // ---- running maximum and reference of the two rows
+      bool grow = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mt[h] = fmaxf(mt[h], __shfl_xor_sync(0xffffffffu, mt[h], 1));
+        mt[h] = fmaxf(mt[h], __shfl_xor_sync(0xffffffffu, mt[h], 2));
+        grow |= mt[h] > m_run[h] || vx[h] >= wbound[h];
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          vx[h] = fmaxf(vx[h], __shfl_xor_sync(0xffffffffu, vx[h], 1));
+          vx[h] = fmaxf(vx[h], __shfl_xor_sync(0xffffffffu, vx[h], 2));
+          if (vx[h] >= wbound[h]) {
+            const int e = bound_exp(vx[h]);
+            ew[h] = 15 - e;
+            wbound[h] = pow2i(e);
+          }
+          m_run[h] = fmaxf(m_run[h], mt[h]);
+          const float Mn = m_run[h] - (float)ew[h];
+          const float alpha = Mref[h] == -INFINITY ? 0.0f : exp2f(Mref[h] - Mn);
+          Mref[h] = Mn;
+          l_part[h] *= alpha;
+          vm_part[h] *= alpha;
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            o[n][2 * h] *= alpha;
+            o[n][2 * h + 1] *= alpha;
+          }
+        }
+      }
+      // ---- weights w = p vs as A fragments of the two 16-slot steps a
+      uint4 ph[2], pl[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float M = Mref[h] == -INFINITY ? 0.0f : Mref[h];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb) {
+            float w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float x = sc[a][bb][2 * h + i];
+              const float pr = exp2f(x - M);
+              l_part[h] += pr;
+              w[i] = pr * vs[a][bb][i];
+              float vmv = pr * vn[a][bb][i];
+              if (part && x == -INFINITY) w[i] = vmv = 0.0f;  // whatever V holds there
+              vm_part[h] += vmv;
+            }
+            const uint32_t hi = pack_half2(w[0], w[1]);
+            // register of the fragment: row half h, k half bb
+            uint32_t& dst = bb ? (h ? ph[a].w : ph[a].z) : (h ? ph[a].y : ph[a].x);
+            dst = hi;
+            if (kTerms == 2) {
+              const float2 f = unpack_half2(hi);
+              uint32_t& dl = bb ? (h ? pl[a].w : pl[a].z) : (h ? pl[a].y : pl[a].x);
+              dl = pack_half2(w[0] - f.x, w[1] - f.y);
+            }
+          }
+      }
+      // ---- P.V: column n = g of n-tile 4m + jj is dim 8 (4m + jj) + g
+      const uint4* vp = reinterpret_cast<const uint4*>(rec + kRecV) + lane * 3;
+      uint32_t vw[12];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint4 x = vp[i];
+        vw[4 * i] = x.x;
+        vw[4 * i + 1] = x.y;
+        vw[4 * i + 2] = x.z;
+        vw[4 * i + 3] = x.w;
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const uint32_t w0 = vw[3 * m], w1 = vw[3 * m + 1], w2 = vw[3 * m + 2];
+#define FT_TREE_VSTEP(JJ)                                                               \
+  {                                                                                     \
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};                                              \
+    const uint32_t b0 = quad_half2<2 * (JJ), 0>(w0, w1, w2);                            \
+    const uint32_t b1 = quad_half2<2 * (JJ), 1>(w0, w1, w2);                            \
+    const uint32_t b2 = quad_half2<2 * (JJ) + 1, 0>(w0, w1, w2);                        \
+    const uint32_t b3 = quad_half2<2 * (JJ) + 1, 1>(w0, w1, w2);                        \
+    mma_f16(t, ph[0], b0, b1);                                                          \
+    mma_f16(t, ph[1], b2, b3);                                                          \
+    if (kTerms == 2) {                                                                  \
+      mma_f16(t, pl[0], b0, b1);                                                        \
+      mma_f16(t, pl[1], b2, b3);                                                        \
+    }                                                                                   \
+    _Pragma("unroll") for (int c = 0; c < 4; ++c) o[4 * m + (JJ)][c] += t[c];           \
+  }
+        FT_TREE_VSTEP(0) FT_TREE_VSTEP(1) FT_TREE_VSTEP(2) FT_TREE_VSTEP(3)
+#undef FT_TREE_VSTEP
+      }
+    }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(empty0 + 8 * s);
+  }
+  // ---- the four warps merge in the stage buffers (every copy has been consumed)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      l_part[h] += __shfl_xor_sync(0xffffffffu, l_part[h], x);
+      vm_part[h] += __shfl_xor_sync(0xffffffffu, vm_part[h], x);
+    }
+    // scores that were all NaN leave no maximum but a NaN sum: keep the row
+    if (Mref[h] == -INFINITY && l_part[h] != l_part[h]) Mref[h] = 0.0f;
+  }
+  asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
+  float* red = reinterpret_cast<float*>(smem);  // [warp][row][2]: M, l
+  float* num = red + kTWarps * kRows * 2;        // [warp][row][128]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = warp * kRows + g + 8 * h;
+    if (r == 0) {
+      red[2 * at] = Mref[h];
+      red[2 * at + 1] = l_part[h];
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+      *reinterpret_cast<float2*>(num + at * kD + 8 * n + 2 * r) =
+          make_float2(fmaf(o[n][2 * h], 16777216.0f, vm_part[h]),
+                      fmaf(o[n][2 * h + 1], 16777216.0f, vm_part[h]));
+  }
+  asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
+  const int nsplit = gridDim.x;
+  for (int i = warp; i < kRows && R0 + i < p.rows; i += kTWarps) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kTWarps; ++w) M = fmaxf(M, red[2 * (w * kRows + i)]);
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kTWarps; ++w) {
+      const int at = w * kRows + i;
+      if (red[2 * at] == -INFINITY) continue;
+      const float f = exp2f(red[2 * at] - M);
+      l = fmaf(f, red[2 * at + 1], l);
+      const float4 v = reinterpret_cast<const float4*>(num + at * kD)[lane];
+      acc[0] = fmaf(f, v.x, acc[0]);
+      acc[1] = fmaf(f, v.y, acc[1]);
+      acc[2] = fmaf(f, v.z, acc[2]);
+      acc[3] = fmaf(f, v.w, acc[3]);
+    }
+    float* pp = p.part + ((row * p.rows + R0 + i) * nsplit + split) * kTPart;
+    if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(M, l);
+    float2* pn = reinterpret_cast<float2*>(pp + 2) + 2 * lane;  // records are 8-byte aligned
+    pn[0] = make_float2(acc[0], acc[1]);
+    pn[1] = make_float2(acc[2], acc[3]);
+  }
+}
+
+// Merges the split partials of one row, one warp a row (4 dims a lane); mode T:
+// the output is rotated back.  Bound by the partials' bytes (520 a split).
+constexpr int kCombineWarps = 4;
+__global__ void __launch_bounds__(32 * kCombineWarps)
+    tree_combine_kernel(const __grid_constant__ TreeParams p, int nsplit, int64_t total,
+                        void* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t R = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
+  if (R >= total) return;
+  const float* pp = p.part + R * nsplit * kTPart;
+  float M = -INFINITY;
+  for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, pp[(int64_t)s * kTPart]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < nsplit; ++s) {
+    const float* ps = pp + (int64_t)s * kTPart;
+    const float2 ml = *reinterpret_cast<const float2*>(ps);
+    const float2 a = reinterpret_cast<const float2*>(ps + 2)[2 * lane];
+    const float2 c = reinterpret_cast<const float2*>(ps + 2)[2 * lane + 1];
+    if (ml.x == -INFINITY) continue;
+    const float f = exp2f(ml.x - M);
+    l = fmaf(f, ml.y, l);
+    v[0] = fmaf(f, a.x, v[0]);
+    v[1] = fmaf(f, a.y, v[1]);
+    v[2] = fmaf(f, c.x, v[2]);
+    v[3] = fmaf(f, c.y, v[3]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : v[k] / l;  // 0: the row saw nothing
+  if (p.signs) {
+    warp_fwht128(v, lane);
+    const float4 sg = reinterpret_cast<const float4*>(p.signs)[lane];
+    v[0] *= 0.08838834764831845f * sg.x;
+    v[1] *= 0.08838834764831845f * sg.y;
+    v[2] *= 0.08838834764831845f * sg.z;
+    v[3] *= 0.08838834764831845f * sg.w;
+  }
+  // row (b, kvh, t, head in group) -> out [b][t][kvh * G + head]
+  const int64_t bk = R / p.rows;
+  const int i = (int)(R % p.rows), t = i / p.G;
+  const int64_t b = bk / p.Hkv, h = (bk % p.Hkv) * p.G + (i - t * p.G);
+  const int64_t at = ((b * p.T + t) * p.Hq + h) * kD + 4 * lane;
+  if (p.q_bf16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
+    uint2 w;
+    w.x = *reinterpret_cast<const uint32_t*>(&x);
+    w.y = *reinterpret_cast<const uint32_t*>(&y);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = w;
+  } else {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) =
+        make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+// Opts the kernels into their dynamic shared memory (once per device) and
+// returns the resident CTAs per SM.
+template <int kTerms>
+int tree_occupancy(int device) {
+  static int cached[64] = {0};
+  if (device >= 0 && device < 64 && cached[device]) return cached[device];
+  cudaFuncSetAttribute(tree_decode_kernel<kTerms>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       tree_smem(kTerms));
+  int occ = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel<kTerms>,
+                                                    (kTWarps + 1) * 32,
+                                                    tree_smem(kTerms)) != cudaSuccess ||
+      occ < 1)
+    occ = 1;
+  if (device >= 0 && device < 64) cached[device] = occ;
+  return occ;
+}
+
+template <class Cache>
+int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_draft,
+                const void* q_dev, int q_is_bf16, int64_t q_heads, const uint64_t* mask_dev,
+                float scale, void* out_dev, cudaStream_t s) {
+  FT_CHECK(q_heads > 0 && q_heads % c->kv_heads == 0, FT_ERR_SHAPE,
+           "q_heads (%lld) must be a multiple of kv_heads (%lld)", (long long)q_heads,
+           (long long)c->kv_heads);
+  FT_CHECK(n_draft > 0, FT_ERR_SHAPE, "no drafts");
+  FT_CHECK(n_draft <= kMaxDraft, FT_ERR_UNSUPPORTED, "%lld drafts: at most %d are supported",
+           (long long)n_draft, kMaxDraft);
+  FT_CHECK(q_heads / c->kv_heads <= 4096, FT_ERR_UNSUPPORTED, "too many q heads per kv head");
+  FT_CHECK(((uintptr_t)q_dev | (uintptr_t)out_dev) % 16 == 0, FT_ERR_SHAPE,
+           "q and out must be 16-byte aligned");
+  p.q = q_dev;
+  p.q_bf16 = q_is_bf16 ? 1 : 0;
+  p.Hq = q_heads;
+  p.Hkv = c->kv_heads;
+  p.G = (int)(q_heads / c->kv_heads);
+  p.T = (int)n_draft;
+  p.rows = p.T * p.G;
+  p.rgroups = (p.rows + kRows - 1) / kRows;
+  p.mask = mask_dev;
+  p.nlb = (p.head_off + p.len + kBlk - 1) / kBlk;
+  const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)kD);
+  p.qk_log2 = sc * 1.4426950408889634f;
+  p.blocks = c->blocks;
+  p.signs = c->signs;
+  p.err = ctx->err_word;
+  // split of the positions: fewest waves x (tiles per CTA + per-CTA overhead)
+  const int64_t units = batch * p.Hkv * p.rgroups;
+  const int64_t ntiles = ceil_div(p.nlb, (int64_t)kTWarps);
+  const int occ = q_is_bf16 ? tree_occupancy<1>(ctx->device) : tree_occupancy<2>(ctx->device);
+  const int64_t resident = (int64_t)occ * ctx->num_sms;
+  int64_t best_cost = INT64_MAX, best_per = ntiles;
+  for (int64_t sp = 1; sp <= 256 && sp <= ntiles; ++sp) {
+    const int64_t per = ceil_div(ntiles, sp);
+    const int64_t waves = ceil_div(units * ceil_div(ntiles, per), resident);
+    const int64_t cost = waves * (per + 2);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best_per = per;
+    }
+  }
+  p.tiles_per = best_per;
+  const int64_t nsplit = ceil_div(ntiles, best_per);
+  FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
+           "decode grid too large");
+  const int64_t total = batch * p.Hkv * p.rows;
+  const int rc = ensure_ws(c->tree, (size_t)(total * nsplit * kTPart) * 4, s, "tree partials",
+                           c->retired);
+  if (rc != FT_OK) return rc;
+  p.part = static_cast<float*>(c->tree.ptr);
+  dim3 grid((unsigned)nsplit, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
+  if (q_is_bf16)
+    tree_decode_kernel<1><<<grid, (kTWarps + 1) * 32, tree_smem(1), s>>>(p);
+  else
+    tree_decode_kernel<2><<<grid, (kTWarps + 1) * 32, tree_smem(2), s>>>(p);
+  FT_LAUNCH_CHECK();
+  tree_combine_kernel<<<(unsigned)ceil_div(total, (int64_t)kCombineWarps), 32 * kCombineWarps, 0,
+                        s>>>(p, (int)nsplit, total, out_dev);
+  FT_LAUNCH_CHECK();
+  return FT_OK;
+}
+
+}  // namespace
+}  // namespace ft
+
+using namespace ft;
+
+extern "C" {
+
+int ft_kv3_tree_decode(ft_ctx* ctx, ft_kv3* c, int64_t n_draft, const void* q_dev, int q_is_bf16,
+                       int64_t q_heads, const uint64_t* mask_dev, float scale, void* out_dev,
+                       void* stream) {
+  FT_CHECK(ctx && c && q_dev && out_dev, FT_ERR_SHAPE, "null argument");
+  FT_CHECK(n_draft <= c->len, FT_ERR_SHAPE, "%lld drafts in a cache of %lld positions",
+           (long long)n_draft, (long long)c->len);
+  FT_CHECK(c->len + kBlk < (int64_t)INT32_MAX - 64, FT_ERR_UNSUPPORTED,
+           "cache too long for the decode's 32-bit slot arithmetic");
+  DeviceScope scope(c->device);
+  TreeParams p{};
+  p.nbc = c->cap / kBlk;
+  p.head_off = c->head % kBlk;
+  p.head_blk = c->head / kBlk;
+  p.len = c->len;
+  return launch_tree(ctx, c, p, c->batch, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
+                     out_dev, static_cast<cudaStream_t>(stream));
+}
+
+int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
+                       int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
+                       int64_t n_draft, const void* q_dev, int q_is_bf16, int64_t q_heads,
+                       const uint64_t* mask_dev, float scale, void* out_dev, void* stream) {
+  FT_CHECK(ctx && c && tables_dev && seq_lens_dev && q_dev && out_dev, FT_ERR_SHAPE,
+           "null argument");
+  FT_CHECK(batch > 0 && max_seq_len > 0 && table_stride > 0 &&
+               max_seq_len <= table_stride * kBlk,
+           FT_ERR_SHAPE, "bad decode shape (batch %lld, max_seq_len %lld, table stride %lld)",
+           (long long)batch, (long long)max_seq_len, (long long)table_stride);
+  FT_CHECK(max_seq_len + kBlk < (int64_t)INT32_MAX - 64, FT_ERR_UNSUPPORTED,
+           "sequence too long for the decode's 32-bit slot arithmetic");
+  DeviceScope scope(c->device);
+  TreeParams p{};
+  p.nbc = 1;
+  p.len = max_seq_len;
+  p.table = tables_dev;
+  p.seq_lens = seq_lens_dev;
+  p.tstride = table_stride;
+  p.n_pages = c->n_pages;
+  return launch_tree(ctx, c, p, batch, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
+                     out_dev, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -25,6 +25,134 @@ from .gpu import _dptr, _stream_ptr, get_context
 
 HEAD_DIM = 128
 REC_BYTES = HEAD_DIM * 3 // 8  # 48
+MAX_DRAFT = 64  # drafts of one tree: the bits of a mask word
+
+
+def tree_mask(parents, device=None) -> torch.Tensor:
+    """Ancestor masks of draft trees for ``tree_decode``: parents [..., n_draft] holds
+    the index of each draft's parent (lower than its own), or -1 for a child of the
+    prefix; bit j of mask[..., i] is set when draft j is i or an ancestor of i.
+    Returns int64 masks on ``device`` (default: the current GPU)."""
+    p = torch.as_tensor(parents).to(device="cpu", dtype=torch.int64)
+    n = p.shape[-1] if p.dim() else 0
+    if not 1 <= n <= MAX_DRAFT:
+        raise ShapeError(f"a tree has 1 to {MAX_DRAFT} drafts")
+    if bool(((p < -1) | (p >= torch.arange(n))).any()):
+        raise ShapeError("a parent is -1 or the index of an earlier draft")
+    m = torch.ones_like(p) << torch.arange(n)
+    for _ in range(6):  # masks of the nearest 2^k ancestors, and the 2^k-th ancestor
+        up = p.clamp(min=0)
+        m = m | torch.where(p >= 0, m.gather(-1, up), 0)
+        p = torch.where(p >= 0, p.gather(-1, up), -1)
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return m.to(device)
+
+
+def _launch_stream(device, stream):
+    """The stream of a call: ``stream``, ordered after what the current one holds (the
+    copies made for the call among it), or the current stream of ``device``."""
+    cur = torch.cuda.current_stream(device)
+    if stream is None:
+        return cur
+    stream.wait_stream(cur)
+    return stream
+
+
+def _used_on(stream, device, *tensors):
+    """Keeps the call's own tensors alive for work on a stream that is not the one they
+    were made on."""
+    if stream != torch.cuda.current_stream(device):
+        for t in tensors:
+            t.record_stream(stream)
+
+
+def _row_stride(t: torch.Tensor, rows: tuple, least: int, what: str, device) -> int:
+    """Distance between the rows of an fp32 tensor [*rows, n >= least] on ``device``
+    whose entries are adjacent and whose rows are equally spaced."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or \
+            t.dim() != 3 or tuple(t.shape[:2]) != tuple(rows) or t.shape[2] < least:
+        raise ShapeError(f"{what} must be fp32 [{rows[0]}, {rows[1]}, >= {least}] on {device}")
+    step = t.stride(1) if rows[1] > 1 else (t.stride(0) if rows[0] > 1 else t.shape[2])
+    if (t.stride(2) != 1 and t.shape[2] > 1) or step < t.shape[2] or \
+            (rows[0] > 1 and t.stride(0) != rows[1] * step):
+        raise ShapeError(f"{what}: rows of adjacent entries, equally spaced, are expected")
+    return step
+
+
+def select_heavy(weights: torch.Tensor, n_keep: int, n_recent: int = 0, length: int | None = None,
+                 seq_lens: torch.Tensor | None = None, stream=None):
+    """The positions that an eviction by accumulated attention weight keeps.
+
+    weights [batch, kv_heads, W] fp32 (``flash_decode(..., weights=...)``); of the first
+    ``length`` (default W) or ``seq_lens[b]`` (int32 [batch] on the device) positions the
+    ``n_recent`` last and the ``n_keep - n_recent`` heaviest of the others stay.  Returns
+    (idx, weights): idx int32 [batch, kv_heads, n_keep], ascending, -1 where a sequence
+    has fewer positions; a new weights tensor of the same shape with the kept
+    positions' weights in front and zeros behind."""
+    if weights.dim() != 3 or not weights.is_cuda:
+        raise ShapeError("weights must be fp32 [batch, kv_heads, positions] on a GPU")
+    B, H, W = weights.shape
+    length = W if length is None else int(length)
+    dev = weights.device
+    step = _row_stride(weights, (B, H), length, "weights", dev)
+    if seq_lens is not None and (seq_lens.dtype != torch.int32 or seq_lens.device != dev or
+                                 tuple(seq_lens.shape) != (B,)):
+        raise ShapeError(f"seq_lens must be int32 [{B}] on {dev}")
+    n_keep, n_recent = int(n_keep), int(n_recent)
+    if n_keep < 1 or not 0 <= n_recent <= n_keep:
+        raise ShapeError("0 <= n_recent <= n_keep and n_keep >= 1 are expected")
+    idx = torch.empty((B, H, n_keep), dtype=torch.int32, device=dev)
+    out = torch.empty((B, H, W), dtype=torch.float32, device=dev)
+    if B == 0:
+        return idx, out
+    lens = None if seq_lens is None else seq_lens.contiguous()
+    s = _launch_stream(dev, stream)
+    call("ft_kv_select_heavy", get_context(dev.index).handle, B, H, C.c_void_p(weights.data_ptr()),
+         step, None if lens is None else _dptr(lens), length, n_keep, n_recent, _dptr(idx),
+         _dptr(out), W, _stream_ptr(s))
+    _used_on(s, dev, weights, idx, out, *([] if lens is None else [lens]))
+    return idx, out
+
+
+def _index_list(idx: torch.Tensor, batch: int, kv_heads: int, device):
+    """int32 index lists [n], [batch, n] or [batch, kv_heads, n] and their strides."""
+    if not isinstance(idx, torch.Tensor) or idx.device != device or \
+            idx.dtype not in (torch.int32, torch.int64):
+        raise ShapeError(f"idx must be an int32 or int64 tensor on {device}")
+    n = idx.shape[-1] if idx.dim() else 0
+    if tuple(idx.shape) not in ((n,), (batch, n), (batch, kv_heads, n)) or idx.dim() == 0:
+        raise ShapeError(f"idx must be [n], [{batch}, n] or [{batch}, {kv_heads}, n]")
+    if idx.dtype == torch.int64:  # no wrap-around: what does not fit stays out of range
+        idx = idx.clamp(-1, 2**31 - 1).to(torch.int32)
+    idx = idx.contiguous()
+    return idx, n, {1: (0, 0), 2: (n, 0), 3: (kv_heads * n, n)}[idx.dim()]
+
+
+def _tree_args(q: torch.Tensor, mask, batch: int, device, out):
+    """Checked q, mask and out of a tree decode: q [batch, n_draft, q_heads, 128]."""
+    if not isinstance(q, torch.Tensor) or q.device != device or q.dim() != 4 or \
+            q.dtype not in (torch.float32, torch.bfloat16) or q.shape[0] != batch or \
+            q.shape[3] != HEAD_DIM:
+        raise ShapeError(f"q must be fp32 or bf16 [{batch}, n_draft, q_heads, {HEAD_DIM}] "
+                         f"on {device}")
+    T = q.shape[1]
+    if not 1 <= T <= MAX_DRAFT:
+        raise UnsupportedError(f"{T} drafts: 1 to {MAX_DRAFT} are supported")
+    q = q.contiguous()
+    if q.data_ptr() % 16:  # a view that starts inside a row of its storage
+        q = q.clone()
+    if mask is not None:
+        if mask.device != device or mask.dtype != torch.int64 or \
+                tuple(mask.shape) not in ((T,), (batch, T)):
+            raise ShapeError(f"mask must be int64 [{T}] or [{batch}, {T}] on {device}")
+        mask = mask.expand(batch, T).contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or \
+            not out.is_contiguous() or out.data_ptr() % 16:
+        raise ShapeError("out must be contiguous, 16-byte aligned and like q")
+    return q, mask, out
 
 
 class Kv3Cache:
@@ -135,18 +263,80 @@ class Kv3Cache:
         return kc, km, vc, vm
 
     def flash_decode(self, q: torch.Tensor, scale: float = 0.0, out: torch.Tensor | None = None,
-                     stream=None) -> torch.Tensor:
+                     stream=None, weights: torch.Tensor | None = None) -> torch.Tensor:
         """q [batch, q_heads, 128] fp32 -> out [batch, q_heads, 128] fp32 over the whole
-        cache; scale 0 selects 1/sqrt(128)."""
+        cache; scale 0 selects 1/sqrt(128).  ``weights`` [batch, kv_heads, >= len] fp32:
+        each position's attention weight, summed over the q heads of its kv head, is
+        added to it (see ``evict_heavy``); the output is the same with and without."""
         if q.dtype != torch.float32 or q.dim() != 3 or q.shape[0] != self.batch or \
                 q.shape[2] != HEAD_DIM:
             raise ShapeError("q must be fp32 [batch, q_heads, 128]")
         q = q.contiguous()
+        if weights is not None:
+            return self._decode_weights(q, scale, out, stream, weights)
         if out is None:
             out = torch.empty_like(q)
         call("ft_flash_decode_3bit", self.ctx.handle, self.handle, _dptr(q), int(q.shape[1]),
              float(scale), _dptr(out), _stream_ptr(stream))
         return out
+
+    def _decode_weights(self, q, scale, out, stream, weights):
+        if q.device != self.device:
+            raise ShapeError(f"q must be on {self.device}")
+        step = _row_stride(weights, (self.batch, self.kv_heads), len(self), "weights", self.device)
+        if out is None:
+            out = torch.empty_like(q)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
+            raise ShapeError("out must be like q")
+        s = _launch_stream(self.device, stream)
+        call("ft_flash_decode_3bit_weights", self.ctx.handle, self.handle, _dptr(q),
+             int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
+             _stream_ptr(s))
+        _used_on(s, self.device, q, out, weights)
+        return out
+
+    def tree_decode(self, q: torch.Tensor, mask: torch.Tensor | None = None, scale: float = 0.0,
+                    out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Attention of drafted tokens: the last n_draft (1..64) positions of the cache are
+        the drafts (append them first).  q [batch, n_draft, q_heads, 128] fp32 or bf16 ->
+        out of the same type; draft i sees all earlier positions and the drafts named by
+        the bits of mask[b, i] (int64 [batch, n_draft] or [n_draft], see ``tree_mask``;
+        None: drafts 0..i).  A draft that sees nothing gets 0."""
+        q, mask, out = _tree_args(q, mask, self.batch, self.device, out)
+        s = _launch_stream(self.device, stream)
+        call("ft_kv3_tree_decode", self.ctx.handle, self.handle, int(q.shape[1]), _dptr(q),
+             int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
+             float(scale), _dptr(out), _stream_ptr(s))
+        _used_on(s, self.device, q, out, *([] if mask is None else [mask]))
+        return out
+
+    # ---- choosing what stays
+    def keep(self, idx: torch.Tensor, start: int = 0, stream=None) -> None:
+        """Positions below ``start`` and the listed ones stay, the rest is dropped: new
+        position start + i is old position idx[..., i] for each sequence and kv head
+        (idx [n], [batch, n] or [batch, kv_heads, n], ascending from ``start`` on).  After
+        a tree decode: the accepted path.  An entry outside [start + i, len) is skipped
+        and reported by ``ctx.check()``."""
+        idx, n, (ib, ih) = _index_list(idx, self.batch, self.kv_heads, self.device)
+        self._keep(idx, n, ib, ih, int(start), stream)
+
+    def _keep(self, idx, n, ib, ih, start, stream):
+        s = _launch_stream(self.device, stream)
+        call("ft_kv3_keep", self.ctx.handle, self.handle, start, n, _dptr(idx), ib, ih,
+             _stream_ptr(s))
+        _used_on(s, self.device, idx)
+
+    def evict_heavy(self, weights: torch.Tensor, n_keep: int, n_recent: int = 0, stream=None):
+        """Evicts down to ``n_keep`` positions per sequence and kv head: the ``n_recent``
+        last and the heaviest of the others by accumulated attention ``weights``
+        [batch, kv_heads, >= len] stay (``select_heavy``).  Returns (idx, weights): the
+        kept old positions and the weights that belong to the new ones."""
+        n = len(self)
+        _row_stride(weights, (self.batch, self.kv_heads), n, "weights", self.device)
+        idx, out = select_heavy(weights, n_keep, n_recent, length=n, stream=stream)
+        if n > int(n_keep):
+            self._keep(idx, int(n_keep), self.kv_heads * int(n_keep), int(n_keep), 0, stream)
+        return idx, out
 
     def close(self):
         if getattr(self, "handle", None):

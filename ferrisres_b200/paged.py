@@ -25,6 +25,7 @@ import torch
 
 from ._lib import OOMError, ShapeError, call
 from .gpu import _dptr, _stream_ptr, get_context
+from .kv import (_index_list, _launch_stream, _row_stride, _tree_args, _used_on, select_heavy)
 
 DEFAULT_BLOCK_SIZE = 16   # the reference's default (paged_attention.rs:21)
 PAGE_POSITIONS = 32       # positions per device page
@@ -399,10 +400,157 @@ class PagedKv3Cache:
             if layer == 0:
                 self._state(r).add_tokens(n_pos)
 
+    def append_packed(self, layer: int, request_ids, k_codes, k_minmax, v_codes, v_minmax,
+                      stream=None):
+        """Appends positions already in the reference's stored form: codes uint8
+        [len(request_ids), n_pos, kv_heads*48], (min, max) fp32 [.., n_pos, kv_heads, 2]."""
+        rids = list(request_ids)
+        if len(set(rids)) != len(rids):
+            raise ShapeError("a request may appear once per append")
+        tens = [t.contiguous() for t in (k_codes, k_minmax, v_codes, v_minmax)]
+        n_pos = int(tens[0].shape[1]) if tens[0].dim() == 3 else -1
+        for t, dtype, shape in zip(tens, (torch.uint8, torch.float32) * 2,
+                                   ((len(rids), n_pos, self.kv_heads * REC_BYTES),
+                                    (len(rids), n_pos, self.kv_heads, 2)) * 2):
+            if t.dtype != dtype or tuple(t.shape) != shape or t.device != self.device:
+                raise ShapeError("codes must be uint8 [requests, n_pos, kv_heads*48] and min/max "
+                                 "fp32 [requests, n_pos, kv_heads, 2] on the cache's device")
+        if n_pos == 0 or not rids:
+            return
+        copies = []
+        starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
+        s = _launch_stream(self.device, stream)
+        self._copy_pages(copies, s)
+        tables, stride = self._tables(layer, rids)
+        start_dev = torch.from_numpy(starts).to(self.device)
+        s = _launch_stream(self.device, stream)
+        call("ft_kvp_append_packed", self.ctx.handle, self.handle, len(rids), n_pos,
+             _dptr(tables), stride, _dptr(start_dev), *[_dptr(t) for t in tens], _stream_ptr(s))
+        _used_on(s, self.device, tables, start_dev, *tens)
+        for r in rids:
+            self._grow_by(layer, r, n_pos)
+
+    def _copy_pages(self, copies, s):
+        if copies:
+            src = np.array([c[0] for c in copies], np.int32)
+            dst = np.array([c[1] for c in copies], np.int32)
+            call("ft_kvp_copy_pages", self.ctx.handle, self.handle, len(copies),
+                 src.ctypes.data_as(C.c_void_p), dst.ctypes.data_as(C.c_void_p), _stream_ptr(s))
+
+    def _grow_by(self, layer, rid, n):
+        st = self._state(rid)
+        st.layer_table(layer).add_tokens(n)
+        if layer == 0:
+            st.add_tokens(n)
+
+    def tree_decode(self, layer: int, request_ids, q: torch.Tensor,
+                    mask: torch.Tensor | None = None, scale: float = 0.0,
+                    out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Attention of drafted tokens, the last n_draft positions of each request in
+        ``layer``: q [len(request_ids), n_draft, q_heads, 128] fp32 or bf16 -> out of the
+        same type (see ``Kv3Cache.tree_decode``)."""
+        rids = list(request_ids)
+        q, mask, out = _tree_args(q, mask, len(rids), self.device, out)
+        if not rids:
+            return out
+        lens = np.array([self.seq_len(r, layer) for r in rids], np.int32)
+        if lens.min() < q.shape[1]:
+            raise ShapeError(f"{q.shape[1]} drafts in a request of {lens.min()} positions")
+        tables, stride = self._tables(layer, rids)
+        lens_dev = torch.from_numpy(lens).to(self.device)
+        s = _launch_stream(self.device, stream)
+        call("ft_kvp_tree_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
+             _dptr(lens_dev), int(lens.max()), int(q.shape[1]), _dptr(q),
+             int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
+             float(scale), _dptr(out), _stream_ptr(s))
+        _used_on(s, self.device, tables, lens_dev, q, out, *([] if mask is None else [mask]))
+        return out
+
+    def keep(self, layer: int, request_ids, idx: torch.Tensor, counts=None, starts=None,
+             stream=None) -> None:
+        """Keeps chosen positions of each request in ``layer``: new position starts[i] + j is
+        old position idx[i, ..., j] for j < counts[i] (idx [n], [requests, n] or
+        [requests, kv_heads, n]; counts default n, starts 0, host integers), the rest is
+        dropped and its pages are freed.  A page that a fork shares is copied first."""
+        rids = list(request_ids)
+        if len(set(rids)) != len(rids):
+            raise ShapeError("a request may appear once per call")
+        idx, n, (ib, ih) = _index_list(idx, len(rids), self.kv_heads, self.device)
+        counts = [n] * len(rids) if counts is None else [int(x) for x in counts]
+        starts = [0] * len(rids) if starts is None else [int(x) for x in starts]
+        self._keep(layer, rids, idx, n, ib, ih, counts, starts, stream)
+
+    def _keep(self, layer, rids, idx, n, ib, ih, counts, starts, stream):
+        if len(counts) != len(rids) or len(starts) != len(rids):
+            raise ShapeError("one count and one start per request are expected")
+        lens = [self.seq_len(r, layer) for r in rids]
+        for c, st, length in zip(counts, starts, lens):
+            if not (0 <= c <= n and 0 <= st and st + c <= length):
+                raise ShapeError(f"{c} positions from {st} on do not come out of a list of {n} "
+                                 f"and a request of {length}")
+        if not rids:
+            return
+        # private copies of the shared pages that the call writes
+        alloc = self.manager.allocator
+        tabs = [self._state(r).layer_table(layer).table() for r in rids]
+        writes = [(t, j) for t, c, st in zip(tabs, counts, starts) if c
+                  for j in range(st // PAGE_POSITIONS, -(-(st + c) // PAGE_POSITIONS))]
+        shared = [(t, j) for t, j in writes if alloc.ref_count(t[j]) > 1]
+        if len(shared) > alloc.num_free():
+            raise OOMError(f"page pool exhausted: {len(shared)} shared pages to copy, "
+                           f"{alloc.num_free()} free")
+        copies = []
+        for t, j in shared:
+            if alloc.ref_count(t[j]) == 1:  # its other owners have moved off in this call
+                continue
+            old, t[j] = t[j], alloc.allocate()
+            copies.append((old, t[j]))
+            alloc.free(old)
+        s = _launch_stream(self.device, stream)
+        self._copy_pages(copies, s)
+        if max(counts) > 0:
+            tables, stride = self._tables(layer, rids)
+            meta = torch.from_numpy(np.array([lens, starts, counts], np.int32)).to(self.device)
+            s = _launch_stream(self.device, stream)
+            call("ft_kvp_keep", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
+                 _dptr(meta[0]), _dptr(meta[1]), _dptr(meta[2]), max(counts), _dptr(idx), ib, ih,
+                 _stream_ptr(s))
+            _used_on(s, self.device, tables, meta, idx)
+        for r, t, c, st, length in zip(rids, tabs, counts, starts, lens):
+            need = -(-(st + c) // PAGE_POSITIONS)
+            while len(t) > need:
+                alloc.free(t.pop())
+            self._grow_by(layer, r, st + c - length)
+
+    def evict_heavy(self, layer: int, request_ids, weights: torch.Tensor, n_keep: int,
+                    n_recent: int = 0, stream=None):
+        """Evicts each request down to ``n_keep`` positions per kv head by accumulated
+        attention ``weights`` [len(request_ids), kv_heads, >= longest] (see
+        ``Kv3Cache.evict_heavy``); shorter requests stay whole.  Returns (idx, weights)."""
+        rids = list(request_ids)
+        if len(set(rids)) != len(rids):
+            raise ShapeError("a request may appear once per call")
+        lens = [self.seq_len(r, layer) for r in rids]
+        longest = max(lens, default=0)
+        _row_stride(weights, (len(rids), self.kv_heads), longest, "weights", self.device)
+        lens_dev = torch.tensor(lens, dtype=torch.int32).to(self.device)
+        idx, out = select_heavy(weights, n_keep, n_recent, length=longest, seq_lens=lens_dev,
+                                stream=stream)
+        n = int(n_keep)
+        over = [x > n for x in lens]
+        if any(over):
+            self._keep(layer, rids, idx, n, self.kv_heads * n, n,
+                       [n if o else 0 for o in over], [0 if o else x for o, x in zip(over, lens)],
+                       stream)
+        return idx, out
+
     def flash_decode(self, layer: int, request_ids, q: torch.Tensor, scale: float = 0.0,
-                     out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, stream=None,
+                     weights: torch.Tensor | None = None) -> torch.Tensor:
         """q [len(request_ids), q_heads, 128] fp32 -> softmax attention over
-        each request's positions in ``layer`` (ragged lengths)."""
+        each request's positions in ``layer`` (ragged lengths).  ``weights``
+        [len(request_ids), kv_heads, >= longest] fp32: each position's attention weight,
+        summed over the q heads of its kv head, is added to it."""
         rids = list(request_ids)
         if q.dim() != 3 or q.shape[0] != len(rids) or q.shape[2] != HEAD_DIM or \
                 q.dtype != torch.float32 or q.device != self.device:
@@ -418,9 +566,20 @@ class PagedKv3Cache:
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
         if stream is not None:
             stream.wait_stream(torch.cuda.current_stream(self.device))
-        call("ft_kvp_flash_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables),
-             stride, _dptr(lens_dev), int(lens.max()), _dptr(q), int(q.shape[1]), float(scale),
-             _dptr(out), _stream_ptr(s))
+        if weights is not None:
+            step = _row_stride(weights, (len(rids), self.kv_heads), int(lens.max()), "weights",
+                               self.device)
+            if out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
+                raise ShapeError("out must be like q")
+            call("ft_kvp_flash_decode_weights", self.ctx.handle, self.handle, len(rids),
+                 _dptr(tables), stride, _dptr(lens_dev), int(lens.max()), _dptr(q),
+                 int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
+                 _stream_ptr(s))
+            _used_on(s, self.device, q, out, weights)
+        else:
+            call("ft_kvp_flash_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables),
+                 stride, _dptr(lens_dev), int(lens.max()), _dptr(q), int(q.shape[1]),
+                 float(scale), _dptr(out), _stream_ptr(s))
         tables.record_stream(s)
         lens_dev.record_stream(s)
         return out

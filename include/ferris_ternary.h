@@ -377,6 +377,51 @@ int ft_kv3_export_range(ft_ctx* ctx, const ft_kv3* c, int64_t start, int64_t end
 int ft_flash_decode_3bit(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads, float scale,
                          float* out_dev, void* stream);
 
+/* Flash decode that also accumulates attention weight: weights[b, hk, s] +=
+ * sum over the q heads h of kv head hk of softmax_s(scale * q[b, h] . K[b, s, hk]),
+ * for every position s.  weights_dev: [batch, kv_heads] rows of weights_stride >=
+ * seq_len floats; entries past the last position are left alone.  out equals
+ * ft_flash_decode_3bit's bit for bit.  No counterpart in the reference, whose
+ * eviction is by age only (turboquant_kv.rs:308-328). */
+int ft_flash_decode_3bit_weights(ft_ctx* ctx, ft_kv3* c, const float* q_dev, int64_t q_heads,
+                                 float scale, float* out_dev, float* weights_dev,
+                                 int64_t weights_stride, void* stream);
+/* Attention of a tree of drafted tokens (speculative decoding; no counterpart
+ * in the reference).  The last n_draft (1..64) positions of each sequence are
+ * its drafts, appended before the call.  Draft i sees every earlier position
+ * and the drafts j whose bit j of mask_dev[b, i] is set (itself included only
+ * if its own bit is); mask_dev null: drafts 0..i.  Bits past n_draft are
+ * ignored.  q, out [batch, n_draft, q_heads, 128], fp32 or (q_is_bf16) bf16 bit
+ * patterns, 16-byte aligned; scale <= 0 selects 1/sqrt(128).  A draft that sees
+ * nothing gets 0; what masked positions hold, infinities and NaN included, has
+ * no effect.  A q row with a NaN or an infinity gives NaN in that row only.
+ * fp32: about 1e-6 of the exact result; bf16: the output's own rounding. */
+int ft_kv3_tree_decode(ft_ctx* ctx, ft_kv3* c, int64_t n_draft, const void* q_dev, int q_is_bf16,
+                       int64_t q_heads, const uint64_t* mask_dev, float scale, void* out_dev,
+                       void* stream);
+/* Eviction by accumulated weight: of each row's positions the n_recent last and
+ * the n_keep - n_recent heaviest of the others (equal weights: the lowest
+ * position first; -0 equals 0; NaN counts as heaviest), as ascending positions
+ * idx[b, hk, 0..n_keep).  weights_dev: [batch, kv_heads] rows of weights_stride
+ * floats; seq_lens_dev: int32 [batch] on the device, or null when every
+ * sequence holds max_seq_len positions.  A sequence of at most n_keep positions
+ * stays whole; its unused entries of idx are -1.  weights_out_dev (optional, not
+ * overlapping weights_dev): [batch, kv_heads] rows of weights_out_stride floats
+ * that receive the weights of the kept positions, then zeros. */
+int ft_kv_select_heavy(ft_ctx* ctx, int64_t batch, int64_t kv_heads, const float* weights_dev,
+                       int64_t weights_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
+                       int64_t n_keep, int64_t n_recent, int32_t* idx_dev, float* weights_out_dev,
+                       int64_t weights_out_stride, void* stream);
+/* Keeps chosen positions, in place: for every sequence b and kv head hk position
+ * start + i becomes position idx_dev[b * idx_batch_stride + hk * idx_head_stride
+ * + i] (stride 0: one list for all), i < count; positions below start stay, and
+ * the cache's length becomes start + count.  Each entry must lie in
+ * [start + i, seq_len), as every ascending list of positions from start on does;
+ * another entry is skipped and reported by ft_ctx_check (FT_ERR_SHAPE).  The
+ * length is host state: a captured call repeats the move only. */
+int ft_kv3_keep(ft_ctx* ctx, ft_kv3* c, int64_t start, int64_t count, const int32_t* idx_dev,
+                int64_t idx_batch_stride, int64_t idx_head_stride, void* stream);
+
 /* ---- paged 3-bit KV cache: the GPU storage behind PagedAttention
  * (src/inference/paged_attention.rs).  The reference keeps only the metadata
  * there -- BlockAllocator (:44-150) hands out block ids, a BlockTable (:158-224)
@@ -433,6 +478,29 @@ int ft_kvp_flash_decode(ft_ctx* ctx, ft_kvp* pool, int64_t batch, const int32_t*
                         int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
                         const float* q_dev, int64_t q_heads, float scale, float* out_dev,
                         void* stream);
+/* The paged forms of the operators above.  weights_dev has a row of
+ * weights_stride >= max_seq_len floats for each (row b of the call, kv head). */
+int ft_kvp_flash_decode_weights(ft_ctx* ctx, ft_kvp* pool, int64_t batch,
+                                const int32_t* tables_dev, int64_t table_stride,
+                                const int32_t* seq_lens_dev, int64_t max_seq_len,
+                                const float* q_dev, int64_t q_heads, float scale, float* out_dev,
+                                float* weights_dev, int64_t weights_stride, void* stream);
+/* seq_lens[b] counts the drafts; a sequence shorter than n_draft has only the
+ * last seq_lens[b] of them (an empty one gives 0 everywhere). */
+int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* pool, int64_t batch, const int32_t* tables_dev,
+                       int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
+                       int64_t n_draft, const void* q_dev, int q_is_bf16, int64_t q_heads,
+                       const uint64_t* mask_dev, float scale, void* out_dev, void* stream);
+/* Sequence b keeps count_dev[b] <= max_count positions from start_dev[b] on
+ * (int32 on the device; start + count <= seq_lens[b], otherwise the sequence is
+ * skipped and reported).  The pages from start on must belong to that sequence
+ * alone (copy shared ones first: ft_kvp_copy_pages), and the block tables and
+ * lengths stay the caller's to update.  max_seq_len of the tables is
+ * table_stride pages. */
+int ft_kvp_keep(ft_ctx* ctx, ft_kvp* pool, int64_t batch, const int32_t* tables_dev,
+                int64_t table_stride, const int32_t* seq_lens_dev, const int32_t* start_dev,
+                const int32_t* count_dev, int64_t max_count, const int32_t* idx_dev,
+                int64_t idx_batch_stride, int64_t idx_head_stride, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -92,6 +92,10 @@ extern "C" {
     pub fn ft_kv3_get_range(ctx: *mut ft_ctx, c: *const ft_kv3, start: i64, end: i64, k_out_dev: *mut f32, v_out_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_kv3_export_range(ctx: *mut ft_ctx, c: *const ft_kv3, start: i64, end: i64, k_codes_dev: *mut u8, k_minmax_dev: *mut f32, v_codes_dev: *mut u8, v_minmax_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_flash_decode_3bit(ctx: *mut ft_ctx, c: *mut ft_kv3, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ft_flash_decode_3bit_weights(ctx: *mut ft_ctx, c: *mut ft_kv3, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, weights_dev: *mut f32, weights_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn ft_kv3_tree_decode(ctx: *mut ft_ctx, c: *mut ft_kv3, n_draft: i64, q_dev: *const c_void, q_is_bf16: c_int, q_heads: i64, mask_dev: *const u64, scale: f32, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ft_kv_select_heavy(ctx: *mut ft_ctx, batch: i64, kv_heads: i64, weights_dev: *const f32, weights_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, n_keep: i64, n_recent: i64, idx_dev: *mut i32, weights_out_dev: *mut f32, weights_out_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn ft_kv3_keep(ctx: *mut ft_ctx, c: *mut ft_kv3, start: i64, count: i64, idx_dev: *const i32, idx_batch_stride: i64, idx_head_stride: i64, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_create(ctx: *mut ft_ctx, num_pages: i64, kv_heads: i64, head_dim: i64, page_size: i64, mode: c_int, seed: u64, out: *mut *mut ft_kvp) -> c_int;
     pub fn ft_kvp_destroy(pool: *mut ft_kvp) -> c_int;
     pub fn ft_kvp_signs(pool: *const ft_kvp, signs_host: *mut f32) -> c_int;
@@ -101,4 +105,7 @@ extern "C" {
     pub fn ft_kvp_get_range(ctx: *mut ft_ctx, pool: *const ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, start: i64, end: i64, k_out_dev: *mut f32, v_out_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_export_range(ctx: *mut ft_ctx, pool: *const ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, start: i64, end: i64, k_codes_dev: *mut u8, k_minmax_dev: *mut f32, v_codes_dev: *mut u8, v_minmax_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_flash_decode(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ft_kvp_flash_decode_weights(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, weights_dev: *mut f32, weights_stride: i64, stream: *mut c_void) -> c_int;
+    pub fn ft_kvp_tree_decode(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, n_draft: i64, q_dev: *const c_void, q_is_bf16: c_int, q_heads: i64, mask_dev: *const u64, scale: f32, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ft_kvp_keep(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, start_dev: *const i32, count_dev: *const i32, max_count: i64, idx_dev: *const i32, idx_batch_stride: i64, idx_head_stride: i64, stream: *mut c_void) -> c_int;
 }
