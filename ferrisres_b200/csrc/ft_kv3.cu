@@ -827,8 +827,9 @@ __global__ void __launch_bounds__((kDecWarps + 1) * 32, FT_KV_MIN_BLOCKS)
     l_part += __shfl_xor_sync(0xffffffffu, l_part, o2);
     vmin_part += __shfl_xor_sync(0xffffffffu, vmin_part, o2);
   }
-  // ---- combine the 4 warps through shared memory (the stage buffers are
-  // free: every issued copy has been consumed)
+  // ---- combine the 4 warps through shared memory: the stage buffers, once
+  // every warp has read its last block out of them
+  asm volatile("bar.sync 1, %0;" ::"r"(kDecWarps * 32) : "memory");
   float* red = reinterpret_cast<float*>(smem);  // [warp][head][4]
   if (g == 0) {
     red[(warp * 4 + r) * 4 + 0] = m_run;

@@ -81,6 +81,21 @@ def test_weights(kv, case, mode):
     c.close()
 
 
+def test_decode_repeats_bit_for_bit(kv):
+    """The warps of a split merge in the stage buffers: none may write there while a slower one
+    still reads its block.  Short splits make the warps end far apart."""
+    g = generator(20)
+    for n in (1000, 8190):
+        c = kv.Kv3Cache(4, 8, n)
+        x = rand(g, 4, n, 8, D)
+        c.append(x, x)
+        q = rand(g, 4, 32, D)
+        ref = c.flash_decode(q)
+        for _ in range(300):
+            assert torch.equal(c.flash_decode(q), ref)
+        c.close()
+
+
 def test_weights_in_strided_rows_and_moved_ring(kv):
     g = generator(3)
     c = kv.Kv3Cache(2, 2, 128)
