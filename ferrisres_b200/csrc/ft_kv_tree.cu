@@ -8,19 +8,25 @@
 // the single-token decode.  q and out are fp32 or bf16.
 //
 // Mathematics.  Rows of one kv head are its T * G queries (row = draft * G +
-// head in group).  q . k = min * sum(q) + (max - min)/7 * sum(q c): the codes
-// c = 0..7 go to the tensor cores as they are (a 3-bit field is the fp16
-// subnormal c * 2^-24, exact), q as fp16 hi + lo of q * 2^sh (sh puts the row's
-// absmax in [2^14, 2^15); hi alone holds a bf16 q exactly down to 2^-29 of the
-// absmax, hi + lo hold 22 bits of an fp32 q).  Likewise p . v = sum(p min) +
-// sum(p (max - min)/7 c), with w = p (max - min)/7 as fp16 (bf16 q: relative
-// rounding 2^-12, an eighth of the output's own) or fp16 hi + lo (fp32 q: 22
-// bits).  Softmax statistics, min terms and numerators are fp32.  The tensor
-// core truncates its fp32 sums, so it sums 32 positions at most; the blocks'
-// sums are added in fp32 with rounding to nearest.
+// head in group).  A code c = 0..7 becomes the fp16 1 + c/8 by two bit
+// operations (the code is its leading mantissa bits) or, one subtraction later,
+// (c - 3.5)/8, exactly either way:
+//     k = (min - 8 st) + 8 st (1 + c/8) = (min + 3.5 st) + 8 st (c - 3.5)/8,
+// st = (max - min)/7, so q . k is a multiple of sum(q) plus 8 st times a product
+// of fp16 matrices.  q enters as fp16 hi + lo of q * 2^sh (sh puts the row's
+// absmax in [2^14, 2^15)): hi alone holds a bf16 q exactly down to 2^-29 of the
+// absmax, hi + lo hold 22 bits of an fp32 q.  p . v likewise: w = p st as fp16
+// (bf16 q: relative rounding 2^-12, an eighth of the output's own) or fp16 hi +
+// lo (fp32 q).  The centred form keeps the products' sums near zero, where the
+// two parts of v do not cancel; the scores of a bf16 q do without it.  (As
+// fp16 subnormals the codes would cost one operation less, but the tensor core
+// aligns a product by the operands' exponents and drops the low bits: 2^-12 of
+// the result were lost.)  Softmax statistics, the sum terms and numerators are
+// fp32; the tensor core truncates its fp32 sums, so it sums 32 positions at
+// most, and the blocks' sums are added with rounding to nearest.
 // The running reference of a row is M = max(x) - ew, 2^ew being the power of
-// two that keeps w = exp2(x - M) (max - min)/7 below 2^15: l, the min terms and
-// the numerator all carry that factor, so it needs no undoing.
+// two that keeps w = exp2(x - M) st below 2^15: l, the sum terms and the
+// numerator all carry that factor, so it needs no undoing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -72,16 +78,28 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t 
 }
 
 // Codes of bytes (0, 2) (h = 0) or (1, 3) (h = 1) of quad Q of a triple, as two
-// fp16 subnormals c * 2^-24.
+// fp16 values 1 + c/8: the field moves to mantissa bits 7..9.
+template <int kLeft>
+__device__ __forceinline__ uint32_t shifted(uint32_t w) {
+  return kLeft >= 0 ? w << (kLeft < 0 ? 0 : kLeft) : w >> (kLeft < 0 ? -kLeft : 0);
+}
 template <int Q, int h>
 __device__ __forceinline__ uint32_t quad_half2(uint32_t w0, uint32_t w1, uint32_t w2) {
+  constexpr uint32_t kOne = 0x3C003C00u;
   if (Q < 6) {
     const uint32_t w = Q < 2 ? w0 : (Q < 4 ? w1 : w2);
-    return (w >> (3 * (Q & 1) + 8 * h)) & 0x00070007u;
+    return (shifted<7 - 3 * (Q & 1) - 8 * h>(w) & 0x03800380u) | kOne;
   }
-  if (Q == 6)
-    return ((w0 >> (6 + 8 * h)) & 0x00030003u) | ((w2 >> (4 + 8 * h)) & 0x00040004u);
-  return ((w1 >> (6 + 8 * h)) & 0x00030003u) | ((w2 >> (5 + 8 * h)) & 0x00040004u);
+  // low two bits from bits 6, 7 of word 0 or 1, the high one from bit Q of word 2
+  const uint32_t lo = (shifted<1 - 8 * h>(Q == 6 ? w0 : w1) & 0x01800180u) | kOne;
+  return (shifted<9 - Q - 8 * h>(w2) & 0x02000200u) | lo;
+}
+// the same centred: (c - 3.5) / 8
+template <int Q, int h>
+__device__ __forceinline__ uint32_t quad_centred(uint32_t w0, uint32_t w1, uint32_t w2) {
+  uint32_t v;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(quad_half2<Q, h>(w0, w1, w2)), "r"(0x3DC03DC0u));
+  return v;
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {  // a in the low half
@@ -114,9 +132,9 @@ __device__ __forceinline__ void warp_fwht128(float (&v)[4], int lane) {
     }
 }
 
-// Query row (4 elements a lane), rotated in mode T; its sum, absmax and sh.
+// Query row (4 elements a lane), rotated in mode T, and its sh.
 __device__ __forceinline__ void load_q_row(const TreeParams& p, int64_t b, int64_t kvh, int R,
-                                           int lane, float (&v)[4], float* sum, int* sh) {
+                                           int lane, float (&v)[4], int* sh) {
   const int t = R / p.G;
   const int64_t h = kvh * p.G + (R - t * p.G);
   const int64_t at = ((b * p.T + t) * p.Hq + h) * kD + 4 * lane;
@@ -144,16 +162,11 @@ __device__ __forceinline__ void load_q_row(const TreeParams& p, int64_t b, int64
     for (int j = 0; j < 4; ++j) v[j] *= 0.08838834764831845f;  // 1 / sqrt(128)
   }
   float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-  float s = (v[0] + v[1]) + (v[2] + v[3]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-  }
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   // amax * 2^sh in [2^14, 2^15); a non-finite row stays as it is and ends NaN
   const int e = (int)((__float_as_uint(amax) >> 23) & 255u);
   *sh = e == 255 ? 0 : min(14 + 127 - e, 120);
-  *sum = s;
 }
 
 // exponent e with v < 2^e for a finite v >= 0, held in [-85, 128]
@@ -208,9 +221,9 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
   if (warp < kTWarps) {
     uint32_t* qw = reinterpret_cast<uint32_t*>(smem + kTOffQf);
     for (int i = warp; i < kRows; i += kTWarps) {
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       int sh = 0;
-      if (R0 + i < p.rows) load_q_row(p, b, kvh, R0 + i, lane, v, &sum, &sh);
+      if (R0 + i < p.rows) load_q_row(p, b, kvh, R0 + i, lane, v, &sh);
       const float mul = pow2i(sh);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] *= mul;
@@ -218,15 +231,22 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
       const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
       qw[at] = h0;
       qw[at + 2] = h1;
+      const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+      float sum = (f0.x + f0.y) + (f1.x + f1.y);  // of the q that the products take
       if (kTerms == 2) {
-        const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-        qw[kTQfBytes / 4 + at] = pack_half2(v[0] - f0.x, v[2] - f0.y);
-        qw[kTQfBytes / 4 + at + 2] = pack_half2(v[1] - f1.x, v[3] - f1.y);
+        const uint32_t l0 = pack_half2(v[0] - f0.x, v[2] - f0.y);
+        const uint32_t l1 = pack_half2(v[1] - f1.x, v[3] - f1.y);
+        qw[kTQfBytes / 4 + at] = l0;
+        qw[kTQfBytes / 4 + at + 2] = l1;
+        const float2 d0 = unpack_half2(l0), d1 = unpack_half2(l1);
+        sum += (d0.x + d0.y) + (d1.x + d1.y);
       }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       if (lane == 0) {
-        qinfo[i] = sum * p.qk_log2;
-        // undoes 2^sh and the codes' 2^-24 (sh <= 120, so the factor is >= 2^-96)
-        qinfo[kRows + i] = ldexpf(p.qk_log2, 24 - sh);
+        // scores = (k's constant part * sum + st * product * 8) * 2^-sh * scale
+        qinfo[i] = sum * ldexpf(p.qk_log2, -sh);
+        qinfo[kRows + i] = ldexpf(p.qk_log2, 3 - sh);
         qmask[i] = R0 + i < p.rows ? row_mask(p.mask, b, p.T, (R0 + i) / p.G) : 0ull;
       }
     }
@@ -325,8 +345,9 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
     uint4 al;                                                                             \
     if (kTerms == 2) al = qf[(8 + (Q)) * 32 + lane];                                      \
     _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) { \
-      const uint32_t b0 = quad_half2<Q, 0>(kw[a][3 * bb], kw[a][3 * bb + 1], kw[a][3 * bb + 2]); \
-      const uint32_t b1 = quad_half2<Q, 1>(kw[a][3 * bb], kw[a][3 * bb + 1], kw[a][3 * bb + 2]); \
+      const uint32_t w0 = kw[a][3 * bb], w1 = kw[a][3 * bb + 1], w2 = kw[a][3 * bb + 2];  \
+      const uint32_t b0 = kTerms == 2 ? quad_centred<Q, 0>(w0, w1, w2) : quad_half2<Q, 0>(w0, w1, w2); \
+      const uint32_t b1 = kTerms == 2 ? quad_centred<Q, 1>(w0, w1, w2) : quad_half2<Q, 1>(w0, w1, w2); \
       mma_f16(sc[a][bb], ah, b0, b1);                                                     \
       if (kTerms == 2) mma_f16(sc[a][bb], al, b0, b1);                                    \
     }                                                                                     \
@@ -334,7 +355,7 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
       FT_TREE_KSTEP(0) FT_TREE_KSTEP(1) FT_TREE_KSTEP(2) FT_TREE_KSTEP(3)
       FT_TREE_KSTEP(4) FT_TREE_KSTEP(5) FT_TREE_KSTEP(6) FT_TREE_KSTEP(7)
 #undef FT_TREE_KSTEP
-      // ---- x = scale * q . k in the log2 domain; vs, vn: (max - min)/7 and min of V
+      // ---- x = scale * q . k in the log2 domain; vs, vn: st and the constant part of V
       float vs[2][2][2], vn[2][2][2];  // [a][bb][i]
       const float4* kmm = reinterpret_cast<const float4*>(rec + kRecKmm);
       const float4* vmm = reinterpret_cast<const float4*>(rec + kRecVmm);
@@ -349,11 +370,12 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
             const float vmin = bb ? vm.z : vm.x, vmax = bb ? vm.w : vm.y;
             const float ks = (kmax - kmin) * 0.14285714285714285f;
             vs[a][bb][i] = (vmax - vmin) * 0.14285714285714285f;
-            vn[a][bb][i] = vmin;
+            vn[a][bb][i] = fmaf(3.5f, vs[a][bb][i], vmin);
+            const float kc = fmaf(kTerms == 2 ? 3.5f : -8.0f, ks, kmin);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               sc[a][bb][2 * h + i] =
-                  fmaf(kmin, qsum[h], ks * (sc[a][bb][2 * h + i] * qscale[h]));
+                  fmaf(kc, qsum[h], ks * (sc[a][bb][2 * h + i] * qscale[h]));
           }
         }
       const int base = j * kBlk - hoff;
@@ -476,10 +498,10 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 #define FT_TREE_VSTEP(JJ)                                                               \
   {                                                                                     \
     float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};                                              \
-    const uint32_t b0 = quad_half2<2 * (JJ), 0>(w0, w1, w2);                            \
-    const uint32_t b1 = quad_half2<2 * (JJ), 1>(w0, w1, w2);                            \
-    const uint32_t b2 = quad_half2<2 * (JJ) + 1, 0>(w0, w1, w2);                        \
-    const uint32_t b3 = quad_half2<2 * (JJ) + 1, 1>(w0, w1, w2);                        \
+    const uint32_t b0 = quad_centred<2 * (JJ), 0>(w0, w1, w2);                            \
+    const uint32_t b1 = quad_centred<2 * (JJ), 1>(w0, w1, w2);                            \
+    const uint32_t b2 = quad_centred<2 * (JJ) + 1, 0>(w0, w1, w2);                        \
+    const uint32_t b3 = quad_centred<2 * (JJ) + 1, 1>(w0, w1, w2);                        \
     mma_f16(t, ph[0], b0, b1);                                                          \
     mma_f16(t, ph[1], b2, b3);                                                          \
     if (kTerms == 2) {                                                                  \
@@ -519,8 +541,8 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 #pragma unroll
     for (int n = 0; n < 16; ++n)
       *reinterpret_cast<float2*>(num + at * kD + 8 * n + 2 * r) =
-          make_float2(fmaf(o[n][2 * h], 16777216.0f, vm_part[h]),
-                      fmaf(o[n][2 * h + 1], 16777216.0f, vm_part[h]));
+          make_float2(fmaf(o[n][2 * h], 8.0f, vm_part[h]),
+                      fmaf(o[n][2 * h + 1], 8.0f, vm_part[h]));
   }
   asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
   const int nsplit = gridDim.x;
