@@ -95,9 +95,9 @@ static_assert(kQdBytes <= kOsmBytes, "q digits are staged in the numerator area"
 
 // ---------------------------------------------------------------- append --
 struct AppendParams {
-  const void* k;  // kPacked: reference bytes [B][n][Hkv*48]; else values [B][n][Hkv][128]
+  const void* k;  // packed: reference bytes [B][n][Hkv*48]; else values [B][n][Hkv][128]
   const void* v;
-  const float* kmm_in;  // kPacked only: [B][n][Hkv][2]
+  const float* kmm_in;  // packed only: [B][n][Hkv][2]
   const float* vmm_in;
   int bf16;
   int64_t n_pos, Hkv, cap, nbc, s0;
@@ -151,20 +151,8 @@ __device__ __forceinline__ uint32_t kvt_code(float x, float sign, int d, float* 
   return c <= 0.0f ? 0u : (c >= 7.0f ? 7u : (uint32_t)c);
 }
 
-// code idx of a reference LSB-first 3-bit stream (the next byte is read only
-// when the code straddles it)
-__device__ __forceinline__ uint32_t ref_stream_code(const uint8_t* bytes, int64_t idx) {
-  const int64_t bit = 3 * idx;
-  const int64_t by = bit >> 3;
-  uint32_t w = bytes[by];
-  if ((bit & 7) > 5) w |= (uint32_t)bytes[by + 1] << 8;
-  return (w >> (bit & 7)) & 7u;
-}
-
 // One CTA per (32-slot block touched, row); thread = dim.  Quantises each new
-// position of the block (or takes its codes from a reference byte stream),
-// and rewrites the block's K and V words and min/max.
-template <bool kPacked>
+// position of the block and rewrites the block's K and V words and min/max.
 __global__ void __launch_bounds__(kD) kv3_append_kernel(AppendParams p) {
   const int64_t x = blockIdx.x, row = blockIdx.y;
   const int64_t b = row / p.Hkv, h = row % p.Hkv;
@@ -205,17 +193,7 @@ __global__ void __launch_bounds__(kD) kv3_append_kernel(AppendParams p) {
     const int64_t vec = (b * p.n_pos + pi) * p.Hkv + h;
     uint32_t ck, cv;
     float kmin, kmax, vmin, vmax;
-    if (kPacked) {
-      const int64_t rowbytes = p.Hkv * kRec;
-      const uint8_t* kb = static_cast<const uint8_t*>(p.k) + (b * p.n_pos + pi) * rowbytes;
-      const uint8_t* vb = static_cast<const uint8_t*>(p.v) + (b * p.n_pos + pi) * rowbytes;
-      ck = ref_stream_code(kb, h * kD + d);
-      cv = ref_stream_code(vb, h * kD + d);
-      kmin = p.kmm_in[vec * 2];
-      kmax = p.kmm_in[vec * 2 + 1];
-      vmin = p.vmm_in[vec * 2];
-      vmax = p.vmm_in[vec * 2 + 1];
-    } else if (p.signs) {
+    if (p.signs) {
       // mode T: norm, signs, Walsh-Hadamard, uniform codebook
       const float xk = load_act(p.k, vec * kD + d, p.bf16);
       const float xv = load_act(p.v, vec * kD + d, p.bf16);
@@ -272,6 +250,164 @@ __global__ void __launch_bounds__(kD) kv3_append_kernel(AppendParams p) {
   for (int i = d; i < kBlkWords; i += kD) {
     kg[i] = kw[i];
     vg[i] = vw[i];
+  }
+}
+
+// Appends positions given in the reference's stored form: one warp per (block
+// touched, row), warps of a CTA on neighbouring kv heads (neighbouring bytes of
+// the input).  Each lane brings the 48 + 48 bytes of one slot to shared memory,
+// then assembles the 12 K and 12 V words that are its own (lane 4g + r):
+//   K triple of slot s: quad Q's four codes are bits 48Q + 12r .. +11 of s's stream;
+//   V triple m of slots r + 4a + 8b: quad 2j + a, byte b is bits 24(4m + j) + 3g ..
+//   +2 of the stream of slot r + 4a + 8b.
+// Slots outside the appended range keep their bits.  About 1100 integer
+// operations a lane and block, in the shadow of its 3584 bytes in and out.
+constexpr int kMoveWarps = 4;
+__device__ __forceinline__ uint32_t spread12(uint32_t f) {  // four 3-bit codes to four bytes
+  return (f & 7u) | (f & 0x38u) << 5 | (f & 0x1C0u) << 10 | (f & 0xE00u) << 15;
+}
+
+// 48 bytes of a stream as 12 words; vec: the address is 16-byte aligned
+__device__ __forceinline__ void load_stream(const uint8_t* src, bool vec, uint32_t (&w)[12]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(src)[i];
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 12; ++i)
+      w[i] = src[4 * i] | src[4 * i + 1] << 8 | src[4 * i + 2] << 16 | (uint32_t)src[4 * i + 3] << 24;
+  }
+}
+
+__global__ void __launch_bounds__(32 * kMoveWarps)
+    kv3_append_packed_kernel(AppendParams p, int64_t nblk, int64_t total) {
+  __shared__ __align__(16) uint32_t stage[kMoveWarps][2][kBlkWords];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kMoveWarps + warp;
+  if (unit >= total) return;
+  const int64_t h = unit % p.Hkv, x = unit / p.Hkv % nblk, b = unit / (p.Hkv * nblk);
+  const int64_t row = b * p.Hkv + h;
+  const int64_t s0 = p.table ? (int64_t)p.pos0[b] : p.s0;
+  const int64_t off0 = s0 % kBlk;
+  const int u_begin = x == 0 ? (int)off0 : 0;
+  const int64_t u_end64 = p.n_pos + off0 - x * kBlk;
+  const int u_end = u_end64 > kBlk ? kBlk : (int)u_end64;
+  if (u_begin >= u_end) return;  // paged: this sequence touches fewer blocks
+  int64_t rec;
+  if (p.table) {
+    const int64_t lb = s0 / kBlk + x;
+    if (s0 < 0 || lb >= p.tstride) {
+      if (lane == 0) atomicCAS(p.err, 0, 1001);
+      return;
+    }
+    const int64_t pg = checked_page(p.table, b * p.tstride + lb, p.n_pages, p.err, 1002);
+    if (pg < 0) return;
+    rec = pg * p.Hkv + h;
+  } else {
+    rec = row * p.nbc + (s0 / kBlk + x) % p.nbc;
+  }
+  uint32_t* kg = p.blocks + rec * kRecWords;
+  uint32_t* vg = kg + kRecV;
+  const bool live = lane >= u_begin && lane < u_end;
+  uint32_t w[12];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int i = 0; i < 12; ++i) w[i] = 0;
+    const int64_t vec = (b * p.n_pos + x * kBlk + lane - off0) * p.Hkv + h;
+    if (live) {
+      const uint8_t* src = static_cast<const uint8_t*>(t ? p.v : p.k);
+      load_stream(src + vec * kRec, ((uintptr_t)src & 15) == 0, w);
+      const float* mm = (t ? p.vmm_in : p.kmm_in) + vec * 2;
+      reinterpret_cast<float2*>(kg + (t ? kRecVmm : kRecKmm))[mm_index(lane)] =
+          make_float2(mm[0], mm[1]);
+    }
+    uint4* st = reinterpret_cast<uint4*>(stage[warp][t] + lane * 12);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) st[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+  __syncwarp();
+  const int g = lane >> 2, r = lane & 3;
+  const bool whole = u_begin == 0 && u_end == kBlk;
+  uint4* k4 = reinterpret_cast<uint4*>(kg + lane * 12);
+  uint4* v4 = reinterpret_cast<uint4*>(vg + lane * 12);
+  uint32_t kd[12], vd[12];
+#pragma unroll
+  for (int i = 0; i < 12; ++i) kd[i] = vd[i] = 0;
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint4 a = k4[i], c = v4[i];
+      kd[4 * i] = a.x, kd[4 * i + 1] = a.y, kd[4 * i + 2] = a.z, kd[4 * i + 3] = a.w;
+      vd[4 * i] = c.x, vd[4 * i + 1] = c.y, vd[4 * i + 2] = c.z, vd[4 * i + 3] = c.w;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int u = g + 8 * e;
+    if (u < u_begin || u >= u_end) continue;
+    const uint32_t* src = stage[warp][0] + u * 12;
+    uint32_t s[12];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint4 q = reinterpret_cast<const uint4*>(src)[i];
+      s[4 * i] = q.x, s[4 * i + 1] = q.y, s[4 * i + 2] = q.z, s[4 * i + 3] = q.w;
+    }
+    uint32_t q[8];
+#pragma unroll
+    for (int Q = 0; Q < 8; ++Q) {
+      const int base = 3 * (Q >> 1) + (Q & 1);  // word of bit 48Q
+      const uint64_t v = s[base] | (uint64_t)s[base + 1] << 32;
+      q[Q] = spread12((uint32_t)(v >> (16 * (Q & 1) + 12 * r)) & 0xFFFu);
+    }
+    kd[3 * e] = q[0] | q[1] << 3 | (q[6] & 0x03030303u) << 6;
+    kd[3 * e + 1] = q[2] | q[3] << 3 | (q[7] & 0x03030303u) << 6;
+    kd[3 * e + 2] = q[4] | q[5] << 3 | (q[6] & 0x04040404u) << 4 | (q[7] & 0x04040404u) << 5;
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int bb = 0; bb < 4; ++bb) {
+      const int u = r + 4 * a + 8 * bb;
+      if (u < u_begin || u >= u_end) continue;
+      const uint4* src = reinterpret_cast<const uint4*>(stage[warp][1] + u * 12);
+      uint32_t s[12];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint4 q = src[i];
+        s[4 * i] = q.x, s[4 * i + 1] = q.y, s[4 * i + 2] = q.z, s[4 * i + 3] = q.w;
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        // the four 24-bit groups 4m + j of the stream
+        const uint32_t w0 = s[3 * m], w1 = s[3 * m + 1], w2 = s[3 * m + 2];
+        const uint32_t c0 = (w0 >> (3 * g)) & 7u;
+        const uint32_t c1 = (__byte_perm(w0, w1, 0x6543) >> (3 * g)) & 7u;
+        const uint32_t c2 = (__byte_perm(w1, w2, 0x5432) >> (3 * g)) & 7u;
+        const uint32_t c3 = (w2 >> (8 + 3 * g)) & 7u;
+        const uint32_t z0 = c0 << (3 * a) | (a ? 0u : (c3 & 3u) << 6);
+        const uint32_t z1 = c1 << (3 * a) | (a ? (c3 & 3u) << 6 : 0u);
+        const uint32_t z2 = c2 << (3 * a) | (c3 >> 2) << (6 + a);
+        if (!whole) {  // clear what the slot held
+          vd[3 * m] &= ~((a ? 0x38u : 0xC7u) << (8 * bb));
+          vd[3 * m + 1] &= ~((a ? 0xF8u : 0x07u) << (8 * bb));
+          vd[3 * m + 2] &= ~((a ? 0xB8u : 0x47u) << (8 * bb));
+        }
+        vd[3 * m] |= z0 << (8 * bb);
+        vd[3 * m + 1] |= z1 << (8 * bb);
+        vd[3 * m + 2] |= z2 << (8 * bb);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    k4[i] = make_uint4(kd[4 * i], kd[4 * i + 1], kd[4 * i + 2], kd[4 * i + 3]);
+    v4[i] = make_uint4(vd[4 * i], vd[4 * i + 1], vd[4 * i + 2], vd[4 * i + 3]);
   }
 }
 
@@ -361,40 +497,115 @@ __global__ void kv3_rotate_kernel(const float* __restrict__ in, float* __restric
 }
 
 // The reference's stored form: codes [B][n][Hkv*48] bytes (pack_3bit over the
-// whole kv_dim vector) and (min, max) [B][n][Hkv][2].  Thread = 8 codes.
-__global__ void kv3_export_kernel(RangeParams p, uint8_t* __restrict__ kbytes,
-                                  float* __restrict__ kmm_out, uint8_t* __restrict__ vbytes,
-                                  float* __restrict__ vmm_out) {
-  const int64_t vec = blockIdx.x;  // (b, pos, h)
-  const int m = threadIdx.x;       // 0..15: codes 8m..8m+7
-  const int64_t h = vec % p.Hkv;
-  const int64_t pos = (vec / p.Hkv) % p.n;
-  const int64_t b = vec / (p.Hkv * p.n);
-  int s;
-  const uint32_t* kb = range_record(p, b, h, pos, &s);
-  if (!kb) return;
-  const uint32_t* vb = kb + kRecV;
-  uint32_t kbits = 0, vbits = 0;
+// whole kv_dim vector) and (min, max) [B][n][Hkv][2].  One warp per (block of
+// the range, row), warps of a CTA on neighbouring kv heads; the record is read
+// into shared memory once and lane u rebuilds slot u's two streams from it
+// (the maps of kv3_append_packed_kernel, backwards).
+__global__ void __launch_bounds__(32 * kMoveWarps)
+    kv3_export_kernel(RangeParams p, int64_t nblk, int64_t total, uint8_t* __restrict__ kbytes,
+                      float* __restrict__ kmm_out, uint8_t* __restrict__ vbytes,
+                      float* __restrict__ vmm_out) {
+  __shared__ __align__(16) uint32_t stage[kMoveWarps][kRecWords];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kMoveWarps + warp;
+  if (unit >= total) return;
+  const int64_t h = unit % p.Hkv, x = unit / p.Hkv % nblk, b = unit / (p.Hkv * nblk);
+  const int64_t off = p.table ? 0 : p.head % kBlk;
+  const int64_t lb = (p.start + off) / kBlk + x;  // logical block
+  const int64_t pos = lb * kBlk + lane - off - p.start;  // of lane's slot, within the range
+  const uint32_t* rec;
+  if (p.table) {
+    const int64_t pg = checked_page(p.table, b * p.tstride + lb, p.n_pages, p.err, 1003);
+    if (pg < 0) return;
+    rec = p.blocks + (pg * p.Hkv + h) * kRecWords;
+  } else {
+    rec = p.blocks + ((b * p.Hkv + h) * p.nbc + (p.head / kBlk + lb) % p.nbc) * kRecWords;
+  }
+  uint32_t* st = stage[warp];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    kbits |= k_code(kb, s, 8 * m + j) << (3 * j);
-    vbits |= v_code(vb, s, 8 * m + j) << (3 * j);
+  for (int i = 0; i < kRecBytes / 512; ++i)
+    reinterpret_cast<uint4*>(st)[32 * i + lane] = reinterpret_cast<const uint4*>(rec)[32 * i + lane];
+  __syncwarp();
+  if (pos < 0 || pos >= p.n) return;
+  const int64_t vec = (b * p.n + pos) * p.Hkv + h;
+  uint32_t w[12];
+  auto store = [&](uint8_t* dst) {
+    if (((uintptr_t)dst & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        reinterpret_cast<uint4*>(dst)[i] =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+      for (int i = 0; i < 12; ++i)
+        for (int k = 0; k < 4; ++k) dst[4 * i + k] = (uint8_t)(w[i] >> (8 * k));
+    }
+  };
+  // K: the slot's triples lie in lanes 4(u % 8) + r
+  uint32_t f[4][8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t* t = st + (4 * (lane & 7) + r) * 12 + 3 * (lane >> 3);
+    const uint32_t w0 = t[0], w1 = t[1], w2 = t[2];
+    uint32_t q[8] = {w0, w0 >> 3, w1, w1 >> 3, w2, w2 >> 3, 0, 0};
+    q[6] = ((w0 >> 6) & 0x03030303u) | ((w2 >> 4) & 0x04040404u);
+    q[7] = ((w1 >> 6) & 0x03030303u) | ((w2 >> 5) & 0x04040404u);
+#pragma unroll
+    for (int Q = 0; Q < 8; ++Q)
+      f[r][Q] = (q[Q] & 7u) | (q[Q] >> 5 & 0x38u) | (q[Q] >> 10 & 0x1C0u) | (q[Q] >> 15 & 0xE00u);
   }
-  const int64_t o = vec * kRec + 3 * m;  // [B][n][Hkv][48] == [B][n][Hkv*48]
-  kbytes[o] = (uint8_t)(kbits & 0xFF);
-  kbytes[o + 1] = (uint8_t)((kbits >> 8) & 0xFF);
-  kbytes[o + 2] = (uint8_t)((kbits >> 16) & 0xFF);
-  vbytes[o] = (uint8_t)(vbits & 0xFF);
-  vbytes[o + 1] = (uint8_t)((vbits >> 8) & 0xFF);
-  vbytes[o + 2] = (uint8_t)((vbits >> 16) & 0xFF);
-  if (m == 0) {
-    const float2 km = reinterpret_cast<const float2*>(kb + kRecKmm)[mm_index(s)];
-    const float2 vm = reinterpret_cast<const float2*>(kb + kRecVmm)[mm_index(s)];
-    kmm_out[vec * 2] = km.x;
-    kmm_out[vec * 2 + 1] = km.y;
-    vmm_out[vec * 2] = vm.x;
-    vmm_out[vec * 2 + 1] = vm.y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // 96 bits: the 12-bit fields of quads 2i and 2i + 1
+    w[3 * i] = f[0][2 * i] | f[1][2 * i] << 12 | f[2][2 * i] << 24;
+    w[3 * i + 1] = f[2][2 * i] >> 8 | f[3][2 * i] << 4 | f[0][2 * i + 1] << 16 | f[1][2 * i + 1] << 28;
+    w[3 * i + 2] = f[1][2 * i + 1] >> 4 | f[2][2 * i + 1] << 8 | f[3][2 * i + 1] << 20;
   }
+  store(kbytes + vec * kRec);
+  // V: byte b, half a of the triples of lanes 4g + r
+  const int a = (lane >> 2) & 1, sb = 8 * (lane >> 3);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    uint32_t G[4] = {0, 0, 0, 0};  // the 24-bit groups 4m + j
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const uint32_t* t = st + kRecV + (4 * g + (lane & 3)) * 12 + 3 * m;
+      const uint32_t y0 = t[0] >> sb, y1 = t[1] >> sb, y2 = t[2] >> sb;
+      G[0] |= ((y0 >> (3 * a)) & 7u) << (3 * g);
+      G[1] |= ((y1 >> (3 * a)) & 7u) << (3 * g);
+      G[2] |= ((y2 >> (3 * a)) & 7u) << (3 * g);
+      G[3] |= ((((a ? y1 : y0) >> 6) & 3u) | ((y2 >> (6 + a)) & 1u) << 2) << (3 * g);
+    }
+    w[3 * m] = G[0] | G[1] << 24;
+    w[3 * m + 1] = G[1] >> 8 | G[2] << 16;
+    w[3 * m + 2] = G[2] >> 16 | G[3] << 8;
+  }
+  store(vbytes + vec * kRec);
+  const float2 km = reinterpret_cast<const float2*>(st + kRecKmm)[mm_index(lane)];
+  const float2 vm = reinterpret_cast<const float2*>(st + kRecVmm)[mm_index(lane)];
+  kmm_out[vec * 2] = km.x;
+  kmm_out[vec * 2 + 1] = km.y;
+  vmm_out[vec * 2] = vm.x;
+  vmm_out[vec * 2 + 1] = vm.y;
+}
+
+int launch_export(const RangeParams& p, uint8_t* k, float* kmm, uint8_t* v, float* vmm,
+                  cudaStream_t s) {
+  const int64_t off = p.table ? 0 : p.head % kBlk;
+  const int64_t nblk = (p.start + p.n + off + kBlk - 1) / kBlk - (p.start + off) / kBlk;
+  const int64_t total = p.B * nblk * p.Hkv;
+  FT_CHECK(ceil_div(total, kMoveWarps) < INT32_MAX, FT_ERR_UNSUPPORTED, "range too long");
+  kv3_export_kernel<<<(unsigned)ceil_div(total, kMoveWarps), 32 * kMoveWarps, 0, s>>>(
+      p, nblk, total, k, kmm, v, vmm);
+  FT_LAUNCH_CHECK();
+  return FT_OK;
+}
+
+int launch_append_packed(const AppendParams& p, int64_t batch, int64_t nblk, cudaStream_t s) {
+  const int64_t total = batch * nblk * p.Hkv;
+  FT_CHECK(ceil_div(total, kMoveWarps) < INT32_MAX, FT_ERR_UNSUPPORTED, "append too long");
+  kv3_append_packed_kernel<<<(unsigned)ceil_div(total, kMoveWarps), 32 * kMoveWarps, 0, s>>>(
+      p, nblk, total);
+  FT_LAUNCH_CHECK();
+  return FT_OK;
 }
 
 // ---------------------------------------------------------------- decode --
@@ -1000,12 +1211,14 @@ int append_common(ft_kv3* c, int64_t n_pos, const AppendParams& proto, bool pack
   // a block is touched by one CTA only: the new slots never wrap onto a block
   // that an earlier CTA of this launch also writes
   FT_CHECK(nblk <= p.nbc, FT_ERR_SHAPE, "append spans more blocks than the ring holds");
-  dim3 grid((unsigned)nblk, (unsigned)(c->batch * c->kv_heads));
-  if (packed)
-    kv3_append_kernel<true><<<grid, kD, 0, s>>>(p);
-  else
-    kv3_append_kernel<false><<<grid, kD, 0, s>>>(p);
-  FT_LAUNCH_CHECK();
+  if (packed) {
+    const int rc = launch_append_packed(p, c->batch, nblk, s);
+    if (rc != FT_OK) return rc;
+  } else {
+    dim3 grid((unsigned)nblk, (unsigned)(c->batch * c->kv_heads));
+    kv3_append_kernel<<<grid, kD, 0, s>>>(p);
+    FT_LAUNCH_CHECK();
+  }
   c->len += n_pos;
   return FT_OK;
 }
@@ -1239,12 +1452,8 @@ int ft_kv3_export_range(ft_ctx* ctx, const ft_kv3* c, int64_t start, int64_t end
   const int64_t n = end - start;
   if (n == 0) return FT_OK;
   DeviceScope scope(c->device);
-  kv3_export_kernel<<<(unsigned)(c->batch * n * c->kv_heads), 16, 0,
-                      static_cast<cudaStream_t>(stream)>>>(range_params(c, start, n), k_codes_dev,
-                                                           k_minmax_dev, v_codes_dev,
-                                                           v_minmax_dev);
-  FT_LAUNCH_CHECK();
-  return FT_OK;
+  return launch_export(range_params(c, start, n), k_codes_dev, k_minmax_dev, v_codes_dev,
+                       v_minmax_dev, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
@@ -1445,12 +1654,10 @@ static int kvp_append(ft_ctx* ctx, ft_kvp* c, int64_t batch, int64_t n_pos,
   p.n_pages = c->n_pages;
   p.err = ctx->err_word;
   const int64_t nblk = (kBlk - 1 + n_pos + kBlk - 1) / kBlk;  // most blocks one sequence touches
-  dim3 grid((unsigned)nblk, (unsigned)(batch * c->kv_heads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (packed)
-    kv3_append_kernel<true><<<grid, kD, 0, s>>>(p);
-  else
-    kv3_append_kernel<false><<<grid, kD, 0, s>>>(p);
+  if (packed) return launch_append_packed(p, batch, nblk, s);
+  dim3 grid((unsigned)nblk, (unsigned)(batch * c->kv_heads));
+  kv3_append_kernel<<<grid, kD, 0, s>>>(p);
   FT_LAUNCH_CHECK();
   return FT_OK;
 }
@@ -1553,11 +1760,8 @@ int ft_kvp_export_range(ft_ctx* ctx, const ft_kvp* c, int64_t batch, const int32
            "null argument");
   if (p.n == 0 || batch == 0) return FT_OK;
   DeviceScope scope(c->device);
-  kv3_export_kernel<<<(unsigned)(batch * p.n * c->kv_heads), 16, 0,
-                      static_cast<cudaStream_t>(stream)>>>(p, k_codes_dev, k_minmax_dev,
-                                                           v_codes_dev, v_minmax_dev);
-  FT_LAUNCH_CHECK();
-  return FT_OK;
+  return launch_export(p, k_codes_dev, k_minmax_dev, v_codes_dev, v_minmax_dev,
+                       static_cast<cudaStream_t>(stream));
 }
 
 static int paged_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,

@@ -514,3 +514,52 @@ def test_captured_keep_and_select(kv):
     c.ctx.check()
     c.close()
     d.close()
+
+
+@pytest.mark.parametrize("H", [1, 3, 8])
+def test_packed_append_in_pieces(kv, paged, H):
+    """Stored positions appended in pieces that begin and end inside blocks, from aligned and
+    unaligned memory, read back byte for byte."""
+    g, rng = generator(30 + H), np.random.default_rng(H)
+    B, n = 2, 333
+    src = kv.Kv3Cache(B, H, n)
+    src.append(rand(g, B, n, H, D), rand(g, B, n, H, D))
+    want = src.export_range(0, n)
+    c = kv.Kv3Cache(B, H, 352)
+    c.append(rand(g, B, 45, H, D), rand(g, B, 45, H, D))
+    c.evict_front(45)  # the head lies inside a block, and the ring wraps
+    p = paged.PagedKv3Cache(1, 30, H)
+    rids = [p.create_request() for _ in range(B)]
+    at = 0
+    for m in (1, 30, 2, 64, 95, 7, 134):
+        part = [t[:, at:at + m] for t in want]
+        c.append_packed(*part)
+        p.append_packed(0, rids, *part)
+        at += m
+    assert at == n
+    for a, b in ((0, n), (1, 2), (31, 33), (40, 300), (332, 333)):
+        for got in (c.export_range(a, b), p.export_range(0, rids, a, b)):
+            for x, y in zip(got, want):
+                assert torch.equal(x, y[:, a:b])
+    # unaligned code bytes in and out
+    from ferrisres_b200._lib import call
+    from ferrisres_b200.gpu import _dptr, _stream_ptr
+    c.reset()
+    moved = []
+    for t in (want[0], want[2]):
+        raw = torch.zeros(t.numel() + 3, dtype=torch.uint8, device="cuda")
+        raw[3:] = t.flatten()
+        moved.append(raw)
+    call("ft_kv3_append_packed", c.ctx.handle, c.handle, n, C.c_void_p(moved[0].data_ptr() + 3), _dptr(want[1]),
+         C.c_void_p(moved[1].data_ptr() + 3), _dptr(want[3]), _stream_ptr())
+    for raw in moved:
+        raw.fill_(255)
+    mm = [torch.empty_like(want[1]), torch.empty_like(want[3])]
+    call("ft_kv3_export_range", c.ctx.handle, c.handle, 0, n, C.c_void_p(moved[0].data_ptr() + 3), _dptr(mm[0]),
+         C.c_void_p(moved[1].data_ptr() + 3), _dptr(mm[1]), _stream_ptr())
+    for raw, t in zip(moved, (want[0], want[2])):
+        assert torch.equal(raw[3:], t.flatten()) and raw[:3].tolist() == [255] * 3
+    assert torch.equal(mm[0], want[1]) and torch.equal(mm[1], want[3])
+    p.ctx.check()
+    for x in (src, c, p):
+        x.close()
