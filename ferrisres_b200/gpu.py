@@ -56,9 +56,29 @@ def get_context(device: int | None = None) -> Context:
         return c
 
 
+# the current stream's handle without the Stream object that torch.cuda.current_stream
+# builds (0.1 instead of 3 us, a sixth of a small call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream_ptr(stream=None):
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
+    return C.c_void_p(_raw_stream(torch.cuda.current_device()))
+
+
+def _call_stream(device, stream, *tensors):
+    """Stream handle of a call that uses ``tensors``: the current stream of ``device``, or
+    ``stream``, ordered after what the current one holds (copies made for the call among
+    it); the tensors then stay allocated until ``stream`` has passed this point."""
+    if stream is None:
+        return C.c_void_p(_raw_stream(device.index))
+    stream.wait_stream(torch.cuda.current_stream(device))
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    return C.c_void_p(stream.cuda_stream)
 
 
 def _dptr(t: torch.Tensor):

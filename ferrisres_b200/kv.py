@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ._lib import ShapeError, UnsupportedError, call
-from .gpu import _dptr, _stream_ptr, get_context
+from .gpu import _call_stream, _dptr, _stream_ptr, get_context
 
 HEAD_DIM = 128
 REC_BYTES = HEAD_DIM * 3 // 8  # 48
@@ -47,24 +47,6 @@ def tree_mask(parents, device=None) -> torch.Tensor:
     if device is None:
         device = torch.device("cuda", torch.cuda.current_device())
     return m.to(device)
-
-
-def _launch_stream(device, stream):
-    """The stream of a call: ``stream``, ordered after what the current one holds (the
-    copies made for the call among it), or the current stream of ``device``."""
-    cur = torch.cuda.current_stream(device)
-    if stream is None:
-        return cur
-    stream.wait_stream(cur)
-    return stream
-
-
-def _used_on(stream, device, *tensors):
-    """Keeps the call's own tensors alive for work on a stream that is not the one they
-    were made on."""
-    if stream != torch.cuda.current_stream(device):
-        for t in tensors:
-            t.record_stream(stream)
 
 
 def _row_stride(t: torch.Tensor, rows: tuple, least: int, what: str, device) -> int:
@@ -107,11 +89,9 @@ def select_heavy(weights: torch.Tensor, n_keep: int, n_recent: int = 0, length: 
     if B == 0:
         return idx, out
     lens = None if seq_lens is None else seq_lens.contiguous()
-    s = _launch_stream(dev, stream)
     call("ft_kv_select_heavy", get_context(dev.index).handle, B, H, C.c_void_p(weights.data_ptr()),
          step, None if lens is None else _dptr(lens), length, n_keep, n_recent, _dptr(idx),
-         _dptr(out), W, _stream_ptr(s))
-    _used_on(s, dev, weights, idx, out, *([] if lens is None else [lens]))
+         _dptr(out), W, _call_stream(dev, stream, weights, idx, out, lens))
     return idx, out
 
 
@@ -255,8 +235,7 @@ class Kv3Cache:
         kc = torch.empty((self.batch, n, self.kv_heads * REC_BYTES), dtype=torch.uint8,
                          device=self.device)
         vc = torch.empty_like(kc)
-        km = torch.empty((self.batch, n, self.kv_heads, 2), dtype=torch.float32,
-                         device=self.device)
+        km = kc.new_empty((self.batch, n, self.kv_heads, 2), dtype=torch.float32)
         vm = torch.empty_like(km)
         call("ft_kv3_export_range", self.ctx.handle, self.handle, int(start), int(end),
              _dptr(kc), _dptr(km), _dptr(vc), _dptr(vm), _stream_ptr(stream))
@@ -288,11 +267,9 @@ class Kv3Cache:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
             raise ShapeError("out must be like q")
-        s = _launch_stream(self.device, stream)
         call("ft_flash_decode_3bit_weights", self.ctx.handle, self.handle, _dptr(q),
              int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
-             _stream_ptr(s))
-        _used_on(s, self.device, q, out, weights)
+             _call_stream(self.device, stream, q, out, weights))
         return out
 
     def tree_decode(self, q: torch.Tensor, mask: torch.Tensor | None = None, scale: float = 0.0,
@@ -303,11 +280,9 @@ class Kv3Cache:
         the bits of mask[b, i] (int64 [batch, n_draft] or [n_draft], see ``tree_mask``;
         None: drafts 0..i).  A draft that sees nothing gets 0."""
         q, mask, out = _tree_args(q, mask, self.batch, self.device, out)
-        s = _launch_stream(self.device, stream)
         call("ft_kv3_tree_decode", self.ctx.handle, self.handle, int(q.shape[1]), _dptr(q),
              int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
-             float(scale), _dptr(out), _stream_ptr(s))
-        _used_on(s, self.device, q, out, *([] if mask is None else [mask]))
+             float(scale), _dptr(out), _call_stream(self.device, stream, q, out, mask))
         return out
 
     # ---- choosing what stays
@@ -321,10 +296,8 @@ class Kv3Cache:
         self._keep(idx, n, ib, ih, int(start), stream)
 
     def _keep(self, idx, n, ib, ih, start, stream):
-        s = _launch_stream(self.device, stream)
         call("ft_kv3_keep", self.ctx.handle, self.handle, start, n, _dptr(idx), ib, ih,
-             _stream_ptr(s))
-        _used_on(s, self.device, idx)
+             _call_stream(self.device, stream, idx))
 
     def evict_heavy(self, weights: torch.Tensor, n_keep: int, n_recent: int = 0, stream=None):
         """Evicts down to ``n_keep`` positions per sequence and kv head: the ``n_recent``

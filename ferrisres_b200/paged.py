@@ -24,8 +24,8 @@ import numpy as np
 import torch
 
 from ._lib import OOMError, ShapeError, call
-from .gpu import _dptr, _stream_ptr, get_context
-from .kv import (_index_list, _launch_stream, _row_stride, _tree_args, _used_on, select_heavy)
+from .gpu import _call_stream, _dptr, _stream_ptr, get_context
+from .kv import _index_list, _row_stride, _tree_args, select_heavy
 
 DEFAULT_BLOCK_SIZE = 16   # the reference's default (paged_attention.rs:21)
 PAGE_POSITIONS = 32       # positions per device page
@@ -419,23 +419,22 @@ class PagedKv3Cache:
             return
         copies = []
         starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
-        s = _launch_stream(self.device, stream)
-        self._copy_pages(copies, s)
+        self._copy_pages(copies, stream)
         tables, stride = self._tables(layer, rids)
         start_dev = torch.from_numpy(starts).to(self.device)
-        s = _launch_stream(self.device, stream)
         call("ft_kvp_append_packed", self.ctx.handle, self.handle, len(rids), n_pos,
-             _dptr(tables), stride, _dptr(start_dev), *[_dptr(t) for t in tens], _stream_ptr(s))
-        _used_on(s, self.device, tables, start_dev, *tens)
+             _dptr(tables), stride, _dptr(start_dev), *[_dptr(t) for t in tens],
+             _call_stream(self.device, stream, tables, start_dev, *tens))
         for r in rids:
             self._grow_by(layer, r, n_pos)
 
-    def _copy_pages(self, copies, s):
+    def _copy_pages(self, copies, stream):
         if copies:
             src = np.array([c[0] for c in copies], np.int32)
             dst = np.array([c[1] for c in copies], np.int32)
             call("ft_kvp_copy_pages", self.ctx.handle, self.handle, len(copies),
-                 src.ctypes.data_as(C.c_void_p), dst.ctypes.data_as(C.c_void_p), _stream_ptr(s))
+                 src.ctypes.data_as(C.c_void_p), dst.ctypes.data_as(C.c_void_p),
+                 _call_stream(self.device, stream))
 
     def _grow_by(self, layer, rid, n):
         st = self._state(rid)
@@ -458,12 +457,11 @@ class PagedKv3Cache:
             raise ShapeError(f"{q.shape[1]} drafts in a request of {lens.min()} positions")
         tables, stride = self._tables(layer, rids)
         lens_dev = torch.from_numpy(lens).to(self.device)
-        s = _launch_stream(self.device, stream)
         call("ft_kvp_tree_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
              _dptr(lens_dev), int(lens.max()), int(q.shape[1]), _dptr(q),
              int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
-             float(scale), _dptr(out), _stream_ptr(s))
-        _used_on(s, self.device, tables, lens_dev, q, out, *([] if mask is None else [mask]))
+             float(scale), _dptr(out),
+             _call_stream(self.device, stream, tables, lens_dev, q, out, mask))
         return out
 
     def keep(self, layer: int, request_ids, idx: torch.Tensor, counts=None, starts=None,
@@ -506,16 +504,13 @@ class PagedKv3Cache:
             old, t[j] = t[j], alloc.allocate()
             copies.append((old, t[j]))
             alloc.free(old)
-        s = _launch_stream(self.device, stream)
-        self._copy_pages(copies, s)
+        self._copy_pages(copies, stream)
         if max(counts) > 0:
             tables, stride = self._tables(layer, rids)
             meta = torch.from_numpy(np.array([lens, starts, counts], np.int32)).to(self.device)
-            s = _launch_stream(self.device, stream)
             call("ft_kvp_keep", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
                  _dptr(meta[0]), _dptr(meta[1]), _dptr(meta[2]), max(counts), _dptr(idx), ib, ih,
-                 _stream_ptr(s))
-            _used_on(s, self.device, tables, meta, idx)
+                 _call_stream(self.device, stream, tables, meta, idx))
         for r, t, c, st, length in zip(rids, tabs, counts, starts, lens):
             need = -(-(st + c) // PAGE_POSITIONS)
             while len(t) > need:
@@ -575,7 +570,9 @@ class PagedKv3Cache:
                  _dptr(tables), stride, _dptr(lens_dev), int(lens.max()), _dptr(q),
                  int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
                  _stream_ptr(s))
-            _used_on(s, self.device, q, out, weights)
+            if stream is not None:
+                for t in (q, out, weights):
+                    t.record_stream(s)
         else:
             call("ft_kvp_flash_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables),
                  stride, _dptr(lens_dev), int(lens.max()), _dptr(q), int(q.shape[1]),
