@@ -13,7 +13,8 @@ positions that the row sees and V = max |v| over them; n of them.
   as a whole: these roundings are independent, so the 2-norm of an fp32 result's error stays well under the
     worst case: within 1e-5 of the result's (mode R, where the comparison's input is exact), the bound of the
     single-token decode.
-  output: bf16 rounds by 2^-8 of the value.
+  output: bf16 rounds by 2^-8 of the value, uniformly up to that, so by at most 2^-8 / sqrt(3) in the
+    2-norm; what comes before (2^-11) hides in that: 0.6 * 2^-8 of the result's norm.
   mode T: the stored vectors rotated back in fp32 (the comparison's input) are off by about
     10 * 2^-24 of their norm <= 12 max|v|: 2^-17 V, and of k likewise: X 2^-17.
 """
@@ -137,6 +138,60 @@ def test_ring_tree_decode(kv, case, mode, dtype):
     c.close()
 
 
+@pytest.mark.parametrize("mode", ["R", "T"])
+@pytest.mark.parametrize("case", [(1, 128 + 1, 1, 1, 1), (1, 256 + 3, 2, 8, 2), (2, 385, 1, 16, 2), (1, 1100, 4, 32, 8),
+                                  (1, 2100, 64, 2, 1), (2, 1500, 64, 4, 1), (1, 3000, 33, 20, 4), (3, 900, 64, 15, 3),
+                                  (1, 20000, 8, 8, 2), (8, 640, 17, 8, 8)])
+def test_whole_prefix_tiles(kv, case, mode):
+    """bf16 queries: the 128-position tiles in front of the drafts, one and many, few and many rows."""
+    B, n, T, Hq, H = case
+    g = generator(n + T)
+    c = kv.Kv3Cache(B, H, n, mode=mode, seed=3)
+    spread = 0.2 + 2 * torch.rand((H, D), generator=g, device="cuda")
+    c.append(rand(g, B, n, H, D) * spread, rand(g, B, n, H, D) * spread)
+    q = (2 * rand(g, B, T, Hq, D)).bfloat16()
+    mask, bits = rand_mask(g, B, T)
+    out = c.tree_decode(q, mask)
+    c.ctx.check()
+    k, v = c.get_range(0, n)
+    for b in range(B):
+        check(out[b], exact(q[b], k[b], v[b], bits[b]), torch.bfloat16, mode, n)
+    c.close()
+
+
+def test_scores_that_rise(kv):
+    """Maxima that move by a little and by a lot along the sequence, values that grow by 2^20, constant
+    vectors: the references of the prefix tiles move in every way."""
+    g = generator(21)
+    n, T, Hq, H = 2500, 6, 8, 2
+    for kind in ("rise", "fall", "steps", "huge", "values", "constant"):
+        k, v = rand(g, 1, n, H, D), rand(g, 1, n, H, D)
+        q = (2 * rand(g, 1, T, Hq, D)).bfloat16()
+        at = torch.arange(n, device="cuda")[None, :, None, None]
+        along = torch.nn.functional.normalize(q.float().mean((1, 2)), dim=-1)  # moves every row's score
+        if kind == "rise":
+            k = k + along * at * 0.03
+        elif kind == "fall":
+            k = k - along * at * 0.03
+        elif kind == "steps":
+            k = k + along * (at // 300 * 37 % 90)
+        elif kind == "huge":
+            k = k * 40
+        elif kind == "values":
+            v = v * torch.exp2(torch.div(at, 128, rounding_mode="floor").float())
+        else:
+            v[:, ::2] = 0.5
+            v[:, 1200:1600] = 0.0
+            k[:, 700] = 1.0
+        c = kv.Kv3Cache(1, H, n)
+        c.append(k, v)
+        out = c.tree_decode(q)
+        c.ctx.check()
+        kk, vv = c.get_range(0, n)
+        check(out[0], exact(q[0], kk[0], vv[0], causal_bits(1, T)[0]), torch.bfloat16, "R", n)
+        c.close()
+
+
 def test_moved_ring(kv):
     """Heads that start inside a block, and a ring that wraps onto its first block."""
     g = generator(5)
@@ -144,6 +199,12 @@ def test_moved_ring(kv):
     c = kv.Kv3Cache(B, H, 256)
     c.append(rand(g, B, 250, H, D), rand(g, B, 250, H, D))
     for drop, add in ((7, 13), (100, 95), (31, 31), (33, 38)):
+        q16 = (2 * rand(g, B, T, Hq, D)).bfloat16()
+        mask, bits = rand_mask(g, B, T)
+        out = c.tree_decode(q16, mask)  # heads inside a block: its slots are the edges' work
+        k, v = c.get_range(0, len(c))
+        for b in range(B):
+            check(out[b], exact(q16[b], k[b], v[b], bits[b]), torch.bfloat16, "R", len(c))
         c.evict_front(drop)
         c.append(rand(g, B, add, H, D), rand(g, B, add, H, D))
         n = len(c)
