@@ -67,24 +67,9 @@ struct TreeParams {
   const int32_t* table;  // paged pool, as the single-token decode
   const int32_t* seq_lens;
   int64_t tstride, n_pages;
-  // edge != 0: the whole 128-position tiles of the prefix belong to
-  // tree_prefix_kernel, which writes partials 0 .. nparts - 2; this launch takes
-  // the blocks around them and writes partial nparts - 1
-  int edge, nparts;
+  int nparts;  // splits
+  uint8_t* qimg;  // bf16 queries: prepared row tiles [B][Hkv][rgroups]
 };
-
-// Blocks [first, last) of a sequence that tree_prefix_kernel takes: every slot
-// is a position of the prefix, and they make whole tiles.
-struct PrefixBlocks {
-  int first, last;
-};
-__device__ __forceinline__ PrefixBlocks prefix_blocks(const TreeParams& p, int64_t len_b) {
-  const int64_t off = p.table ? 0 : p.head_off;
-  const int first = off ? 1 : 0;
-  const int64_t end = len_b - p.T + off;  // slots in front of the drafts
-  const int64_t n = end <= first * kBlk ? 0 : (end / kBlk - first) / kTWarps * kTWarps;
-  return {first, first + (int)n};
-}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -112,11 +97,14 @@ __device__ __forceinline__ uint32_t quad_half2(uint32_t w0, uint32_t w1, uint32_
   return (shifted<9 - Q - 8 * h>(w2) & 0x02000200u) | lo;
 }
 // the same centred: (c - 3.5) / 8
+__device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
+  uint32_t v;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+  return v;
+}
 template <int Q, int h>
 __device__ __forceinline__ uint32_t quad_centred(uint32_t w0, uint32_t w1, uint32_t w2) {
-  uint32_t v;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(quad_half2<Q, h>(w0, w1, w2)), "r"(0x3DC03DC0u));
-  return v;
+  return sub_half2(quad_half2<Q, h>(w0, w1, w2), 0x3DC03DC0u);
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {  // a in the low half
@@ -149,25 +137,26 @@ __device__ __forceinline__ void warp_fwht128(float (&v)[4], int lane) {
     }
 }
 
-// Query row (4 elements a lane), rotated in mode T, and its sh.
-__device__ __forceinline__ void load_q_row(const TreeParams& p, int64_t b, int64_t kvh, int R,
-                                           int lane, float (&v)[4], int* sh) {
+// Four elements of query row R (lane's), as stored.
+__device__ __forceinline__ uint4 load_q_raw(const TreeParams& p, int64_t b, int64_t kvh, int R,
+                                            int lane) {
   const int t = R / p.G;
   const int64_t h = kvh * p.G + (R - t * p.G);
   const int64_t at = ((b * p.T + t) * p.Hq + h) * kD + 4 * lane;
   if (p.q_bf16) {
     const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at);
-    v[0] = __uint_as_float(w.x << 16);
-    v[1] = __uint_as_float(w.x & 0xffff0000u);
-    v[2] = __uint_as_float(w.y << 16);
-    v[3] = __uint_as_float(w.y & 0xffff0000u);
-  } else {
-    const float4 w = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
-    v[0] = w.x;
-    v[1] = w.y;
-    v[2] = w.z;
-    v[3] = w.w;
+    return make_uint4(w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u);
   }
+  return *reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at);
+}
+
+// The row's values, rotated in mode T, and its sh.
+__device__ __forceinline__ void q_row(const TreeParams& p, const uint4& raw, int lane,
+                                      float (&v)[4], int* sh) {
+  v[0] = __uint_as_float(raw.x);
+  v[1] = __uint_as_float(raw.y);
+  v[2] = __uint_as_float(raw.z);
+  v[3] = __uint_as_float(raw.w);
   if (p.signs) {
     const float4 sg = reinterpret_cast<const float4*>(p.signs)[lane];
     v[0] *= sg.x;
@@ -220,15 +209,6 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
     }
     nlb_b = (len_b + kBlk - 1) / kBlk;
   }
-  // edge launches count their blocks without the prefix's: block i is block
-  // i + skip from `gap` on
-  int gap = 0, skip = 0;
-  if (p.edge) {
-    const PrefixBlocks pre = prefix_blocks(p, len_b);
-    gap = pre.first;
-    skip = pre.last - pre.first;
-    nlb_b -= skip;
-  }
   const int64_t ntiles_all = (nlb_b + kTWarps - 1) / kTWarps;
   const int64_t t_begin = (int64_t)split * p.tiles_per;
   int64_t t_end = t_begin + p.tiles_per;
@@ -246,10 +226,18 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
   // dims 4r, 4r+2 and 2r+8, 2r+9 dims 4r+1, 4r+3 (bytes 0, 2 and 1, 3 of a quad)
   if (warp < kTWarps) {
     uint32_t* qw = reinterpret_cast<uint32_t*>(smem + kTOffQf);
-    for (int i = warp; i < kRows; i += kTWarps) {
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      int sh = 0;
-      if (R0 + i < p.rows) load_q_row(p, b, kvh, R0 + i, lane, v, &sh);
+    uint4 raw[kRows / kTWarps];  // every load first
+#pragma unroll
+    for (int k = 0; k < kRows / kTWarps; ++k) {
+      const int i = warp + k * kTWarps;
+      raw[k] = R0 + i < p.rows ? load_q_raw(p, b, kvh, R0 + i, lane) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kRows / kTWarps; ++k) {
+      const int i = warp + k * kTWarps;
+      float v[4];
+      int sh;
+      q_row(p, raw[k], lane, v, &sh);
       const float mul = pow2i(sh);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] *= mul;
@@ -295,17 +283,12 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
         const int nb = nlb_b - j0 < kTWarps ? (int)(nlb_b - j0) : kTWarps;
         tc::mbar_arrive_expect_tx(full0 + 8 * s, nb * kRecBytes);
         const uint32_t sb = stage_base + s * kTStageBytes;
-        if (p.table || p.edge) {
-          for (int i = 0; i < nb; ++i) {
-            const int64_t jb = j0 + i + (j0 + i >= gap ? skip : 0);
-            int64_t rec;
-            if (p.table) {  // a bad table entry reads page 0 and is reported
-              int64_t pg = checked_page(p.table, b * p.tstride + jb, p.n_pages, p.err, 1008);
-              rec = (pg < 0 ? 0 : pg) * p.Hkv + kvh;
-            } else {
-              rec = row * p.nbc + (p.head_blk + jb) % p.nbc;
-            }
-            tc::bulk_g2s(sb + i * kRecBytes, p.blocks + rec * kRecWords, kRecBytes, full0 + 8 * s);
+        if (p.table) {
+          for (int i = 0; i < nb; ++i) {  // a bad table entry reads page 0 and is reported
+            int64_t pg = checked_page(p.table, b * p.tstride + j0 + i, p.n_pages, p.err, 1008);
+            if (pg < 0) pg = 0;
+            tc::bulk_g2s(sb + i * kRecBytes, p.blocks + (pg * p.Hkv + kvh) * kRecWords, kRecBytes,
+                         full0 + 8 * s);
           }
         } else {
           const int n1 = pb + nb <= p.nbc ? nb : (int)(p.nbc - pb);
@@ -409,7 +392,7 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
                   fmaf(kc, qsum[h], ks * (sc[a][bb][2 * h + i] * qscale[h]));
           }
         }
-      const int base = (j + (j >= gap ? skip : 0)) * kBlk - hoff;
+      const int base = j * kBlk - hoff;
       // blocks of the prefix are seen whole; the others slot by slot
       const bool part = base < 0 || base + kBlk > P;
       float mt[2], vx[2];
@@ -576,7 +559,6 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
                       fmaf(o[n][2 * h + 1], 8.0f, vm_part[h]));
   }
   asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
-  const int part_at = p.edge ? p.nparts - 1 : split;
   for (int i = warp; i < kRows && R0 + i < p.rows; i += kTWarps) {
     float M = -INFINITY;
 #pragma unroll
@@ -594,7 +576,7 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
       acc[2] = fmaf(f, v.z, acc[2]);
       acc[3] = fmaf(f, v.w, acc[3]);
     }
-    float* pp = p.part + ((row * p.rows + R0 + i) * p.nparts + part_at) * kTPart;
+    float* pp = p.part + ((row * p.rows + R0 + i) * p.nparts + split) * kTPart;
     if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(M, l);
     float2* pn = reinterpret_cast<float2*>(pp + 2) + 2 * lane;  // records are 8-byte aligned
     pn[0] = make_float2(acc[0], acc[1]);
@@ -602,18 +584,16 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
   }
 }
 
-// ------------------------------------------------------- prefix on tcgen05 --
-// The whole 128-position tiles of the prefix, which every draft sees, for up to
-// 128 query rows at once: S = Q K' (M rows, N positions) and O += P V' on the
-// 5th-generation tensor core, K' and V' being the tile's codes as fp16.  No mask
-// enters here; the blocks around the tiles are tree_decode_kernel's.
+// ------------------------------------------------- bf16 queries on tcgen05 --
+// S = Q K' (128 query rows x 128 positions a tile), then O += P V', on the
+// 5th-generation tensor core, K' and V' being the tile's codes as fp16.
 //
-// One CTA per SM, 14 warps.  A producer warp streams the records of a tile (4 of
-// 3584 bytes) into raw buffers; four converter warps, one record each, write
-// the operands K' (1 + c/8) and V' ((c - 3.5)/8) in the swizzled K-major layout
-// and each position's factors; one thread issues the MMAs; two groups of four
-// softmax warps take the even and the odd tiles, each with its own S and O in
-// TMEM and its own running statistics, and merge at the end.  P overwrites S.
+// One CTA per SM, 28 warps.  A producer warp streams the records of a tile (4 of
+// 3584 bytes) into raw buffers; four warps write the operand K' (1 + c/8) and four
+// V' ((c - 3.5)/8), one record each, in the swizzled K-major layout; two warps
+// compute each position's factors; one thread issues the MMAs; two groups of eight
+// softmax warps (16 rows each) take the even and the odd tiles, each with its own S
+// and O in TMEM and its own running statistics, and merge at the end.  P overwrites S.
 // The K index of the first product is dims in the order 32 (Q/2) + 8r + 4 (Q%2)
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
@@ -626,21 +606,27 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 // a step on average, 2^-14 after 2048 steps, against 2^-9 of the bf16 output; fp32
 // queries use tree_decode_kernel.
 constexpr int kPreRows = 128;
-constexpr int kPreWarps = 14;
+constexpr int kPreWarps = 28;
 constexpr int kPreRaw = 3;
 constexpr int kOperand = 128 * 128 * 2;  // bytes of Q, K' or V' (two swizzled panels)
 constexpr int kPreOffK = kOperand;
 constexpr int kPreOffV = kPreOffK + 2 * kOperand;
 constexpr int kPreOffRaw = kPreOffV + 2 * kOperand;
 constexpr int kPreOffFac = kPreOffRaw + kPreRaw * kTStageBytes;
-constexpr int kFacBytes = 64 * 32 + 16;  // per position pair {8st, 8st, kc, kc} {st, st, vc, vc}; e per record
-constexpr int kPreOffQinfo = kPreOffFac + 4 * kFacBytes;
-constexpr int kPreOffBars = kPreOffQinfo + kPreRows * 8;
-constexpr int kPreBars = 2 * kPreRaw + 5 * 2 + 4 + 1;
+constexpr int kFacBytes = 64 * 32 + 16;  // per position pair {st, st, kc, kc} {vst, vst, vc, vc}; e per record
+constexpr int kPreOffQinfo = kPreOffFac + 4 * kFacBytes;  // [128] sum term, [128] factor
+constexpr int kPreOffMask = kPreOffQinfo + kPreRows * 8;  // [128] draft bits
+constexpr int kPreOffBars = kPreOffMask + kPreRows * 8;
+// what tree_query_kernel prepares for a row tile: the operand as it lies in shared
+// memory, then the row sums, factors and draft bits
+constexpr int kQImage = kOperand + kPreRows * 16;
+static_assert(kPreOffMask == kPreOffQinfo + kPreRows * 8, "one copy brings both");
+constexpr int kPreBars = 2 * kPreRaw + 5 * 2 + 2 * 4 + 2;
 constexpr int kPreSmem = kPreOffBars + kPreBars * 8 + 16 + 1024;  // 1024: alignment
 static_assert(kPreSmem <= 227 * 1024, "one CTA per SM");
-constexpr int kMergeStride = kD + 4;  // floats per row of the merge area (conflict-free float4)
-static_assert(kPreRows * kMergeStride * 4 <= 4 * kOperand, "the merge uses the operand buffers");
+constexpr int kMergeStride = kD + 4;  // floats per row of a merge area (conflict-free float4)
+constexpr int kMergeArea = kPreRows * kMergeStride;
+static_assert(2 * kMergeArea * 4 <= kPreOffRaw, "the merge uses the operand buffers");
 static_assert(2 * kPreRows * 12 <= kPreRaw * kTStageBytes, "row statistics use the raw buffers");
 
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -673,9 +659,76 @@ __device__ __forceinline__ float ex2(float x) {  // 2 ulp, 0 below 2^-126
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Registers of a warpgroup from here on.  The seven groups' shares add up to the
+// 896 x 72 that the block is launched with: 4 x 88, 2 x 56, 40 (x 128 threads).
+template <int kRegs>
+__device__ __forceinline__ void more_regs() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void fewer_regs() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+// Lane (row of the MMA) of query row i of a tile: the first 64 rows take 16 lanes
+// in each quarter of the SM, so that fewer rows still use all four.
+__device__ __forceinline__ int row_lane(int i) {
+  return 32 * ((i >> 4) & 3) + 16 * (i >> 6) + (i & 15);
+}
+
+// The query operand of tree_tile_kernel, 32 rows a CTA, four a warp: fp16 in the
+// swizzled K-major layout, the rows' sums, factors and draft bits.  A kernel of
+// its own: every split of the positions needs the same operand, and its code,
+// fetched anew by each launch, took longer in the big kernel than here.
+constexpr int kQueryRows = 32;
+__global__ void __launch_bounds__(256) tree_query_kernel(const __grid_constant__ TreeParams p) {
+  tc::pdl_launch_dependents();  // the tile kernel may start to load the cache
+  const int64_t tile = blockIdx.x / (kPreRows / kQueryRows);  // (row, row tile)
+  const int64_t row = tile / p.rgroups, b = row / p.Hkv, kvh = row % p.Hkv;
+  const int R0 = (int)(tile % p.rgroups) * kPreRows;
+  const int i0 = (blockIdx.x % (kPreRows / kQueryRows)) * kQueryRows + (threadIdx.x >> 5) * 4;
+  const int lane = threadIdx.x & 31;
+  uint8_t* img = p.qimg + tile * (int64_t)kQImage;
+  uint4 raw[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    raw[y] = R0 + i0 + y < p.rows ? load_q_raw(p, b, kvh, R0 + i0 + y, lane)
+                                  : make_uint4(0, 0, 0, 0);
+  uint64_t mask = 0;
+  if (lane < 4 && R0 + i0 + lane < p.rows) mask = row_mask(p.mask, b, p.T, (R0 + i0 + lane) / p.G);
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int i = i0 + y;
+    float v[4];
+    int sh;
+    q_row(p, raw[y], lane, v, &sh);
+    const float mul = pow2i(sh);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= mul;
+    const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
+    const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+    float sum = (f0.x + f0.y) + (f1.x + f1.y);  // of the q that the products take
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int Q = lane >> 2, c = 4 * ((Q >> 1) & 1) + (lane & 3), at = row_lane(i);
+    *reinterpret_cast<uint2*>(img + (Q >> 2) * (kOperand / 2) + at * 128 + ((c ^ (at & 7)) << 4) +
+                              (Q & 1) * 8) = make_uint2(h0, h1);
+    if (lane == y) {
+      float* info = reinterpret_cast<float*>(img + kOperand);
+      info[at] = sum * ldexpf(p.qk_log2, -sh);
+      info[kPreRows + at] = ldexpf(p.qk_log2, 3 - sh);
+      reinterpret_cast<uint64_t*>(info + 2 * kPreRows)[at] = mask;
+    }
+  }
+}
+
+template <bool kValue>
+struct Masked {
+  static constexpr bool value = kValue;
+};
 
 __global__ void __launch_bounds__(kPreWarps * 32, 1)
-    tree_prefix_kernel(const __grid_constant__ TreeParams p) {
+    tree_tile_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = tc::smem_u32(smem);
@@ -683,9 +736,9 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
   const uint32_t raw_full = bars, raw_empty = raw_full + 8 * kPreRaw;
   const uint32_t k_full = raw_empty + 8 * kPreRaw, v_full = k_full + 16;
   const uint32_t qk_done = v_full + 16, pv_done = qk_done + 16, p_full = pv_done + 16;
-  const uint32_t fac_empty = p_full + 16, fin = fac_empty + 32;
+  const uint32_t fac_full = p_full + 16, fac_empty = fac_full + 32;
+  const uint32_t q_full = fac_empty + 32, fin = q_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPreOffBars + kPreBars * 8);
-  float* qinfo = reinterpret_cast<float*>(smem + kPreOffQinfo);  // [128] sum term, [128] factor
 
   const int split = blockIdx.x;
   const int64_t kvh = blockIdx.y / p.rgroups;
@@ -693,13 +746,16 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
   const int64_t b = blockIdx.z, row = b * p.Hkv + kvh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, r = lane & 3;
-  int64_t len_b = p.len;
-  if (p.table) {  // the edge launch reports a bad length
+  int64_t len_b = p.len, nlb_b = p.nlb;
+  if (p.table) {
     len_b = p.seq_lens[b];
-    len_b = len_b < 0 ? 0 : (len_b > p.len ? p.len : len_b);
+    if (len_b < 0 || len_b > p.len) {
+      if (tid == 0) atomicCAS(p.err, 0, 1007);
+      len_b = len_b < 0 ? 0 : p.len;
+    }
+    nlb_b = (len_b + kBlk - 1) / kBlk;
   }
-  const PrefixBlocks pre = prefix_blocks(p, len_b);
-  const int64_t t_all = (pre.last - pre.first) / kTWarps, t_begin = (int64_t)split * p.tiles_per;
+  const int64_t t_all = (nlb_b + kTWarps - 1) / kTWarps, t_begin = (int64_t)split * p.tiles_per;
   const int64_t t_end = t_begin + p.tiles_per < t_all ? t_begin + p.tiles_per : t_all;
   const int n = t_end > t_begin ? (int)(t_end - t_begin) : 0;
   const int nrows = p.rows - R0 < kPreRows ? p.rows - R0 : kPreRows;
@@ -709,359 +765,422 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       part[(int64_t)i * p.nparts * kTPart] = -INFINITY;
       part[(int64_t)i * p.nparts * kTPart + 1] = 0.0f;
     }
+    tc::pdl_wait();  // this grid never ends before the query kernel
     return;
   }
 
   if (tid == 0) {
     for (int s = 0; s < kPreRaw; ++s) {
       tc::mbar_init(raw_full + 8 * s, 1);
-      tc::mbar_init(raw_empty + 8 * s, 4);
+      tc::mbar_init(raw_empty + 8 * s, 10);  // K', V' and factor warps
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(k_full + 8 * s, 4);
       tc::mbar_init(v_full + 8 * s, 4);
       tc::mbar_init(qk_done + 8 * s, 1);
       tc::mbar_init(pv_done + 8 * s, 1);
-      tc::mbar_init(p_full + 8 * s, 4);
+      tc::mbar_init(p_full + 8 * s, 8);
     }
-    for (int s = 0; s < 4; ++s) tc::mbar_init(fac_empty + 8 * s, 4);
+    for (int s = 0; s < 4; ++s) {
+      tc::mbar_init(fac_full + 8 * s, 2);
+      tc::mbar_init(fac_empty + 8 * s, 8);
+    }
+    tc::mbar_init(q_full, 1);
     tc::mbar_init(fin, 1);
     tc::fence_barrier_init();
   }
-  if (warp == 13) tc::tmem_alloc(tc::smem_u32(tmem_slot), 512);
-  // the query operand: row i, 8 bytes a lane
-  if (warp < 12) {
-    for (int i = warp; i < kPreRows; i += 12) {
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      int sh = 0;
-      if (i < nrows) load_q_row(p, b, kvh, R0 + i, lane, v, &sh);
-      const float mul = pow2i(sh);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] *= mul;
-      const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
-      const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-      float sum = (f0.x + f0.y) + (f1.x + f1.y);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      const int Q = lane >> 2, c = 4 * ((Q >> 1) & 1) + (lane & 3);
-      *reinterpret_cast<uint2*>(smem + (Q >> 2) * (kOperand / 2) + i * 128 + ((c ^ (i & 7)) << 4) +
-                                (Q & 1) * 8) = make_uint2(h0, h1);
-      if (lane == 0) {
-        qinfo[i] = sum * ldexpf(p.qk_log2, -sh);
-        qinfo[kPreRows + i] = ldexpf(p.qk_log2, 3 - sh);
-      }
-    }
-    tc::fence_async_smem();
-  }
+  if (warp == 25) tc::tmem_alloc(tc::smem_u32(tmem_slot), 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tS = tmem, tO = tmem + 256;  // S (and P) 2 x 128 columns, O 2 x 128
 
-  if (warp == 12) {
-    // ------------------------------------------------------ producer warp --
-    if (lane == 0) {
-      bool ok = true;
-      int issued = 0;
-      for (int j = 0; j < n && ok; ++j) {
-        const int s = j % kPreRaw;
-        if (j >= kPreRaw) ok = tc::mbar_wait(raw_empty + 8 * s, ((j / kPreRaw) - 1) & 1, p.err, 51);
-        if (!ok) break;
-        tc::mbar_arrive_expect_tx(raw_full + 8 * s, kTStageBytes);
-        const uint32_t dst = sbase + kPreOffRaw + s * kTStageBytes;
-        const int64_t jb = pre.first + (t_begin + j) * kTWarps;
-        for (int i = 0; i < kTWarps; ++i) {
-          int64_t rec;
-          if (p.table) {
-            const int64_t pg = checked_page(p.table, b * p.tstride + jb + i, p.n_pages, p.err, 1008);
-            rec = (pg < 0 ? 0 : pg) * p.Hkv + kvh;
-          } else {
-            rec = row * p.nbc + (p.head_blk + jb + i) % p.nbc;
+  if (warp >= 24) {
+    fewer_regs<40>();
+    if (warp == 24) {
+      // ---------------------------------------------------- producer warp --
+      if (lane == 0) {
+        bool ok = true;
+        int issued = 0;
+        int64_t pb = (p.head_blk + t_begin * kTWarps) % p.nbc;
+        for (int j = 0; j < n && ok; ++j) {
+          if (j == (n < kPreRaw ? n - 1 : kPreRaw - 1)) {
+            // the first records are on their way; the queries come from the
+            // kernel before this one
+            tc::pdl_wait();
+            const uint8_t* img = p.qimg + ((row * p.rgroups + R0 / kPreRows) * (int64_t)kQImage);
+            tc::mbar_arrive_expect_tx(q_full, kQImage);
+            tc::bulk_g2s(sbase, img, kOperand, q_full);
+            tc::bulk_g2s(sbase + kPreOffQinfo, img + kOperand, kQImage - kOperand, q_full);
           }
-          tc::bulk_g2s(dst + i * kRecBytes, p.blocks + rec * kRecWords, kRecBytes,
-                       raw_full + 8 * s);
+          const int s = j % kPreRaw;
+          if (j >= kPreRaw)
+            ok = tc::mbar_wait_sleep(raw_empty + 8 * s, ((j / kPreRaw) - 1) & 1, p.err, 51);
+          if (!ok) break;
+          const int64_t jb = (t_begin + j) * kTWarps;
+          const int nb = nlb_b - jb < kTWarps ? (int)(nlb_b - jb) : kTWarps;
+          tc::mbar_arrive_expect_tx(raw_full + 8 * s, nb * kRecBytes);
+          const uint32_t dst = sbase + kPreOffRaw + s * kTStageBytes;
+          if (p.table) {
+            for (int i = 0; i < nb; ++i) {  // a bad table entry reads page 0 and is reported
+              const int64_t pg =
+                  checked_page(p.table, b * p.tstride + jb + i, p.n_pages, p.err, 1008);
+              tc::bulk_g2s(dst + i * kRecBytes,
+                           p.blocks + ((pg < 0 ? 0 : pg) * p.Hkv + kvh) * kRecWords, kRecBytes,
+                           raw_full + 8 * s);
+            }
+          } else {
+            // nb consecutive records from physical block pb, wrapping at most once
+            const int n1 = pb + nb <= p.nbc ? nb : (int)(p.nbc - pb);
+            tc::bulk_g2s(dst, p.blocks + (row * p.nbc + pb) * kRecWords, n1 * kRecBytes,
+                         raw_full + 8 * s);
+            if (n1 < nb)
+              tc::bulk_g2s(dst + n1 * kRecBytes, p.blocks + row * p.nbc * kRecWords,
+                           (nb - n1) * kRecBytes, raw_full + 8 * s);
+            pb += nb;
+            if (pb >= p.nbc) pb -= p.nbc;
+          }
+          ++issued;
         }
-        ++issued;
+        // the copies in flight must land before the CTA may exit
+        for (int j = issued - kPreRaw < 0 ? 0 : issued - kPreRaw; j < issued; ++j)
+          tc::mbar_wait_sleep(raw_full + 8 * (j % kPreRaw), (j / kPreRaw) & 1, p.err, 52);
+        tc::mbar_wait_sleep(q_full, 0, p.err, 52);
       }
-      // the copies in flight must land before the CTA may exit
-      for (int j = issued - kPreRaw < 0 ? 0 : issued - kPreRaw; j < issued; ++j)
-        tc::mbar_wait(raw_full + 8 * (j % kPreRaw), (j / kPreRaw) & 1, p.err, 52);
-    }
-  } else if (warp == 13) {
-    // ----------------------------------------------------------- MMA warp --
-    if (lane == 0) {
+    } else if (warp == 25) {
+      // --------------------------------------------------------- MMA warp --
+      // the warp stays together; one elected lane issues
       constexpr uint32_t idesc = tc::idesc_f16(128, 128);
-      bool ok = true;
+      uint32_t leader;
+      bool ok = tc::mbar_wait_sleep(q_full, 0, p.err, 50);
+      const uint64_t qd = tc::smem_desc_sw128(sbase);
       auto qk = [&](int j) {
         const int s = j & 1;
-        ok = tc::mbar_wait(k_full + 8 * s, (j >> 1) & 1, p.err, 53);
+        ok = tc::mbar_wait_sleep(k_full + 8 * s, (j >> 1) & 1, p.err, 53);
         if (!ok) return;
         tc::tc_fence_after();
-        const uint64_t qd = tc::smem_desc_sw128(sbase);
         const uint64_t kd = tc::smem_desc_sw128(sbase + kPreOffK + s * kOperand);
+        if (tc::elect_one(leader)) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
-          tc::mma_f16_ss(tS + 128 * s, qd + at, kd + at, idesc, k > 0);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
+            tc::mma_f16_ss(tS + 128 * s, qd + at, kd + at, idesc, k > 0);
+          }
+          tc::mma_commit(qk_done + 8 * s);
         }
-        tc::mma_commit(qk_done + 8 * s);
+        __syncwarp();
       };
       auto pv = [&](int j) {
         const int s = j & 1;
-        ok = tc::mbar_wait(p_full + 8 * s, (j >> 1) & 1, p.err, 54) &&
-             tc::mbar_wait(v_full + 8 * s, (j >> 1) & 1, p.err, 55);
+        ok = tc::mbar_wait_sleep(p_full + 8 * s, (j >> 1) & 1, p.err, 54) &&
+             tc::mbar_wait_sleep(v_full + 8 * s, (j >> 1) & 1, p.err, 55);
         if (!ok) return;
         tc::tc_fence_after();
         const uint64_t vd = tc::smem_desc_sw128(sbase + kPreOffV + s * kOperand);
+        if (tc::elect_one(leader)) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
-          tc::mma_f16_ts(tO + 128 * s, tS + 128 * s + 8 * k, vd + at, idesc, j >= 2 || k > 0);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
+            tc::mma_f16_ts(tO + 128 * s, tS + 128 * s + 8 * k, vd + at, idesc, j >= 2 || k > 0);
+          }
+          tc::mma_commit(pv_done + 8 * s);
         }
-        tc::mma_commit(pv_done + 8 * s);
+        __syncwarp();
       };
       // the MMAs of one thread run in order, so P of tile j is read before the
       // scores of tile j + 2 replace it
-      qk(0);
+      if (ok) qk(0);
       if (ok && n > 1) qk(1);
       for (int j = 0; j < n && ok; ++j) {
         pv(j);
         if (ok && j + 2 < n) qk(j + 2);
       }
-      tc::mma_commit(fin);  // nothing is in flight when the TMEM is freed
-      tc::mbar_wait(fin, 0, p.err, 56);
+      if (tc::elect_one(leader)) tc::mma_commit(fin);  // then nothing is in flight
+      __syncwarp();
+      tc::mbar_wait_sleep(fin, 0, p.err, 56);
+    } else {
+      // ----------------------------------------------------- factor warps --
+      // scores are st x product + kc x sum(q) (a code enters as 1 + c/8), values
+      // vst x product + vc x sum(p) (as (c - 3.5)/8)
+      const int half = warp - 26;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        ok = tc::mbar_wait_sleep(raw_full + 8 * (j % kPreRaw), (j / kPreRaw) & 1, p.err, 57);
+        if (ok && j >= 4) ok = tc::mbar_wait_sleep(fac_empty + 8 * (j & 3), ((j >> 2) - 1) & 1, p.err, 58);
+        if (!ok) break;
+        float* fac = reinterpret_cast<float*>(smem + kPreOffFac + (j & 3) * kFacBytes);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int w = 2 * half + i;
+          const uint32_t* rec = reinterpret_cast<const uint32_t*>(
+              smem + kPreOffRaw + (j % kPreRaw) * kTStageBytes + w * kRecBytes);
+          const float2 km = reinterpret_cast<const float2*>(rec + kRecKmm)[mm_index(lane)];
+          const float2 vm = reinterpret_cast<const float2*>(rec + kRecVmm)[mm_index(lane)];
+          const float ks = (km.y - km.x) * 0.14285714285714285f;
+          const float vs = (vm.y - vm.x) * 0.14285714285714285f;
+          const int oe = lane >> 3;
+          const int col = 32 * w + 8 * (lane & 3) + 4 * ((lane >> 2) & 1) +
+                          (oe == 1 ? 2 : (oe == 2 ? 1 : oe));
+          float* fp = fac + (col >> 1) * 8 + (col & 1);
+          fp[0] = ks;
+          fp[2] = fmaf(-8.0f, ks, km.x);
+          fp[4] = vs;
+          fp[6] = fmaf(3.5f, vs, vm.x);
+          int e = bound_exp(vs < INFINITY ? vs : 0.0f);
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, x));
+          if (lane == 0) reinterpret_cast<int*>(fac + 64 * 8)[w] = e;
+        }
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(fac_full + 8 * (j & 3));
+          tc::mbar_arrive(raw_empty + 8 * (j % kPreRaw));
+        }
+      }
     }
-  } else if (warp >= 8) {
-    // ---------------------------------------------------- converter warps --
-    const int w = warp - 8;
+  } else if (warp >= 16) {
+    // -------------------------------------------------- K' and V' warps --
+    // Four warps each, one record a warp.  The words go to registers first, so that
+    // the raw buffer is free for the tile after next while the operand's is awaited.
+    fewer_regs<56>();
+    const bool isv = warp >= 20;
+    const int w = warp & 3;
+    const int gk = ((g & 1) << 2) | (g >> 1);
+    const uint32_t full = isv ? v_full : k_full, done = isv ? pv_done : qk_done;
+    // K: the words of lane 4 gk + r, so that eight lanes of a store meet eight banks
+    const int words = w * kRecWords + (isv ? kRecV + lane * 12 : (4 * gk + r) * 12);
     bool ok = true;
-    const int gk = ((g & 1) << 2) | (g >> 1);  // K words of this lane: those of lane 4 gk + r
-    auto convert_k = [&](int j) {
-      ok = ok && tc::mbar_wait(raw_full + 8 * (j % kPreRaw), (j / kPreRaw) & 1, p.err, 57);
-      if (ok && j >= 2) ok = tc::mbar_wait(qk_done + 8 * (j & 1), ((j >> 1) - 1) & 1, p.err, 58);
-      if (ok && j >= 4) ok = tc::mbar_wait(fac_empty + 8 * (j & 3), ((j >> 2) - 1) & 1, p.err, 59);
-      if (!ok) return;
-      const uint32_t* rec = reinterpret_cast<const uint32_t*>(
-          smem + kPreOffRaw + (j % kPreRaw) * kTStageBytes + w * kRecBytes);
-      uint32_t kw[12];
+    for (int j = 0; j < n; ++j) {
+      ok = tc::mbar_wait_sleep(raw_full + 8 * (j % kPreRaw), (j / kPreRaw) & 1, p.err, 59);
+      if (!ok) break;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          reinterpret_cast<const uint32_t*>(smem + kPreOffRaw + (j % kPreRaw) * kTStageBytes) + words);
+      uint32_t wd[12];
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        const uint4 x = reinterpret_cast<const uint4*>(rec + (4 * gk + r) * 12)[i];
-        kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
+        const uint4 x = src[i];
+        wd[4 * i] = x.x, wd[4 * i + 1] = x.y, wd[4 * i + 2] = x.z, wd[4 * i + 3] = x.w;
       }
-      uint8_t* op = smem + kPreOffK + (j & 1) * kOperand;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // slot gk + 8e is row 32w + 8 (gk % 4) + 4 (gk / 4) + (0 2 1 3)[e]
-        const int sub = 4 * (gk >> 2) + (e == 1 ? 2 : (e == 2 ? 1 : e));
-        uint8_t* rowp = op + (32 * w + 8 * (gk & 3) + sub) * 128;
-        const uint32_t w0 = kw[3 * e], w1 = kw[3 * e + 1], w2 = kw[3 * e + 2];
-#define FT_PRE_K(I)                                                                          \
-  *reinterpret_cast<uint4*>(rowp + ((I) >> 1) * (kOperand / 2) +                              \
-                            (((4 * ((I) & 1) + r) ^ sub) << 4)) =                             \
-      make_uint4(quad_half2<2 * (I), 0>(w0, w1, w2), quad_half2<2 * (I), 1>(w0, w1, w2),      \
-                 quad_half2<2 * (I) + 1, 0>(w0, w1, w2), quad_half2<2 * (I) + 1, 1>(w0, w1, w2));
-        FT_PRE_K(0) FT_PRE_K(1) FT_PRE_K(2) FT_PRE_K(3)
-#undef FT_PRE_K
-      }
-      // factors of slot `lane`
-      const float2 km = reinterpret_cast<const float2*>(rec + kRecKmm)[mm_index(lane)];
-      const float2 vm = reinterpret_cast<const float2*>(rec + kRecVmm)[mm_index(lane)];
-      const float ks = (km.y - km.x) * 0.14285714285714285f;
-      const float vs = (vm.y - vm.x) * 0.14285714285714285f;
-      const int oe = lane >> 3;
-      const int col = 32 * w + 8 * (lane & 3) + 4 * ((lane >> 2) & 1) + (oe == 1 ? 2 : (oe == 2 ? 1 : oe));
-      float* fac = reinterpret_cast<float*>(smem + kPreOffFac + (j & 3) * kFacBytes);
-      float* fp = fac + (col >> 1) * 8 + (col & 1);
-      fp[0] = ks;
-      fp[2] = fmaf(-8.0f, ks, km.x);
-      fp[4] = vs;
-      fp[6] = fmaf(3.5f, vs, vm.x);
-      int e = bound_exp(vs < INFINITY ? vs : 0.0f);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, x));
-      if (lane == 0) reinterpret_cast<int*>(fac + 64 * 8)[w] = e;
-      tc::fence_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(k_full + 8 * (j & 1));
-    };
-    auto convert_v = [&](int j) {
-      if (ok && j >= 2) ok = tc::mbar_wait(pv_done + 8 * (j & 1), ((j >> 1) - 1) & 1, p.err, 60);
-      if (!ok) return;
-      const uint32_t* rec = reinterpret_cast<const uint32_t*>(
-          smem + kPreOffRaw + (j % kPreRaw) * kTStageBytes + w * kRecBytes);
-      uint32_t vw[12];
+      if (lane == 0) tc::mbar_arrive(raw_empty + 8 * (j % kPreRaw));
+      if (j >= 2) ok = tc::mbar_wait_sleep(done + 8 * (j & 1), ((j >> 1) - 1) & 1, p.err, 60);
+      if (!ok) break;
+      if (isv) {
+        // triple m: dim 8 (4m + J) + g is row 8 (4m + J) + gk; chunk 4 (w % 2) + r of panel w / 2
+        uint8_t* at = smem + kPreOffV + (j & 1) * kOperand + (w >> 1) * (kOperand / 2) + gk * 128 +
+                      (((4 * (w & 1) + r) ^ gk) << 4);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const uint4 x = reinterpret_cast<const uint4*>(rec + kRecV + lane * 12)[i];
-        vw[4 * i] = x.x, vw[4 * i + 1] = x.y, vw[4 * i + 2] = x.z, vw[4 * i + 3] = x.w;
-      }
-      // dim 8t + g is row 8t + gk; chunk 4 (w % 2) + r of panel w / 2
-      uint8_t* op = smem + kPreOffV + (j & 1) * kOperand + (w >> 1) * (kOperand / 2) + gk * 128 +
-                    (((4 * (w & 1) + r) ^ gk) << 4);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const uint32_t w0 = vw[3 * m], w1 = vw[3 * m + 1], w2 = vw[3 * m + 2];
-#define FT_PRE_V(J)                                                                                \
-  *reinterpret_cast<uint4*>(op + (4 * m + (J)) * 1024) =                                            \
-      make_uint4(quad_centred<2 * (J), 0>(w0, w1, w2), quad_centred<2 * (J), 1>(w0, w1, w2),        \
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t w0 = wd[3 * m], w1 = wd[3 * m + 1], w2 = wd[3 * m + 2];
+#define FT_PRE_V(J)                                                                                 \
+  *reinterpret_cast<uint4*>(at + (4 * m + (J)) * 1024) =                                             \
+      make_uint4(quad_centred<2 * (J), 0>(w0, w1, w2), quad_centred<2 * (J), 1>(w0, w1, w2),         \
                  quad_centred<2 * (J) + 1, 0>(w0, w1, w2), quad_centred<2 * (J) + 1, 1>(w0, w1, w2));
-        FT_PRE_V(0) FT_PRE_V(1) FT_PRE_V(2) FT_PRE_V(3)
+          FT_PRE_V(0) FT_PRE_V(1) FT_PRE_V(2) FT_PRE_V(3)
 #undef FT_PRE_V
+        }
+      } else {
+        // slot gk + 8e is row 32w + 8 (gk % 4) + 4 (gk / 4) + (0 2 1 3)[e]; quads 2J, 2J + 1 go to
+        // chunk 4 (J % 2) + r of panel J / 2
+        uint8_t* op = smem + kPreOffK + (j & 1) * kOperand + (32 * w + 8 * (gk & 3)) * 128;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t w0 = wd[3 * e], w1 = wd[3 * e + 1], w2 = wd[3 * e + 2];
+          const int sub = 4 * (gk >> 2) + ((e & 1) << 1 | e >> 1);
+          uint8_t* a0 = op + sub * 128 + ((r ^ sub) << 4);
+          uint8_t* a1 = op + sub * 128 + (((r + 4) ^ sub) << 4);
+#define FT_PRE_K(J, AT)                                                                  \
+  *reinterpret_cast<uint4*>(AT) =                                                         \
+      make_uint4(quad_half2<2 * (J), 0>(w0, w1, w2), quad_half2<2 * (J), 1>(w0, w1, w2),  \
+                 quad_half2<2 * (J) + 1, 0>(w0, w1, w2), quad_half2<2 * (J) + 1, 1>(w0, w1, w2));
+          FT_PRE_K(0, a0) FT_PRE_K(1, a1) FT_PRE_K(2, a0 + kOperand / 2) FT_PRE_K(3, a1 + kOperand / 2)
+#undef FT_PRE_K
+        }
       }
       tc::fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        tc::mbar_arrive(v_full + 8 * (j & 1));
-        tc::mbar_arrive(raw_empty + 8 * (j % kPreRaw));
-      }
-    };
-    convert_k(0);
-    for (int j = 0; j < n && ok; ++j) {
-      if (j + 1 < n) convert_k(j + 1);
-      convert_v(j);
+      if (lane == 0) tc::mbar_arrive(full + 8 * (j & 1));
     }
   } else {
-    // ------------------------------------------------------ softmax warps --
-    const int st = warp >> 2, quad = warp & 3;
-    const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-    const bool live = 32 * quad < nrows;  // this warp's rows exist
-    // rows 32 quad + 8 i + g, i = 0..3
-    uint64_t qsum[4], qfac[4], l2[4], vm2[4], negM[4];
-    float M[4];
+    // ------------------------------------------------------- softmax warps --
+    more_regs<88>();
+    const float* qinfo = reinterpret_cast<const float*>(smem + kPreOffQinfo);
+    const uint64_t* qmask = reinterpret_cast<const uint64_t*>(smem + kPreOffMask);
+    bool ok = tc::mbar_wait_sleep(q_full, 0, p.err, 67);
+    // warp: tiles st, st + 2, ..; lanes 32 quad + 16 half + {g, g + 8} (see row_lane)
+    const int st = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    const uint32_t lanes = (uint32_t)(32 * quad + 16 * half) << 16;
+    const int row0 = 32 * quad + 16 * half + g;
+    const bool live = 64 * half + 16 * quad < nrows;  // this warp's rows exist
+    // 32-bit slot arithmetic: the host keeps head_off + len below 2^31 - 64
+    const int hoff = p.table ? 0 : (int)p.head_off, len32 = (int)len_b;
+    const int P = len32 - p.T;  // prefix length; negative: the first drafts do not exist
+    uint64_t qsum[2], qfac[2], l2[2], vm2[2], negM[2];
+    bool unset = true;  // a row has no reference yet (warp-uniform)
+    uint32_t have = 0;  // bit i: row i has one
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 32 * quad + 8 * i + g;
-      qsum[i] = pair(qinfo[at], qinfo[at]);
-      qfac[i] = pair(qinfo[kPreRows + at], qinfo[kPreRows + at]);
-      l2[i] = vm2[i] = pair(0.0f, 0.0f);
-      M[i] = -INFINITY;
-      negM[i] = pair(0.0f, 0.0f);
+    for (int i = 0; i < 2; ++i) {
+      const float a = qinfo[row0 + 8 * i], f = qinfo[kPreRows + row0 + 8 * i];
+      qsum[i] = pair(a, a);
+      qfac[i] = pair(f, f);
+      l2[i] = vm2[i] = negM[i] = pair(0.0f, 0.0f);
     }
-    bool ok = true;
-    for (int j = st; j < n; j += 2) {
-      ok = ok && tc::mbar_wait(k_full + 8 * st, (j >> 1) & 1, p.err, 61) &&
-           tc::mbar_wait(qk_done + 8 * st, (j >> 1) & 1, p.err, 62);
-      if (!ok) break;
-      tc::tc_fence_after();
+    // One tile: P of this warp's rows.  Two instances: with kMasked each score is
+    // tested against the mask (the tiles at the sequence's ends), so that the
+    // prefix's loop stays small.
+    auto tile = [&](auto masked, int j) {
+      constexpr bool kMasked = decltype(masked)::value;
       const uint32_t ts = tS + 128 * st + lanes;
       const float* fac = reinterpret_cast<const float*>(smem + kPreOffFac + (j & 3) * kFacBytes);
-      if (live) {
+      uint32_t sv[16];
+      tc::tmem_ld_16x256b_x4(ts, sv);
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          // 32 positions (a record): x[2 i' + half][...] of rows 16 hf + g, + 8
-          uint32_t sv[2][16];
-          tc::tmem_ld_16x256b_x4(ts + 32 * c, sv[0]);
-          tc::tmem_ld_16x256b_x4(ts + (16u << 16) + 32 * c, sv[1]);
-          tc::tmem_wait_ld();
-          const float4* f4 = reinterpret_cast<const float4*>(fac) + (16 * c + r) * 2;
-          uint64_t x[2][4][2];  // [rows 16 hf + g | + 8][k][.] : pair of positions 8k + 2r, + 1
-          float top = -INFINITY;
+      for (int c = 0; c < 4; ++c) {
+        // 32 positions (a record); x[k][i]: row i, positions 8k + 2r, + 1
+        const float4* f4 = reinterpret_cast<const float4*>(fac) + (16 * c + r) * 2;
+        const float eb = (float)(15 - reinterpret_cast<const int*>(fac + 64 * 8)[c]);
+        uint64_t x[4][2];
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 kf = f4[8 * k];
+          const uint64_t ks = pair(kf.x, kf.y), kc = pair(kf.z, kf.w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t s2 = pair(__uint_as_float(sv[4 * k + 2 * i]),
+                                     __uint_as_float(sv[4 * k + 2 * i + 1]));
+            x[k][i] = fma2(ks, mul2(s2, qfac[i]), fma2(kc, qsum[i], negM[i]));
+          }
+        }
+        if (c < 3) tc::tmem_ld_16x256b_x4(ts + 32 * (c + 1), sv);  // the next record's scores
+        float bound[2] = {eb, eb}, m[2];
+        if (kMasked) {
+          // position 8k + 2r + o of the record is slot k + 4 (r / 2) + 8 (r % 2) + 16 o
+          const int base = ((int)(t_begin + j) * kTWarps + c) * kBlk - hoff;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t mask = qmask[row0 + 8 * i];
+            int e = -85;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpair(x[k][i]);
+              const float4 vf = f4[8 * k + 1];
+              const int p0 = base + k + 4 * (r >> 1) + 8 * (r & 1), p1 = p0 + 16;
+              const bool s0 = p0 >= 0 && p0 < len32 && (p0 < P || ((mask >> (p0 - P)) & 1ull));
+              const bool s1 = p1 >= 0 && p1 < len32 && (p1 < P || ((mask >> (p1 - P)) & 1ull));
+              if (s0) e = max(e, bound_exp(vf.x < INFINITY ? vf.x : 0.0f));
+              if (s1) e = max(e, bound_exp(vf.y < INFINITY ? vf.y : 0.0f));
+              x[k][i] = pair(s0 ? f.x : -INFINITY, s1 ? f.y : -INFINITY);
+            }
+            // what a row sees bounds it, not what masked places hold
+            e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+            e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+            bound[i] = (float)(15 - e);
+          }
+        }
+        bool above = unset;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float t[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float4 kf = f4[8 * k];
-            const uint64_t ks = pair(kf.x, kf.y), kc = pair(kf.z, kf.w);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int i = 2 * hf + u;
-                const uint64_t s2 = pair(__uint_as_float(sv[hf][4 * k + 2 * u]),
-                                         __uint_as_float(sv[hf][4 * k + 2 * u + 1]));
-                const uint64_t y = fma2(ks, mul2(s2, qfac[i]), fma2(kc, qsum[i], negM[i]));
-                x[hf][k][u] = y;
-                const float2 f = unpair(y);
-                top = fmaxf(top, fmaxf(f.x, f.y));
-              }
+            const float2 f = unpair(x[k][i]);
+            t[k] = fmaxf(f.x, f.y);
           }
-          const int e = reinterpret_cast<const int*>(fac + 64 * 8)[c];
-          const float bound = (float)(15 - e);
-          const bool first = j == st && c == 0;
-          if (__any_sync(0xffffffffu, top > bound) || first) {
-            // a score above its row's bound (or the first ones): new references
-            float alpha[4];
+          m[i] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          above |= m[i] > bound[i];
+        }
+        if (__builtin_expect(__any_sync(0xffffffffu, above), 0)) {
+          // a score above its row's bound, or a row's first: new references
+          float alpha[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float m = -INFINITY;
+          for (int i = 0; i < 2; ++i) {
+            m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
+            m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 2));
+            const bool first = !((have >> i) & 1u);
+            // x - M so far; up by the whole steps that put the maximum 8 below the bound
+            float up = first || m[i] > bound[i] ? ceilf(m[i] - (bound[i] - 8.0f)) : 0.0f;
+            // nothing seen yet, or NaN or infinite scores (the row then ends NaN)
+            if (!(fabsf(up) < 1e30f)) up = 0.0f;
+            else if (first) have |= 1u << i;
+            alpha[i] = first ? 1.0f : exp2f(-up);  // nothing is summed before the first
+            const uint64_t a2 = pair(alpha[i], alpha[i]), u2 = pair(-up, -up);
+            negM[i] = add2(negM[i], u2);
+            l2[i] = mul2(l2[i], a2);
+            vm2[i] = mul2(vm2[i], a2);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 f = unpair(x[i >> 1][k][i & 1]);
-                m = fmaxf(m, fmaxf(f.x, f.y));
+            for (int k = 0; k < 4; ++k) x[k][i] = add2(x[k][i], u2);
+          }
+          unset = __any_sync(0xffffffffu, have != 3u);
+          if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+            tc::tmem_wait_ld();
+            tc::tmem_wait_st();
+#pragma unroll 1
+            for (int k = 0; k < c; ++k) {  // P columns of this tile
+              uint32_t t[8];
+              tc::tmem_ld_16x256b_x2(ts + 16 * k, t);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&t[q]),
+                                          __float2half2_rn(alpha[(q >> 1) & 1]));
+                t[q] = *reinterpret_cast<const uint32_t*>(&h);
               }
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-              // x - M so far; up by the whole steps that put the maximum 8 below the bound
-              float up = first || m > bound ? ceilf(m - (bound - 8.0f)) : 0.0f;
-              // NaN or infinite scores: the row ends NaN whatever its reference
-              if (!(fabsf(up) < 1e30f)) up = 0.0f;
-              alpha[i] = first ? 1.0f : exp2f(-up);  // nothing is summed yet
-              M[i] = first ? up : M[i] + up;
-              negM[i] = pair(-M[i], -M[i]);
-              const uint64_t a2 = pair(alpha[i], alpha[i]), u2 = pair(-up, -up);
-              l2[i] = mul2(l2[i], a2);
-              vm2[i] = mul2(vm2[i], a2);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) x[i >> 1][k][i & 1] = add2(x[i >> 1][k][i & 1], u2);
+              tc::tmem_st_16x256b_x2(ts + 16 * k, t);
             }
-            if (!first) {
-              // alpha of TMEM lane `lane` of this warp: row 8 i + g' lies in thread 4 g'
-              float al = 1.0f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float a = __shfl_sync(0xffffffffu, alpha[i], 4 * (lane & 7));
-                if ((lane >> 3) == i) al = a;
-              }
-              const __half2 al2 = __float2half2_rn(al);
-              tc::tmem_wait_st();
-              for (int k = 0; k < c; ++k) {  // P columns of this tile
-                uint32_t t[16];
-                tc::tmem_ld_x16(ts + 16 * k, t);
+            if (j >= 2) {  // O, once the product of tile j - 2 is in it
+              ok = ok && tc::mbar_wait_sleep(pv_done + 8 * st, ((j >> 1) - 1) & 1, p.err, 65);
+              tc::tc_fence_after();
+#pragma unroll 1
+              for (int k = 0; ok && k < 8; ++k) {
+                uint32_t t[8];
+                tc::tmem_ld_16x256b_x2(tO + 128 * st + lanes + 16 * k, t);
                 tc::tmem_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&t[q]), al2);
-                  t[q] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-                tc::tmem_st_x16(ts + 16 * k, t);
+                for (int q = 0; q < 8; ++q)
+                  t[q] = __float_as_uint(__uint_as_float(t[q]) * alpha[(q >> 1) & 1]);
+                tc::tmem_st_16x256b_x2(tO + 128 * st + lanes + 16 * k, t);
               }
-              if (j >= 2) {  // O, once the product of tile j - 2 is in it
-                ok = ok && tc::mbar_wait(pv_done + 8 * st, ((j >> 1) - 1) & 1, p.err, 63);
-                tc::tc_fence_after();
-                for (int k = 0; ok && k < 8; ++k) {
-                  uint32_t t[16];
-                  tc::tmem_ld_x16(tO + 128 * st + lanes + 16 * k, t);
-                  tc::tmem_wait_ld();
-#pragma unroll
-                  for (int q = 0; q < 16; ++q) t[q] = __float_as_uint(__uint_as_float(t[q]) * al);
-                  tc::tmem_st_x16(tO + 128 * st + lanes + 16 * k, t);
-                }
-              }
-              tc::tmem_wait_st();
             }
+            tc::tmem_wait_st();
           }
-          uint32_t pw[2][8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float4 vf = f4[8 * k + 1];
-            const uint64_t vs = pair(vf.x, vf.y), vc = pair(vf.z, vf.w);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int i = 2 * hf + u;
-                const float2 f = unpair(x[hf][k][u]);
-                const uint64_t pr = pair(ex2(f.x), ex2(f.y));
-                l2[i] = add2(l2[i], pr);
-                vm2[i] = fma2(pr, vc, vm2[i]);
-                const float2 wt = unpair(mul2(pr, vs));
-                pw[hf][2 * k + u] = pack_half2(wt.x, wt.y);
-              }
-          }
-          tc::tmem_st_16x128b_x4(ts + 16 * c, pw[0]);
-          tc::tmem_st_16x128b_x4(ts + (16u << 16) + 16 * c, pw[1]);
         }
-        tc::tmem_wait_st();
+        uint32_t pw[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 vf = f4[8 * k + 1];
+          const uint64_t vs = pair(vf.x, vf.y), vc = pair(vf.z, vf.w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 f = unpair(x[k][i]);
+            const uint64_t pr = pair(ex2(f.x), ex2(f.y));
+            l2[i] = add2(l2[i], pr);
+            float2 wt = unpair(mul2(pr, vs));
+            if (!kMasked) {
+              vm2[i] = fma2(pr, vc, vm2[i]);
+            } else {  // whatever V holds in masked places
+              float2 vt = unpair(mul2(pr, vc));
+              if (f.x == -INFINITY) wt.x = vt.x = 0.0f;
+              if (f.y == -INFINITY) wt.y = vt.y = 0.0f;
+              vm2[i] = add2(vm2[i], pair(vt.x, vt.y));
+            }
+            pw[2 * k + i] = pack_half2(wt.x, wt.y);
+          }
+        }
+        tc::tmem_st_16x128b_x4(ts + 16 * c, pw);
+      }
+      tc::tmem_wait_st();
+    };
+    for (int j = st; j < n; j += 2) {
+      ok = ok && tc::mbar_wait_sleep(fac_full + 8 * (j & 3), (j >> 2) & 1, p.err, 63) &&
+           tc::mbar_wait_sleep(qk_done + 8 * st, (j >> 1) & 1, p.err, 64);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (live) {
+        const int base = (int)(t_begin + j) * (kTWarps * kBlk) - hoff;
+        if (base < 0 || base + kTWarps * kBlk > P) tile(Masked<true>(), j);
+        else tile(Masked<false>(), j);
       }
       tc::tc_fence_before();
       __syncwarp();
@@ -1070,14 +1189,13 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
         tc::mbar_arrive(fac_empty + 8 * (j & 3));
       }
     }
-    // ---- the two groups merge: row statistics in the raw buffers, the odd
-    // group's numerators in the operand buffers (all products are done)
-    const int mine = st < n ? (n - st + 1) / 2 : 0;  // tiles of this group
-    if (ok) ok = tc::mbar_wait(fin, 0, p.err, 64);
+    // ---- the two groups merge: row statistics in the raw buffers, numerators in
+    // the operand buffers (every product is done)
+    if (ok) ok = tc::mbar_wait_sleep(fin, 0, p.err, 66);
     tc::tc_fence_after();
-    float* stat = reinterpret_cast<float*>(smem + kPreOffRaw) + st * kPreRows * 3;
+    float* stats = reinterpret_cast<float*>(smem + kPreOffRaw);  // [group][row]: M, l, sum term
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const float2 lf = unpair(l2[i]), vf = unpair(vm2[i]);
       float l = lf.x + lf.y, v = vf.x + vf.y;
 #pragma unroll
@@ -1086,104 +1204,112 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
         v += __shfl_xor_sync(0xffffffffu, v, x);
       }
       if (r == 0) {
-        float* t = stat + (32 * quad + 8 * i + g) * 3;
-        t[0] = mine > 0 ? M[i] : -INFINITY;
+        float* t = stats + (st * kPreRows + row0 + 8 * i) * 3;
+        t[0] = l == 0.0f ? -INFINITY : -unpair(negM[i]).x;  // l == 0: the group saw nothing
         t[1] = l;
         t[2] = v;
       }
     }
-    float* area = reinterpret_cast<float*>(smem + kPreOffK);
-    const int myrow = 32 * quad + lane;
-    float* arow = area + myrow * kMergeStride;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float* s0 = reinterpret_cast<const float*>(smem + kPreOffRaw) + myrow * 3;
-    const float* s1 = s0 + kPreRows * 3;
-    const float M0 = s0[0], M1 = s1[0], Mx = fmaxf(M0, M1);
-    const float f0 = M0 == -INFINITY ? 0.0f : exp2f(M0 - Mx);
-    const float f1 = M1 == -INFINITY ? 0.0f : exp2f(M1 - Mx);
-    const float f = st ? f1 : f0, vterm = st ? s1[2] : s0[2];
-    for (int pass = 1; pass >= 0; --pass) {  // the odd group stores, then the even one adds
-      if (st == pass && live) {
-        for (int k = 0; k < 8; ++k) {
-          uint32_t t[16];
-          if (mine > 0) {
-            tc::tmem_ld_x16(tO + 128 * st + lanes + 16 * k, t);
-            tc::tmem_wait_ld();
-          }
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    const int myrow = 32 * quad + lane;  // here a warp takes 32 rows and half the dims
+    if (16 * quad < nrows) {
+      const float* mine = stats + (st * kPreRows + myrow) * 3;
+      const float Mx = fmaxf(stats[myrow * 3], stats[(kPreRows + myrow) * 3]);
+      const bool some = st < n && mine[0] != -INFINITY;
+      const float f = some ? exp2f(mine[0] - Mx) : 0.0f, vterm = mine[2];
+      float* arow = reinterpret_cast<float*>(smem) + st * kMergeArea + myrow * kMergeStride;
+#pragma unroll 1
+      for (int k = 4 * half; k < 4 * half + 4; ++k) {
+        uint32_t t[16];
+        tc::tmem_ld_x16(tO + 128 * st + ((uint32_t)(32 * quad) << 16) + 16 * k, t);
+        tc::tmem_wait_ld();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // column 8t' + ((d % 2) * 4 + d / 2) holds dim 8t' + d
-            float o[8];
+        for (int h = 0; h < 2; ++h) {
+          // column 8t' + 4 (d % 2) + d / 2 holds dim 8t' + d
+          float o[8];
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
-              o[d] = mine > 0 ? f * fmaf(8.0f, __uint_as_float(t[8 * h + (d & 1) * 4 + (d >> 1)]), vterm)
-                              : 0.0f;
-            float4* dst = reinterpret_cast<float4*>(arow + 16 * k + 8 * h);
-            float4 a = make_float4(o[0], o[1], o[2], o[3]), c = make_float4(o[4], o[5], o[6], o[7]);
-            if (pass == 0) {
-              const float4 x = dst[0], y = dst[1];
-              a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-              c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
-            }
-            dst[0] = a;
-            dst[1] = c;
+          for (int d = 0; d < 8; ++d) {
+            const float v = __uint_as_float(t[8 * h + (d & 1) * 4 + (d >> 1)]);
+            o[d] = some ? f * fmaf(8.0f, v, vterm) : 0.0f;
           }
+          float4* dst = reinterpret_cast<float4*>(arow + 16 * k + 8 * h);
+          dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+          dst[1] = make_float4(o[4], o[5], o[6], o[7]);
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
     }
+    tc::tc_fence_before();
+    asm volatile("bar.sync 1, 512;" ::: "memory");
     // partial records, one warp a row
-    for (int i = warp; i < nrows; i += 8) {
-      const float* t0 = reinterpret_cast<const float*>(smem + kPreOffRaw) + i * 3;
+    for (int i = warp; i < nrows; i += 16) {
+      const int at = row_lane(i);
+      const float* t0 = stats + at * 3;
       const float* t1 = t0 + kPreRows * 3;
       const float mx = fmaxf(t0[0], t1[0]);
       const float a0 = t0[0] == -INFINITY ? 0.0f : exp2f(t0[0] - mx) * t0[1];
       const float a1 = t1[0] == -INFINITY ? 0.0f : exp2f(t1[0] - mx) * t1[1];
       float* pp = part + (int64_t)i * p.nparts * kTPart;
       if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(mx, a0 + a1);
-      const float4 v = reinterpret_cast<const float4*>(area + i * kMergeStride)[lane];
+      const float4* a = reinterpret_cast<const float4*>(smem) + at * (kMergeStride / 4) + lane;
+      const float4 v = a[0], w = a[kMergeArea / 4];
       float2* pn = reinterpret_cast<float2*>(pp + 2) + 2 * lane;
-      pn[0] = make_float2(v.x, v.y);
-      pn[1] = make_float2(v.z, v.w);
+      pn[0] = make_float2(v.x + w.x, v.y + w.y);
+      pn[1] = make_float2(v.z + w.z, v.w + w.w);
     }
-    tc::tc_fence_before();
   }
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 25) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
 }
 
-// Merges the split partials of one row, one warp a row (4 dims a lane); mode T:
-// the output is rotated back.  Bound by the partials' bytes (520 a split).
+// Merges the split partials of a row: one CTA a row, its warps share the splits
+// (so that all loads are in flight at once; a warp a row took 13 us over 512 rows x
+// 17 splits, this 4), 4 dims a lane; mode T: the output is rotated back.
 constexpr int kCombineWarps = 4;
 __global__ void __launch_bounds__(32 * kCombineWarps)
-    tree_combine_kernel(const __grid_constant__ TreeParams p, int64_t total,
-                        void* __restrict__ out) {
-  const int nsplit = p.nparts;
-  const int lane = threadIdx.x & 31;
-  const int64_t R = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
-  if (R >= total) return;
+    tree_combine_kernel(const __grid_constant__ TreeParams p, void* __restrict__ out) {
+  __shared__ float sm[kCombineWarps][2 + kD];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nsplit = p.nparts;
+  const int64_t R = blockIdx.x;
   const float* pp = p.part + R * nsplit * kTPart;
-  float M = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, pp[(int64_t)s * kTPart]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float M = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
+  for (int s = warp; s < nsplit; s += kCombineWarps) {
     const float* ps = pp + (int64_t)s * kTPart;
     const float2 ml = *reinterpret_cast<const float2*>(ps);
     const float2 a = reinterpret_cast<const float2*>(ps + 2)[2 * lane];
     const float2 c = reinterpret_cast<const float2*>(ps + 2)[2 * lane + 1];
     if (ml.x == -INFINITY) continue;
-    const float f = exp2f(ml.x - M);
-    l = fmaf(f, ml.y, l);
-    v[0] = fmaf(f, a.x, v[0]);
-    v[1] = fmaf(f, a.y, v[1]);
-    v[2] = fmaf(f, c.x, v[2]);
-    v[3] = fmaf(f, c.y, v[3]);
+    const float Mn = fmaxf(M, ml.x);
+    const float f0 = exp2f(M - Mn), f = exp2f(ml.x - Mn);  // M = -inf at first: 0
+    M = Mn;
+    l = fmaf(f, ml.y, l * f0);
+    v[0] = fmaf(f, a.x, v[0] * f0);
+    v[1] = fmaf(f, a.y, v[1] * f0);
+    v[2] = fmaf(f, c.x, v[2] * f0);
+    v[3] = fmaf(f, c.y, v[3] * f0);
+  }
+  if (lane == 0) {
+    sm[warp][0] = M;
+    sm[warp][1] = l;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sm[warp][2 + 32 * k + lane] = v[k];
+  __syncthreads();
+  if (warp != 0) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) M = fmaxf(M, sm[w][0]);
+  l = v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) {
+    if (sm[w][0] == -INFINITY) continue;
+    const float f = exp2f(sm[w][0] - M);
+    l = fmaf(f, sm[w][1], l);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = fmaf(f, sm[w][2 + 32 * k + lane], v[k]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : v[k] / l;  // 0: the row saw nothing
@@ -1214,17 +1340,16 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
 
 // Opts the kernels into their dynamic shared memory (once per device) and
 // returns the resident CTAs per SM.
-template <int kTerms>
 int tree_occupancy(int device) {
   static int cached[64] = {0};
   if (device >= 0 && device < 64 && cached[device]) return cached[device];
-  cudaFuncSetAttribute(tree_decode_kernel<kTerms>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       tree_smem(kTerms));
-  cudaFuncSetAttribute(tree_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
+  cudaFuncSetAttribute(tree_decode_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       tree_smem(2));
+  cudaFuncSetAttribute(tree_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
   int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel<kTerms>,
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel<2>,
                                                     (kTWarps + 1) * 32,
-                                                    tree_smem(kTerms)) != cudaSuccess ||
+                                                    tree_smem(2)) != cudaSuccess ||
       occ < 1)
     occ = 1;
   if (device >= 0 && device < 64) cached[device] = occ;
@@ -1246,8 +1371,7 @@ int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t ove
   return best;
 }
 
-constexpr int64_t kPreMinTiles = 1;
-constexpr int64_t kPreOverhead = 6;
+constexpr int64_t kPreOverhead = 3;
 
 template <class Cache>
 int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_draft,
@@ -1269,7 +1393,6 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
   p.G = (int)(q_heads / c->kv_heads);
   p.T = (int)n_draft;
   p.rows = p.T * p.G;
-  p.rgroups = (p.rows + kRows - 1) / kRows;
   p.mask = mask_dev;
   p.nlb = (p.head_off + p.len + kBlk - 1) / kBlk;
   const float sc = scale > 0.0f ? scale : 1.0f / sqrtf((float)kD);
@@ -1277,49 +1400,46 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
   p.blocks = c->blocks;
   p.signs = c->signs;
   p.err = ctx->err_word;
+  const int64_t total = batch * p.Hkv * p.rows;
+  const int64_t ntiles = ceil_div(p.nlb, (int64_t)kTWarps);
+  const int occ = tree_occupancy(ctx->device);
+  const int crows = q_is_bf16 ? kPreRows : kRows;
+  p.rgroups = (p.rows + crows - 1) / crows;
   FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
            "decode grid too large");
-  // the longest sequence's whole prefix tiles; they go to the tensor-core kernel
-  // from kPreMinTiles on
-  const int64_t first = p.head_off ? 1 : 0;
-  const int64_t pre_tiles = ((p.head_off + p.len - p.T) / kBlk - first) / kTWarps;
-  const int64_t total = batch * p.Hkv * p.rows;
-  p.edge = q_is_bf16 && pre_tiles >= kPreMinTiles ? 1 : 0;
-  const int occ = q_is_bf16 ? tree_occupancy<1>(ctx->device) : tree_occupancy<2>(ctx->device);
-  int64_t nsplit = 1;
-  if (p.edge) {
-    TreeParams pp = p;
-    pp.rgroups = (p.rows + kPreRows - 1) / kPreRows;
-    pp.tiles_per = split_tiles(batch * p.Hkv * pp.rgroups, pre_tiles, ctx->num_sms, kPreOverhead);
-    nsplit = ceil_div(pre_tiles, pp.tiles_per);
-    p.nparts = pp.nparts = (int)nsplit + 1;
-    const int rc = ensure_ws(c->tree, (size_t)(total * p.nparts * kTPart) * 4, s, "tree partials",
-                             c->retired);
-    if (rc != FT_OK) return rc;
-    p.part = pp.part = static_cast<float*>(c->tree.ptr);
-    dim3 grid((unsigned)nsplit, (unsigned)(p.Hkv * pp.rgroups), (unsigned)batch);
-    tree_prefix_kernel<<<grid, kPreWarps * 32, kPreSmem, s>>>(pp);
+  p.tiles_per = q_is_bf16
+                    ? split_tiles(batch * p.Hkv * p.rgroups, ntiles, ctx->num_sms, kPreOverhead)
+                    : split_tiles(batch * p.Hkv * p.rgroups, ntiles, (int64_t)occ * ctx->num_sms, 2);
+  p.nparts = (int)ceil_div(ntiles, p.tiles_per);
+  const int64_t tiles = batch * p.Hkv * p.rgroups;
+  const size_t images = q_is_bf16 ? (size_t)tiles * kQImage : 0;
+  FT_CHECK(total < INT32_MAX && tiles < INT32_MAX / 4, FT_ERR_UNSUPPORTED, "too many query rows");
+  const int rc = ensure_ws(c->tree, images + (size_t)(total * p.nparts * kTPart) * 4, s,
+                           "tree decode", c->retired);
+  if (rc != FT_OK) return rc;
+  p.qimg = static_cast<uint8_t*>(c->tree.ptr);
+  p.part = reinterpret_cast<float*>(p.qimg + images);
+  dim3 grid((unsigned)p.nparts, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
+  if (q_is_bf16) {
+    tree_query_kernel<<<(unsigned)(tiles * (kPreRows / kQueryRows)), 256, 0, s>>>(p);
     FT_LAUNCH_CHECK();
-    p.tiles_per = ceil_div(p.nlb, (int64_t)kTWarps);  // the edges are one split
-    nsplit = 1;
+    // starts while the query kernel runs, and waits for it before it reads the images
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kPreWarps * 32);
+    cfg.dynamicSmemBytes = kPreSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    FT_CUDA(cudaLaunchKernelEx(&cfg, tree_tile_kernel, p));
   } else {
-    const int64_t ntiles = ceil_div(p.nlb, (int64_t)kTWarps);
-    p.tiles_per = split_tiles(batch * p.Hkv * p.rgroups, ntiles, (int64_t)occ * ctx->num_sms, 2);
-    nsplit = ceil_div(ntiles, p.tiles_per);
-    p.nparts = (int)nsplit;
-    const int rc = ensure_ws(c->tree, (size_t)(total * p.nparts * kTPart) * 4, s, "tree partials",
-                             c->retired);
-    if (rc != FT_OK) return rc;
-    p.part = static_cast<float*>(c->tree.ptr);
-  }
-  dim3 grid((unsigned)nsplit, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
-  if (q_is_bf16)
-    tree_decode_kernel<1><<<grid, (kTWarps + 1) * 32, tree_smem(1), s>>>(p);
-  else
     tree_decode_kernel<2><<<grid, (kTWarps + 1) * 32, tree_smem(2), s>>>(p);
+  }
   FT_LAUNCH_CHECK();
-  tree_combine_kernel<<<(unsigned)ceil_div(total, (int64_t)kCombineWarps), 32 * kCombineWarps, 0,
-                        s>>>(p, total, out_dev);
+  tree_combine_kernel<<<(unsigned)total, 32 * kCombineWarps, 0, s>>>(p, out_dev);
   FT_LAUNCH_CHECK();
   return FT_OK;
 }
