@@ -14,6 +14,7 @@
 #include <cooperative_groups.h>
 
 #include "ft_kv3.cuh"
+#include "ft_tc.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -31,9 +32,10 @@ struct SelectParams {
   int* err;
 };
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBins = 2048;
+static_assert(kSelBins == 2 * kSelThreads, "two bins a thread");
 constexpr int kSelKeys = 40960;  // keys held in shared memory; further ones are read again
 constexpr int kSelSmem = kSelBins * 4 + 4 * 64 * 4;
 
@@ -57,6 +59,10 @@ __global__ void __launch_bounds__(kSelThreads)
   uint32_t* keys = bc + 192;         // [cap]
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  auto meet = [&]() {  // a cluster of one needs no cluster barrier
+    if (C > 1) cl.sync();
+    else __syncthreads();
+  };
   const int64_t row = blockIdx.x / C;
   const int64_t b = row / p.H;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -108,17 +114,15 @@ __global__ void __launch_bounds__(kSelThreads)
       const uint32_t k = key_at(i);
       if ((k & pmask) == prefix) atomicAdd(&hist[(k >> shift) & bmask], 1u);
     }
-    cl.sync();
-    // thread t owns bins 4t .. 4t+3 of the cluster's histogram
-    uint32_t own[4] = {0, 0, 0, 0}, sum = 0;
+    meet();
+    // thread t owns bins 2t, 2t + 1 of the cluster's histogram
+    uint32_t own[2] = {0, 0}, sum = 0;
     for (int c = 0; c < C; ++c) {
-      const uint4 v = *reinterpret_cast<const uint4*>(cl.map_shared_rank(hist, c) + 4 * tid);
+      const uint2 v = *reinterpret_cast<const uint2*>(cl.map_shared_rank(hist, c) + 2 * tid);
       own[0] += v.x;
       own[1] += v.y;
-      own[2] += v.z;
-      own[3] += v.w;
     }
-    sum = own[0] + own[1] + own[2] + own[3];
+    sum = own[0] + own[1];
     // keys in bins above: suffix sums over the threads
     uint32_t inc = sum;
 #pragma unroll
@@ -131,12 +135,11 @@ __global__ void __launch_bounds__(kSelThreads)
     uint32_t above = inc - sum;
     for (int k = warp + 1; k < kSelWarps; ++k) above += red[k];
     if (above < need && need <= above + sum) {  // exactly one thread
-      int d = 3;
-      while (above + own[d] < need) above += own[d--];
-      bc[0] = (uint32_t)(4 * tid + d);
-      bc[1] = need - above;
+      const bool low = above + own[1] < need;
+      bc[0] = (uint32_t)(2 * tid + (low ? 0 : 1));
+      bc[1] = need - above - (low ? own[1] : 0u);
     }
-    cl.sync();  // also: every CTA has read the histograms before they are cleared
+    meet();  // also: every CTA has read the histograms before they are cleared
     prefix |= bc[0] << shift;
     pmask |= bmask << shift;
     need = bc[1];
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(kSelThreads)
     bc[2] = a;
     bc[3] = e;
   }
-  cl.sync();
+  meet();
   uint32_t gt_before = 0, eq_before = 0;
   for (int c = 0; c < rank; ++c) {
     gt_before += cl.map_shared_rank(bc, c)[2];
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(kSelThreads)
     gt_before += __popc(bg);
     eq_before += __popc(be);
   }
-  cl.sync();  // no CTA leaves while another reads its counts
+  meet();  // no CTA leaves while another reads its counts
 }
 
 // ------------------------------------------------------------------ keep --
@@ -214,19 +217,27 @@ struct KeepParams {
 };
 
 constexpr int kKeepWarps = 8;
+constexpr int kKeepSpan = 11;  // source records a CTA stages in shared memory, twice
+constexpr int kKeepSmem = (2 * kKeepSpan + kKeepWarps) * kRecBytes;
 
 // One cluster per (sequence, kv head).  Rounds of (CTAs x warps) destination
-// blocks in ascending order: every warp gathers the 32 positions of its block
-// into registers, the cluster meets at a barrier, then the warps write.  A
-// round reads positions at or above its own first one and writes none above its
-// last, so what a later round reads is still in place and what this round reads
-// is read before the barrier.
+// blocks in ascending order: every warp assembles one block in shared memory, the
+// cluster meets at a barrier, then the blocks are written by bulk copies.  A round
+// reads positions at or above its own first one and writes none above its last, so
+// what a later round reads is still in place and what this round reads is read
+// before the barrier.
+// The sources of a CTA's 256 positions span few blocks when most positions stay:
+// up to kKeepSpan records come in by one bulk copy, each read once, while the round
+// before is assembled; a wider span is gathered from global memory.  (16384 of 17408
+// positions of 128 rows: all gathers from global memory 171 us, staged without the
+// overlap 180.)
 // Gathering one slot: its K codes are 4 triples (one a lane r, copied as they
 // are); its V codes are one byte lane of three words in each of 8 lanes and 4
 // triples, 6 bits of 8 x 3, which move to the byte and the half (a) of the
-// destination slot.  Bound by L1 and memory, a block of 3584 bytes in and out.
+// destination slot.
 __global__ void __launch_bounds__(32 * kKeepWarps, 2)
     keep_kernel(const __grid_constant__ KeepParams p) {
+  extern __shared__ __align__(128) uint32_t assembled[];
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks();
   const int64_t row = blockIdx.x / C;
@@ -258,109 +269,203 @@ __global__ void __launch_bounds__(32 * kKeepWarps, 2)
     if (pb >= p.nbc) pb -= p.nbc;
     return p.blocks + (row * p.nbc + pb) * kRecWords;
   };
-  const int64_t blk0 = (start + off) / kBlk, blk1 = (start + count + off + kBlk - 1) / kBlk;
+  const int blk0 = (int)((start + off) / kBlk);
+  const int blk1 = (int)((start + count + off + kBlk - 1) / kBlk);
   const int per = C * kKeepWarps;
   const int me = (int)cl.block_rank() * kKeepWarps + warp;
-  for (int64_t first = blk0; first < blk1; first += per) {
-    const int64_t lb = first + me;
-    bool write = false;
-    uint32_t kd[12], vd[12];
-    float2 kmd = make_float2(0.0f, 0.0f), vmd = kmd;
-    uint32_t* dst = nullptr;
-    if (lb < blk1) {
-      dst = record(lb);
-      // lane u looks up the source of slot u: itself where the list does not reach
-      const int64_t pos = lb * kBlk + lane - off;
-      int64_t src = pos;
-      if (pos >= start && pos < start + count) {
-        const int64_t s = idx[pos - start];
-        if (s >= pos && s < len) src = s;
-        else atomicCAS(p.err, 0, 1012);  // would overwrite or leave the cache: skipped
+  uint32_t* buf = assembled + warp * kRecWords;
+  __shared__ int span[2][2][kKeepWarps];
+  __shared__ uint64_t bar[2];
+  if (threadIdx.x == 0) {
+    tc::mbar_init(tc::smem_u32(&bar[0]), 1);
+    tc::mbar_init(tc::smem_u32(&bar[1]), 1);
+    tc::fence_barrier_init();
+  }
+  // the list's entry for slot `lane` of block lb, or that position itself
+  auto entry = [&](int lb) -> int {
+    const int64_t pos = (int64_t)lb * kBlk + lane - off;
+    return pos >= start && pos < start + count ? idx[pos - start] : (int)pos;
+  };
+  // Lane u's source for slot u of block lb (itself where the list does not reach),
+  // and the span of the warp's sources.
+  auto look = [&](int lb, int s, int at) -> int {
+    const int pos = lb * kBlk + lane - (int)off;
+    int src = pos;
+    if (lb < blk1 && s != pos) {
+      if (s >= pos && s < len) src = s;
+      else atomicCAS(p.err, 0, 1012);  // would overwrite or leave the cache: skipped
+    }
+    const int sblk = (int)((src + off) / kBlk);
+    const int lo = __reduce_min_sync(0xffffffffu, src != pos ? sblk : INT32_MAX);
+    const int hi = __reduce_max_sync(0xffffffffu, src != pos ? sblk : -1);
+    if (lane == 0) {
+      span[at][0][warp] = lo;
+      span[at][1][warp] = hi;
+    }
+    return src;
+  };
+  // Issues the copy of a round's sources, if they are few enough; its first block,
+  // or -1.  Every thread gets the same answer.
+  auto stage = [&](int at) -> int {
+    const int lo = __reduce_min_sync(0xffffffffu, span[at][0][lane % kKeepWarps]);
+    const int hi = __reduce_max_sync(0xffffffffu, span[at][1][lane % kKeepWarps]);
+    if (hi < 0 || hi - lo >= kKeepSpan) return -1;
+    if (threadIdx.x == 0) {
+      const uint32_t full = tc::smem_u32(&bar[at]);
+      tc::mbar_arrive_expect_tx(full, (hi - lo + 1) * kRecBytes);
+      for (int i = lo; i <= hi; ++i) {
+        const uint32_t* rec = record(i);
+        // a bad page is reported, and none of its slots is taken from here
+        tc::bulk_g2s(tc::smem_u32(assembled + (kKeepWarps + at * kKeepSpan + i - lo) * kRecWords),
+                     rec ? rec : p.blocks, kRecBytes, full);
       }
-      const int64_t ss = src + off;
-      const bool moved = src != pos;
-      write = __any_sync(0xffffffffu, moved) && dst != nullptr;
-      if (write) {
-        const uint32_t* mine = moved ? record(ss / kBlk) : dst;
+    }
+    return lo;
+  };
+  int src = look(blk0 + me, entry(blk0 + me), 0);
+  int ahead = entry(blk0 + per + me);  // entries of the round after
+  __syncthreads();
+  int lo = stage(0), at = 0;
+  uint32_t phases = 0;  // bit `at`: parity of the next wait on bar[at]
+  for (int first = blk0; first < blk1; first += per) {
+    const int lb = first + me;
+    // the next round's sources are read while this one is assembled: they lie above
+    // all that this round writes
+    const int src_next = look(lb + per, ahead, at ^ 1);
+    ahead = entry(lb + 2 * per);
+    // the copy of the round before has read this warp's block
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncthreads();
+    const int lo_next = first + per < blk1 ? stage(at ^ 1) : -1;
+    bool staged = lo >= 0;
+    if (staged) {
+      staged = tc::mbar_wait(tc::smem_u32(&bar[at]), (phases >> at) & 1u, p.err, 70);
+      phases ^= 1u << at;
+    }
+    const int pos = lb * kBlk + lane - (int)off;
+    const bool moved = src != pos;
+    uint32_t* home = lb < blk1 ? record(lb) : nullptr;
+    const bool write = __any_sync(0xffffffffu, moved) && home != nullptr;
+    if (write) {
+        const int sblk = (int)((src + off) / kBlk);
+        const uint32_t* mine = home;
+        if (moved) {
+          mine = record(sblk);
+          if (mine && staged)
+            mine = assembled + (kKeepWarps + at * kKeepSpan + sblk - lo) * kRecWords;
+        }
         const bool bad = mine == nullptr;
-        if (bad) mine = dst;  // reported; the slot keeps what it holds
-        const int slot = bad ? lane : (int)(ss % kBlk);
+        if (bad) mine = home;  // reported; the slot keeps what it holds
+        const int slot = bad ? lane : (int)((src + off) % kBlk);
         const unsigned long long base = (unsigned long long)mine;
-        kmd = reinterpret_cast<const float2*>(mine + kRecKmm)[mm_index(slot)];
-        vmd = reinterpret_cast<const float2*>(mine + kRecVmm)[mm_index(slot)];
+        reinterpret_cast<float2*>(buf + kRecKmm)[mm_index(lane)] =
+            reinterpret_cast<const float2*>(mine + kRecKmm)[mm_index(slot)];
+        reinterpret_cast<float2*>(buf + kRecVmm)[mm_index(lane)] =
+            reinterpret_cast<const float2*>(mine + kRecVmm)[mm_index(slot)];
         // K: lane (g, r) assembles the triples of slots g + 8e
+        uint4* k4 = reinterpret_cast<uint4*>(buf + lane * 12);
+        uint32_t kd[12];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, g + 8 * e);
           const int t = __shfl_sync(0xffffffffu, slot, g + 8 * e);
           const uint32_t* k = rec + (4 * (t & 7) + r) * 12 + 3 * (t >> 3);
 #pragma unroll
-          for (int i = 0; i < 3; ++i) kd[3 * e + i] = k[i];
+          for (int y = 0; y < 3; ++y) kd[3 * e + y] = k[y];
         }
-        // V: lane (g, r) assembles slots r + 4a + 8bb, byte bb of its words
 #pragma unroll
-        for (int i = 0; i < 12; ++i) vd[i] = 0;
+        for (int y = 0; y < 3; ++y)
+          k4[y] = make_uint4(kd[4 * y], kd[4 * y + 1], kd[4 * y + 2], kd[4 * y + 3]);
+        // V: lane (g, r) assembles slots u = r + 4a + 8bb, byte bb of its words, from
+        // lane 4g + t % 4 of the source's record.  Positions that keep their distance
+        // share that lane, so its 48 bytes are loaded when they change.
+        // The work is done on the four triples m at once: z[w][bb] holds word w's byte
+        // of triple m in byte m, and is transposed at the end.
+        uint32_t x[12], z[3][4];
+        unsigned long long have = 0;
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+        for (int q = 0; q < 8; ++q) {
+          const int a = q & 1, bb = q >> 1, u = r + 4 * q;
+          const unsigned long long rb = __shfl_sync(0xffffffffu, base, u);
+          const int t = __shfl_sync(0xffffffffu, slot, u);
+          const unsigned long long from = rb + 4 * (kRecV + (4 * g + (t & 3)) * 12);
+          if (from != have) {
+            have = from;
+            const uint4* v4 = reinterpret_cast<const uint4*>(from);
 #pragma unroll
-          for (int bb = 0; bb < 4; ++bb) {
-            const int u = r + 4 * a + 8 * bb;
-            const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, u);
-            const int t = __shfl_sync(0xffffffffu, slot, u);
-            const uint4* v4 =
-                reinterpret_cast<const uint4*>(rec + kRecV + (4 * g + (t & 3)) * 12);
-            uint32_t x[12];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-              const uint4 q = v4[i];
-              x[4 * i] = q.x;
-              x[4 * i + 1] = q.y;
-              x[4 * i + 2] = q.z;
-              x[4 * i + 3] = q.w;
-            }
-            const int sa = (t >> 2) & 1, sb = 8 * (t >> 3);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              // bytes of the three words; half a of a triple (quads 2j + a) is
-              // bits 0-2 (a = 0) or 3-5 (a = 1) of each byte, plus bits 6-7 of
-              // byte 0 or 1 and bit 6 or 7 of byte 2
-              const uint32_t y0 = x[3 * m] >> sb, y1 = x[3 * m + 1] >> sb, y2 = x[3 * m + 2] >> sb;
-              const int f = 3 * sa;
-              const uint32_t lo2 = ((sa ? y1 : y0) >> 6) & 3u, hi1 = (y2 >> (6 + sa)) & 1u;
-              uint32_t z0 = ((y0 >> f) & 7u) << (3 * a);
-              uint32_t z1 = ((y1 >> f) & 7u) << (3 * a);
-              const uint32_t z2 = (((y2 >> f) & 7u) << (3 * a)) | (hi1 << (6 + a));
-              if (a) z1 |= lo2 << 6;
-              else z0 |= lo2 << 6;
-              vd[3 * m] |= z0 << (8 * bb);
-              vd[3 * m + 1] |= z1 << (8 * bb);
-              vd[3 * m + 2] |= z2 << (8 * bb);
+            for (int y = 0; y < 3; ++y) {
+              const uint4 v = v4[y];
+              x[4 * y] = v.x;
+              x[4 * y + 1] = v.y;
+              x[4 * y + 2] = v.z;
+              x[4 * y + 3] = v.w;
             }
           }
-      }
-    }
-    cl.sync();
-    if (write) {
-      uint4* k4 = reinterpret_cast<uint4*>(dst + lane * 12);
-      uint4* v4 = reinterpret_cast<uint4*>(dst + kRecV + lane * 12);
+          // byte t / 8 of word w of each triple; half a of a triple (quads 2j + a) is bits
+          // 0-2 (a = 0) or 3-5 (a = 1) of each byte, plus bits 6-7 of byte 0 or 1 and bit 6
+          // or 7 of byte 2
+          const int sa = (t >> 2) & 1;
+          const uint32_t sel = (uint32_t)(t >> 3) * 0x11u + 0x40u;
+          uint32_t y[3];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        k4[i] = make_uint4(kd[4 * i], kd[4 * i + 1], kd[4 * i + 2], kd[4 * i + 3]);
-        v4[i] = make_uint4(vd[4 * i], vd[4 * i + 1], vd[4 * i + 2], vd[4 * i + 3]);
-      }
-      reinterpret_cast<float2*>(dst + kRecKmm)[mm_index(lane)] = kmd;
-      reinterpret_cast<float2*>(dst + kRecVmm)[mm_index(lane)] = vmd;
+          for (int w = 0; w < 3; ++w)
+            y[w] = __byte_perm(__byte_perm(x[w], x[3 + w], sel), __byte_perm(x[6 + w], x[9 + w], sel),
+                               0x5410);
+          const uint32_t lo2 = ((sa ? y[1] : y[0]) >> 6) & 0x03030303u;
+          const uint32_t hi1 = (y[2] >> (6 + sa)) & 0x01010101u;
+          const uint32_t c0 = (y[0] >> (3 * sa)) & 0x07070707u;
+          const uint32_t c1 = (y[1] >> (3 * sa)) & 0x07070707u;
+          const uint32_t c2 = (y[2] >> (3 * sa)) & 0x07070707u;
+          if (a == 0) {
+            z[0][bb] = c0 | lo2 << 6;
+            z[1][bb] = c1;
+            z[2][bb] = c2 | hi1 << 6;
+          } else {
+            z[0][bb] |= c0 << 3;
+            z[1][bb] |= c1 << 3 | lo2 << 6;
+            z[2][bb] |= c2 << 3 | hi1 << 7;
+          }
+        }
+        uint32_t vd[12];
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {  // 4 x 4 bytes: (bb, m) to (m, bb)
+          const uint32_t p01l = __byte_perm(z[w][0], z[w][1], 0x5140);
+          const uint32_t p01h = __byte_perm(z[w][0], z[w][1], 0x7362);
+          const uint32_t p23l = __byte_perm(z[w][2], z[w][3], 0x5140);
+          const uint32_t p23h = __byte_perm(z[w][2], z[w][3], 0x7362);
+          vd[w] = __byte_perm(p01l, p23l, 0x5410);
+          vd[3 + w] = __byte_perm(p01l, p23l, 0x7632);
+          vd[6 + w] = __byte_perm(p01h, p23h, 0x5410);
+          vd[9 + w] = __byte_perm(p01h, p23h, 0x7632);
+        }
+        uint4* v4 = reinterpret_cast<uint4*>(buf + kRecV + lane * 12);
+#pragma unroll
+        for (int y = 0; y < 3; ++y)
+          v4[y] = make_uint4(vd[4 * y], vd[4 * y + 1], vd[4 * y + 2], vd[4 * y + 3]);
     }
+    tc::fence_async_smem();
+    if (C > 1) cl.sync();
+    else __syncthreads();
+    if (write && lane == 0) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(home),
+                   "r"(tc::smem_u32(buf)), "r"(kRecBytes)
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    src = src_next;
+    lo = lo_next;
+    at ^= 1;
   }
+  // the last copies are done before the CTA's shared memory goes
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// CTAs of a cluster (a power of two, at most 8) for `rows` rows of `units`
-// units of work, each CTA taking `per` units at a time: as many as keep every
-// SM busy, and none without work.
-int cluster_size(int num_sms, int64_t rows, int64_t units, int64_t per) {
-  int c = 1;
-  while (c < 8 && rows * c < 2 * num_sms && units > c * per) c *= 2;
-  return c;
+// CTAs of a cluster (at most 8) for `rows` rows of `units` units of work, each CTA
+// taking `per` units at a time: as many as are resident at once, none without work.
+int cluster_size(int resident, int64_t rows, int64_t units, int64_t per) {
+  int64_t c = resident / rows;
+  if (c > ceil_div(units, per)) c = ceil_div(units, per);
+  return c < 1 ? 1 : (c > 8 ? 8 : (int)c);
 }
 
 template <class Kernel, class... Args>
@@ -386,8 +491,14 @@ int launch_cluster(Kernel kernel, int64_t rows, int cluster, int threads, size_t
 
 int launch_keep(ft_ctx* ctx, const KeepParams& p, int64_t rows, cudaStream_t s) {
   const int64_t blocks = ceil_div(p.count, kBlk) + 1;
-  const int c = cluster_size(ctx->num_sms, rows, blocks, kKeepWarps);
-  return launch_cluster(keep_kernel, rows, c, 32 * kKeepWarps, 0, s, p);
+  const int c = cluster_size(2 * ctx->num_sms, rows, blocks, kKeepWarps);
+  static bool opted[64] = {false};  // once per device
+  if (ctx->device >= 64 || !opted[ctx->device]) {
+    FT_CUDA(cudaFuncSetAttribute(keep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kKeepSmem));
+    if (ctx->device < 64) opted[ctx->device] = true;
+  }
+  return launch_cluster(keep_kernel, rows, c, 32 * kKeepWarps, kKeepSmem, s, p);
 }
 
 }  // namespace
@@ -438,7 +549,9 @@ int ft_kv_select_heavy(ft_ctx* ctx, int64_t batch, int64_t kv_heads, const float
   p.out_len = weights_out_stride;
   p.err = ctx->err_word;
   const int64_t rows = batch * kv_heads;
-  const int c = cluster_size(ctx->num_sms, rows, max_seq_len, 8 * kSelThreads);
+  // one CTA a row up to 32 keys a thread: the cluster's barriers cost more than they
+  // save (16384 keys a row, 128 rows: 50 us on clusters of four)
+  const int c = cluster_size(ctx->num_sms, rows, max_seq_len, 32 * kSelThreads);
   // keys that do not fit shared memory are read from global memory again
   const int64_t share = ceil_div(max_seq_len, c);
   const int cap = (int)(share < kSelKeys ? share : kSelKeys);
