@@ -1079,12 +1079,13 @@ __global__ void __launch_bounds__((kDecWarps + 1) * 32, FT_KV_MIN_BLOCKS)
   }
 }
 
-// Merges the split partials of one (sequence, q head): thread = dim.
-// Mode T (signs != null): the rotated-domain output is rotated back.
+// Merges the split partials of one (sequence, q head): thread % 128 = dim (the
+// second half of a block of 256 repeats the first's work and writes the same
+// values).  Mode T (signs != null): the rotated-domain output is rotated back.
 __device__ __forceinline__ void combine_head(const float* __restrict__ part, int nsplit,
                                              float* __restrict__ out,
                                              const float* __restrict__ signs, int64_t bh) {
-  const int d = threadIdx.x;
+  const int d = threadIdx.x % kD;
   const float* pp = part + bh * nsplit * kPart;
   float M = -INFINITY;
   for (int s = 0; s < nsplit; ++s) M = fmaxf(M, pp[s * kPart]);
@@ -1114,10 +1115,14 @@ __global__ void kv3_combine_kernel(const float* __restrict__ part, int nsplit,
 // Attention weight of every position, added to weights [B][Hkv][wstride]:
 // w[b, hk, s] += sum over the q heads of group hk of exp2(score - M) / l, with
 // (M, l) the softmax statistics that the split partials give.  Blocks x <
-// chunks take kWeightChunk positions each; the G blocks behind them merge the
-// outputs, so that a decode with weights is two launches like one without.
+// chunks take kWeightChunk slots each, four adjacent ones a thread (their loads
+// are independent: with one position a thread and eight rounds the latency of the
+// scores made 8190 positions of 32 rows 14 us); the G blocks behind them merge
+// the outputs, so that a decode with weights is two launches like one without.
+// Bound by the scores' bytes, 4 G a position, and 8 of the weight.
 constexpr int kWeightChunk = 1024;
-__global__ void __launch_bounds__(kD)
+constexpr int kWeightThreads = kWeightChunk / 4;
+__global__ void __launch_bounds__(kWeightThreads)
     kv3_weights_kernel(const __grid_constant__ DecodeParams p, int nsplit, int chunks,
                        float* __restrict__ weights, int64_t wstride, float* __restrict__ out,
                        const float* __restrict__ signs) {
@@ -1133,11 +1138,12 @@ __global__ void __launch_bounds__(kD)
     len = p.seq_lens[b];  // the decode kernel reports a bad length
     len = len < 0 ? 0 : (len > p.len ? p.len : len);
   }
-  const int64_t first = (int64_t)x * kWeightChunk;
-  if (first >= len) return;
+  // slots of the sequence's blocks: position + head_off
+  const int64_t slot = (int64_t)x * kWeightChunk + 4 * threadIdx.x;
+  if ((int64_t)x * kWeightChunk >= len + p.head_off) return;
   extern __shared__ float stat[];  // [G] M, then [G] 1 / l
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int h = warp; h < p.G; h += kD / 32) {
+  for (int h = warp; h < p.G; h += kWeightThreads / 32) {
     const float* pp = p.part + (h0 + h) * nsplit * kPart;
     float M = -INFINITY;
     for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, pp[s * kPart]);
@@ -1155,16 +1161,33 @@ __global__ void __launch_bounds__(kD)
       stat[p.G + h] = 1.0f / l;
     }
   }
-  __syncthreads();
-  float* w = weights + (b * p.Hkv + kvh) * wstride;
-  const float* sc = p.scores + h0 * p.score_stride + p.head_off;
-  const int64_t end = first + kWeightChunk < len ? first + kWeightChunk : len;
-  for (int64_t i = first + threadIdx.x; i < end; i += kD) {
-    float a = 0.0f;
-    for (int h = 0; h < p.G; ++h)
-      a = fmaf(exp2f(sc[h * p.score_stride + i] - stat[h]), stat[p.G + h], a);
-    w[i] += a;
+  const int64_t pos = slot - p.head_off;
+  float* w = weights + (b * p.Hkv + kvh) * wstride + pos;
+  float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, old[4];
+  bool in[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    in[k] = pos + k >= 0 && pos + k < len;
+    old[k] = in[k] ? w[k] : 0.0f;
   }
+  __syncthreads();
+  if (slot >= len + p.head_off) return;
+  // rows of score_stride (a multiple of 32) floats: 16-byte aligned; the slots past
+  // the last position hold scores of their block that are not used
+  const float4* sc = reinterpret_cast<const float4*>(p.scores + h0 * p.score_stride + slot);
+  const int64_t step = p.score_stride / 4;
+#pragma unroll 4
+  for (int h = 0; h < p.G; ++h) {
+    const float4 v = sc[h * step];
+    const float M = stat[h], il = stat[p.G + h];
+    add[0] = fmaf(exp2f(v.x - M), il, add[0]);
+    add[1] = fmaf(exp2f(v.y - M), il, add[1]);
+    add[2] = fmaf(exp2f(v.z - M), il, add[2]);
+    add[3] = fmaf(exp2f(v.w - M), il, add[3]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (in[k]) w[k] = old[k] + add[k];
 }
 
 // Opts the decode kernel into its dynamic shared memory (once per device) and
@@ -1525,11 +1548,11 @@ int launch_decode(ft_ctx* ctx, Cache* c, DecodeParams p, int64_t batch, int64_t 
     p.scores = static_cast<float*>(c->scores.ptr);
     kv3_decode_kernel<true><<<grid, (kDecWarps + 1) * 32, kDecSmem, s>>>(p);
     FT_LAUNCH_CHECK();
-    const int64_t chunks = ceil_div(p.len, kWeightChunk);
+    const int64_t chunks = ceil_div(p.head_off + p.len, kWeightChunk);
     FT_CHECK(chunks + p.G < INT32_MAX && kv_heads <= 65535, FT_ERR_UNSUPPORTED,
              "decode grid too large");
     dim3 wgrid((unsigned)(chunks + p.G), (unsigned)kv_heads, (unsigned)batch);
-    kv3_weights_kernel<<<wgrid, kD, (unsigned)(2 * p.G * sizeof(float)), s>>>(
+    kv3_weights_kernel<<<wgrid, kWeightThreads, (unsigned)(2 * p.G * sizeof(float)), s>>>(
         p, (int)nsplit, (int)chunks, weights_dev, weights_stride, out_dev, signs);
     FT_LAUNCH_CHECK();
     return FT_OK;

@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(kSelThreads)
 
   uint32_t prefix = 0, pmask = 0;
   uint32_t need = (uint32_t)heavy;  // still to be found among keys with this prefix
+#pragma unroll 1  // small code: a launch fetches every instruction anew
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const uint32_t bmask = pass == 2 ? 1023u : 2047u;

@@ -124,9 +124,11 @@ def _tree_args(q: torch.Tensor, mask, batch: int, device, out):
         q = q.clone()
     if mask is not None:
         if mask.device != device or mask.dtype != torch.int64 or \
-                tuple(mask.shape) not in ((T,), (batch, T)):
+                mask.shape not in ((T,), (batch, T)):
             raise ShapeError(f"mask must be int64 [{T}] or [{batch}, {T}] on {device}")
-        mask = mask.expand(batch, T).contiguous()
+        if mask.dim() == 1:
+            mask = mask.expand(batch, T)
+        mask = mask.contiguous()
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or \
