@@ -44,9 +44,9 @@ constexpr int kTStageBytes = kTWarps * kRecBytes;
 constexpr int kTPart = 2 + kD;      // partial record: M, l, numerator[128]
 constexpr int kTQfBytes = 8 * 32 * 16;  // q fragments of one term [k-step][lane][16 B]
 constexpr int kTOffQf = kTStages * kTStageBytes;
-constexpr int tree_off_info(int terms) { return kTOffQf + terms * kTQfBytes; }
-constexpr int tree_off_bars(int terms) { return tree_off_info(terms) + kRows * 16; }
-constexpr int tree_smem(int terms) { return tree_off_bars(terms) + 16 * kTStages; }
+constexpr int kTOffInfo = kTOffQf + 2 * kTQfBytes;  // hi and lo
+constexpr int kTOffBars = kTOffInfo + kRows * 16;
+constexpr int kTreeSmem = kTOffBars + 16 * kTStages;
 constexpr int kTMergeBytes = kTWarps * kRows * (kD + 2) * 4;
 static_assert(kTMergeBytes <= kTStages * kTStageBytes, "the warps merge in the stage buffers");
 
@@ -72,7 +72,7 @@ struct TreeParams {
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -113,6 +113,12 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {  // a in the 
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+__device__ __forceinline__ float ex2(float x) {  // 2 ulp, 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Draft tokens of row R (0 <= R < rows): the mask bits of its draft.
@@ -183,14 +189,13 @@ __device__ __forceinline__ int bound_exp(float v) {
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <int kTerms>
-__global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
+__global__ void __launch_bounds__((kTWarps + 1) * 32, 2)
     tree_decode_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const uint4* qf = reinterpret_cast<const uint4*>(smem + kTOffQf);
-  float* qinfo = reinterpret_cast<float*>(smem + tree_off_info(kTerms));  // sum(q), then scale
-  uint64_t* qmask = reinterpret_cast<uint64_t*>(smem + tree_off_info(kTerms) + kRows * 8);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + tree_off_bars(kTerms));
+  float* qinfo = reinterpret_cast<float*>(smem + kTOffInfo);  // sum(q), then scale
+  uint64_t* qmask = reinterpret_cast<uint64_t*>(smem + kTOffInfo + kRows * 8);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kTOffBars);
   const uint32_t full0 = tc::smem_u32(bars), empty0 = full0 + 8 * kTStages;
 
   const int split = blockIdx.x;
@@ -247,14 +252,12 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
       qw[at + 2] = h1;
       const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
       float sum = (f0.x + f0.y) + (f1.x + f1.y);  // of the q that the products take
-      if (kTerms == 2) {
-        const uint32_t l0 = pack_half2(v[0] - f0.x, v[2] - f0.y);
-        const uint32_t l1 = pack_half2(v[1] - f1.x, v[3] - f1.y);
-        qw[kTQfBytes / 4 + at] = l0;
-        qw[kTQfBytes / 4 + at + 2] = l1;
-        const float2 d0 = unpack_half2(l0), d1 = unpack_half2(l1);
-        sum += (d0.x + d0.y) + (d1.x + d1.y);
-      }
+      const uint32_t l0 = pack_half2(v[0] - f0.x, v[2] - f0.y);
+      const uint32_t l1 = pack_half2(v[1] - f1.x, v[3] - f1.y);
+      qw[kTQfBytes / 4 + at] = l0;
+      qw[kTQfBytes / 4 + at + 2] = l1;
+      const float2 d0 = unpack_half2(l0), d1 = unpack_half2(l1);
+      sum += (d0.x + d0.y) + (d1.x + d1.y);
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       if (lane == 0) {
@@ -353,18 +356,19 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 #pragma unroll
           for (int c = 0; c < 4; ++c) sc[a][bb][c] = 0.0f;
       }
+      // (products of one sum are kept four apart: each waits for the one before)
 #define FT_TREE_KSTEP(Q)                                                                  \
   {                                                                                       \
-    const uint4 ah = qf[(Q) * 32 + lane];                                                 \
-    uint4 al;                                                                             \
-    if (kTerms == 2) al = qf[(8 + (Q)) * 32 + lane];                                      \
+    const uint4 ah = qf[(Q) * 32 + lane], al = qf[(8 + (Q)) * 32 + lane];                 \
+    uint32_t b0[2][2], b1[2][2];                                                          \
     _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) { \
       const uint32_t w0 = kw[a][3 * bb], w1 = kw[a][3 * bb + 1], w2 = kw[a][3 * bb + 2];  \
-      const uint32_t b0 = kTerms == 2 ? quad_centred<Q, 0>(w0, w1, w2) : quad_half2<Q, 0>(w0, w1, w2); \
-      const uint32_t b1 = kTerms == 2 ? quad_centred<Q, 1>(w0, w1, w2) : quad_half2<Q, 1>(w0, w1, w2); \
-      mma_f16(sc[a][bb], ah, b0, b1);                                                     \
-      if (kTerms == 2) mma_f16(sc[a][bb], al, b0, b1);                                    \
+      b0[a][bb] = quad_centred<Q, 0>(w0, w1, w2);                                         \
+      b1[a][bb] = quad_centred<Q, 1>(w0, w1, w2);                                         \
+      mma_f16(sc[a][bb], ah, b0[a][bb], b1[a][bb]);                                       \
     }                                                                                     \
+    _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) \
+      mma_f16(sc[a][bb], al, b0[a][bb], b1[a][bb]);                                       \
   }
       FT_TREE_KSTEP(0) FT_TREE_KSTEP(1) FT_TREE_KSTEP(2) FT_TREE_KSTEP(3)
       FT_TREE_KSTEP(4) FT_TREE_KSTEP(5) FT_TREE_KSTEP(6) FT_TREE_KSTEP(7)
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
             const float ks = (kmax - kmin) * 0.14285714285714285f;
             vs[a][bb][i] = (vmax - vmin) * 0.14285714285714285f;
             vn[a][bb][i] = fmaf(3.5f, vs[a][bb][i], vmin);
-            const float kc = fmaf(kTerms == 2 ? 3.5f : -8.0f, ks, kmin);
+            const float kc = fmaf(3.5f, ks, kmin);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               sc[a][bb][2 * h + i] =
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float x = sc[a][bb][2 * h + i];
-              const float pr = exp2f(x - M);
+              const float pr = ex2(x - M);
               l_part[h] += pr;
               w[i] = pr * vs[a][bb][i];
               float vmv = pr * vn[a][bb][i];
@@ -488,11 +492,9 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
             // register of the fragment: row half h, k half bb
             uint32_t& dst = bb ? (h ? ph[a].w : ph[a].z) : (h ? ph[a].y : ph[a].x);
             dst = hi;
-            if (kTerms == 2) {
-              const float2 f = unpack_half2(hi);
-              uint32_t& dl = bb ? (h ? pl[a].w : pl[a].z) : (h ? pl[a].y : pl[a].x);
-              dl = pack_half2(w[0] - f.x, w[1] - f.y);
-            }
+            const float2 f = unpack_half2(hi);
+            uint32_t& dl = bb ? (h ? pl[a].w : pl[a].z) : (h ? pl[a].y : pl[a].x);
+            dl = pack_half2(w[0] - f.x, w[1] - f.y);
           }
       }
       // ---- P.V: column n = g of n-tile 4m + jj is dim 8 (4m + jj) + g
@@ -509,23 +511,27 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, kTerms == 1 ? 3 : 2)
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         const uint32_t w0 = vw[3 * m], w1 = vw[3 * m + 1], w2 = vw[3 * m + 2];
-#define FT_TREE_VSTEP(JJ)                                                               \
-  {                                                                                     \
-    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};                                              \
-    const uint32_t b0 = quad_centred<2 * (JJ), 0>(w0, w1, w2);                            \
-    const uint32_t b1 = quad_centred<2 * (JJ), 1>(w0, w1, w2);                            \
-    const uint32_t b2 = quad_centred<2 * (JJ) + 1, 0>(w0, w1, w2);                        \
-    const uint32_t b3 = quad_centred<2 * (JJ) + 1, 1>(w0, w1, w2);                        \
-    mma_f16(t, ph[0], b0, b1);                                                          \
-    mma_f16(t, ph[1], b2, b3);                                                          \
-    if (kTerms == 2) {                                                                  \
-      mma_f16(t, pl[0], b0, b1);                                                        \
-      mma_f16(t, pl[1], b2, b3);                                                        \
-    }                                                                                   \
-    _Pragma("unroll") for (int c = 0; c < 4; ++c) o[4 * m + (JJ)][c] += t[c];           \
-  }
+        uint32_t bv[4][4];
+        float t[4][4];
+#define FT_TREE_VSTEP(JJ)                                      \
+  bv[JJ][0] = quad_centred<2 * (JJ), 0>(w0, w1, w2);           \
+  bv[JJ][1] = quad_centred<2 * (JJ), 1>(w0, w1, w2);           \
+  bv[JJ][2] = quad_centred<2 * (JJ) + 1, 0>(w0, w1, w2);       \
+  bv[JJ][3] = quad_centred<2 * (JJ) + 1, 1>(w0, w1, w2);       \
+  t[JJ][0] = t[JJ][1] = t[JJ][2] = t[JJ][3] = 0.0f;            \
+  mma_f16(t[JJ], ph[0], bv[JJ][0], bv[JJ][1]);
         FT_TREE_VSTEP(0) FT_TREE_VSTEP(1) FT_TREE_VSTEP(2) FT_TREE_VSTEP(3)
 #undef FT_TREE_VSTEP
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], pl[0], bv[jj][0], bv[jj][1]);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], ph[1], bv[jj][2], bv[jj][3]);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], pl[1], bv[jj][2], bv[jj][3]);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[4 * m + jj][c] += t[jj][c];
       }
     }
     __syncwarp();
@@ -653,11 +659,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t v;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
   return v;
-}
-__device__ __forceinline__ float ex2(float x) {  // 2 ulp, 0 below 2^-126
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // Registers of a warpgroup from here on.  The seven groups' shares add up to the
 // 896 x 72 that the block is launched with: 4 x 88, 2 x 56, 40 (x 128 threads).
@@ -1343,25 +1344,31 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
 int tree_occupancy(int device) {
   static int cached[64] = {0};
   if (device >= 0 && device < 64 && cached[device]) return cached[device];
-  cudaFuncSetAttribute(tree_decode_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       tree_smem(2));
+  cudaFuncSetAttribute(tree_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       kTreeSmem);
   cudaFuncSetAttribute(tree_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
   int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel<2>,
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel,
                                                     (kTWarps + 1) * 32,
-                                                    tree_smem(2)) != cudaSuccess ||
+                                                    kTreeSmem) != cudaSuccess ||
       occ < 1)
     occ = 1;
   if (device >= 0 && device < 64) cached[device] = occ;
   return occ;
 }
 
-// Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost in tiles).
-int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t overhead) {
+// Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost in
+// tiles).  Paged sequences differ in length, which only the device knows: there the
+// splits are made small enough for three waves, down to four tiles, so that CTAs of
+// short sequences make room (6 sequences of 2006 to 8191 positions, 24 drafts: 104 us
+// with splits for equal lengths).
+int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t overhead,
+                    bool ragged) {
   int64_t best_cost = INT64_MAX, best = ntiles;
   for (int64_t sp = 1; sp <= 256 && sp <= ntiles; ++sp) {
-    const int64_t per = ceil_div(ntiles, sp);
-    const int64_t waves = ceil_div(units * ceil_div(ntiles, per), resident);
+    const int64_t per = ceil_div(ntiles, sp), ctas = units * ceil_div(ntiles, per);
+    if (ragged && per > 4 && ctas < 3 * resident && sp < 256 && sp < ntiles) continue;
+    const int64_t waves = ceil_div(ctas, resident);
     const int64_t cost = waves * (per + overhead);
     if (cost < best_cost) {
       best_cost = cost;
@@ -1408,8 +1415,10 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
   FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
            "decode grid too large");
   p.tiles_per = q_is_bf16
-                    ? split_tiles(batch * p.Hkv * p.rgroups, ntiles, ctx->num_sms, kPreOverhead)
-                    : split_tiles(batch * p.Hkv * p.rgroups, ntiles, (int64_t)occ * ctx->num_sms, 2);
+                    ? split_tiles(batch * p.Hkv * p.rgroups, ntiles, ctx->num_sms, kPreOverhead,
+                                  p.table != nullptr)
+                    : split_tiles(batch * p.Hkv * p.rgroups, ntiles, (int64_t)occ * ctx->num_sms, 2,
+                                  p.table != nullptr);
   p.nparts = (int)ceil_div(ntiles, p.tiles_per);
   const int64_t tiles = batch * p.Hkv * p.rgroups;
   const size_t images = q_is_bf16 ? (size_t)tiles * kQImage : 0;
@@ -1436,7 +1445,7 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
     cfg.numAttrs = 1;
     FT_CUDA(cudaLaunchKernelEx(&cfg, tree_tile_kernel, p));
   } else {
-    tree_decode_kernel<2><<<grid, (kTWarps + 1) * 32, tree_smem(2), s>>>(p);
+    tree_decode_kernel<<<grid, (kTWarps + 1) * 32, kTreeSmem, s>>>(p);
   }
   FT_LAUNCH_CHECK();
   tree_combine_kernel<<<(unsigned)total, 32 * kCombineWarps, 0, s>>>(p, out_dev);

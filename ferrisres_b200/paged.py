@@ -355,6 +355,21 @@ class PagedKv3Cache:
             a[i, :len(t)] = t
         return torch.from_numpy(a).to(self.device), stride
 
+    def _upload(self, layer: int, rids, *rows):
+        """The block tables and further int32 rows [len(rids)] in one copy to the device:
+        (tables, table stride, *rows)."""
+        tabs = [self._state(r).layer_table(layer).table() for r in rids]
+        stride = max(1, max(len(t) for t in tabs))
+        n = len(rids)
+        a = np.zeros(len(rows) * n + n * stride, np.int32)
+        for i, row in enumerate(rows):
+            a[i * n:(i + 1) * n] = row
+        b = a[len(rows) * n:].reshape(n, stride)
+        for i, t in enumerate(tabs):
+            b[i, :len(t)] = t
+        d = torch.from_numpy(a).to(self.device)
+        return (d[len(rows) * n:], stride, *(d[i * n:(i + 1) * n] for i in range(len(rows))))
+
     def _kv_view(self, t: torch.Tensor, n_req: int) -> torch.Tensor:
         if t.device != self.device or t.dtype not in (torch.float32, torch.bfloat16):
             raise ShapeError("k, v must be fp32 or bf16 tensors on the cache's device")
@@ -420,8 +435,7 @@ class PagedKv3Cache:
         copies = []
         starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
         self._copy_pages(copies, stream)
-        tables, stride = self._tables(layer, rids)
-        start_dev = torch.from_numpy(starts).to(self.device)
+        tables, stride, start_dev = self._upload(layer, rids, starts)
         call("ft_kvp_append_packed", self.ctx.handle, self.handle, len(rids), n_pos,
              _dptr(tables), stride, _dptr(start_dev), *[_dptr(t) for t in tens],
              _call_stream(self.device, stream, tables, start_dev, *tens))
@@ -452,13 +466,12 @@ class PagedKv3Cache:
         q, mask, out = _tree_args(q, mask, len(rids), self.device, out)
         if not rids:
             return out
-        lens = np.array([self.seq_len(r, layer) for r in rids], np.int32)
-        if lens.min() < q.shape[1]:
-            raise ShapeError(f"{q.shape[1]} drafts in a request of {lens.min()} positions")
-        tables, stride = self._tables(layer, rids)
-        lens_dev = torch.from_numpy(lens).to(self.device)
+        lens = [self.seq_len(r, layer) for r in rids]
+        if min(lens) < q.shape[1]:
+            raise ShapeError(f"{q.shape[1]} drafts in a request of {min(lens)} positions")
+        tables, stride, lens_dev = self._upload(layer, rids, lens)
         call("ft_kvp_tree_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
-             _dptr(lens_dev), int(lens.max()), int(q.shape[1]), _dptr(q),
+             _dptr(lens_dev), max(lens), int(q.shape[1]), _dptr(q),
              int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
              float(scale), _dptr(out),
              _call_stream(self.device, stream, tables, lens_dev, q, out, mask))
@@ -506,11 +519,10 @@ class PagedKv3Cache:
             alloc.free(old)
         self._copy_pages(copies, stream)
         if max(counts) > 0:
-            tables, stride = self._tables(layer, rids)
-            meta = torch.from_numpy(np.array([lens, starts, counts], np.int32)).to(self.device)
+            tables, stride, *meta = self._upload(layer, rids, lens, starts, counts)
             call("ft_kvp_keep", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
-                 _dptr(meta[0]), _dptr(meta[1]), _dptr(meta[2]), max(counts), _dptr(idx), ib, ih,
-                 _call_stream(self.device, stream, tables, meta, idx))
+                 *[_dptr(m) for m in meta], max(counts), _dptr(idx), ib, ih,
+                 _call_stream(self.device, stream, tables, idx))
         for r, t, c, st, length in zip(rids, tabs, counts, starts, lens):
             need = -(-(st + c) // PAGE_POSITIONS)
             while len(t) > need:
