@@ -21,12 +21,11 @@
 // two parts of v do not cancel; the scores of a bf16 q do without it.  (As
 // fp16 subnormals the codes would cost one operation less, but the tensor core
 // aligns a product by the operands' exponents and drops the low bits: 2^-12 of
-// the result were lost.)  Softmax statistics, the sum terms and numerators are
-// fp32; the tensor core truncates its fp32 sums, so it sums 32 positions at
-// most, and the blocks' sums are added with rounding to nearest.
-// The running reference of a row is M = max(x) - ew, 2^ew being the power of
-// two that keeps w = exp2(x - M) st below 2^15: l, the sum terms and the
-// numerator all carry that factor, so it needs no undoing.
+// the result were lost.)  Softmax statistics, the sum terms and the merge of the
+// splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
+// With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 24
+// drafts of 6 sequences took 104 us where tree_tile_kernel takes 47, and 64 drafts
+// over 8 x 32768 positions 1868 us where it takes 541.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,24 +36,15 @@ namespace ft {
 namespace {
 
 constexpr int kMaxDraft = 64;       // bits of a mask word
-constexpr int kRows = 16;           // query rows per CTA (one MMA tile)
-constexpr int kTWarps = 4;          // compute warps = 32-slot blocks per tile
-constexpr int kTStages = 4;
+constexpr int kTWarps = 4;          // 32-slot blocks per tile
 constexpr int kTStageBytes = kTWarps * kRecBytes;
 constexpr int kTPart = 2 + kD;      // partial record: M, l, numerator[128]
-constexpr int kTQfBytes = 8 * 32 * 16;  // q fragments of one term [k-step][lane][16 B]
-constexpr int kTOffQf = kTStages * kTStageBytes;
-constexpr int kTOffInfo = kTOffQf + 2 * kTQfBytes;  // hi and lo
-constexpr int kTOffBars = kTOffInfo + kRows * 16;
-constexpr int kTreeSmem = kTOffBars + 16 * kTStages;
-constexpr int kTMergeBytes = kTWarps * kRows * (kD + 2) * 4;
-static_assert(kTMergeBytes <= kTStages * kTStageBytes, "the warps merge in the stage buffers");
 
 struct TreeParams {
   const void* q;  // [B][T][Hq][128], fp32 or bf16
   int q_bf16;
   int64_t Hq, Hkv;
-  int G, T, rows, rgroups;  // rows = T * G per kv head, in groups of kRows
+  int G, T, rows, rgroups;  // rows = T * G per kv head, in tiles of 128
   const uint64_t* mask;     // [B][T], or null: draft i sees drafts 0..i
   int64_t nbc, head_off, head_blk, len;
   int64_t nlb;        // logical 32-slot blocks covering the longest sequence
@@ -68,16 +58,8 @@ struct TreeParams {
   const int32_t* seq_lens;
   int64_t tstride, n_pages;
   int nparts;  // splits
-  uint8_t* qimg;  // bf16 queries: prepared row tiles [B][Hkv][rgroups]
+  uint8_t* qimg;  // prepared row tiles [B][Hkv][rgroups]
 };
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
 
 // Codes of bytes (0, 2) (h = 0) or (1, 3) (h = 1) of quad Q of a triple, as two
 // fp16 values 1 + c/8: the field moves to mantissa bits 7..9.
@@ -189,408 +171,7 @@ __device__ __forceinline__ int bound_exp(float v) {
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-__global__ void __launch_bounds__((kTWarps + 1) * 32, 2)
-    tree_decode_kernel(const __grid_constant__ TreeParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint4* qf = reinterpret_cast<const uint4*>(smem + kTOffQf);
-  float* qinfo = reinterpret_cast<float*>(smem + kTOffInfo);  // sum(q), then scale
-  uint64_t* qmask = reinterpret_cast<uint64_t*>(smem + kTOffInfo + kRows * 8);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kTOffBars);
-  const uint32_t full0 = tc::smem_u32(bars), empty0 = full0 + 8 * kTStages;
-
-  const int split = blockIdx.x;
-  const int64_t kvh = blockIdx.y / p.rgroups;
-  const int R0 = (int)(blockIdx.y % p.rgroups) * kRows;
-  const int64_t b = blockIdx.z;
-  const int64_t row = b * p.Hkv + kvh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, r = lane & 3;
-  int64_t len_b = p.len, nlb_b = p.nlb;
-  if (p.table) {
-    len_b = p.seq_lens[b];
-    if (len_b < 0 || len_b > p.len) {
-      if (tid == 0) atomicCAS(p.err, 0, 1007);
-      len_b = len_b < 0 ? 0 : p.len;
-    }
-    nlb_b = (len_b + kBlk - 1) / kBlk;
-  }
-  const int64_t ntiles_all = (nlb_b + kTWarps - 1) / kTWarps;
-  const int64_t t_begin = (int64_t)split * p.tiles_per;
-  int64_t t_end = t_begin + p.tiles_per;
-  if (t_end > ntiles_all) t_end = ntiles_all;
-  const int ntiles = t_end > t_begin ? (int)(t_end - t_begin) : 0;
-
-  if (tid == 0) {
-    for (int s = 0; s < kTStages; ++s) {
-      tc::mbar_init(full0 + 8 * s, 1);
-      tc::mbar_init(empty0 + 8 * s, kTWarps);
-    }
-    tc::fence_barrier_init();
-  }
-  // q fragments: k-step Q covers dims 16Q .. 16Q+15, its k index 2r, 2r+1 being
-  // dims 4r, 4r+2 and 2r+8, 2r+9 dims 4r+1, 4r+3 (bytes 0, 2 and 1, 3 of a quad)
-  if (warp < kTWarps) {
-    uint32_t* qw = reinterpret_cast<uint32_t*>(smem + kTOffQf);
-    uint4 raw[kRows / kTWarps];  // every load first
-#pragma unroll
-    for (int k = 0; k < kRows / kTWarps; ++k) {
-      const int i = warp + k * kTWarps;
-      raw[k] = R0 + i < p.rows ? load_q_raw(p, b, kvh, R0 + i, lane) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < kRows / kTWarps; ++k) {
-      const int i = warp + k * kTWarps;
-      float v[4];
-      int sh;
-      q_row(p, raw[k], lane, v, &sh);
-      const float mul = pow2i(sh);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] *= mul;
-      const int at = ((lane >> 2) * 32 + (i & 7) * 4 + (lane & 3)) * 4 + (i >> 3);
-      const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
-      qw[at] = h0;
-      qw[at + 2] = h1;
-      const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-      float sum = (f0.x + f0.y) + (f1.x + f1.y);  // of the q that the products take
-      const uint32_t l0 = pack_half2(v[0] - f0.x, v[2] - f0.y);
-      const uint32_t l1 = pack_half2(v[1] - f1.x, v[3] - f1.y);
-      qw[kTQfBytes / 4 + at] = l0;
-      qw[kTQfBytes / 4 + at + 2] = l1;
-      const float2 d0 = unpack_half2(l0), d1 = unpack_half2(l1);
-      sum += (d0.x + d0.y) + (d1.x + d1.y);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (lane == 0) {
-        // scores = (k's constant part * sum + st * product * 8) * 2^-sh * scale
-        qinfo[i] = sum * ldexpf(p.qk_log2, -sh);
-        qinfo[kRows + i] = ldexpf(p.qk_log2, 3 - sh);
-        qmask[i] = R0 + i < p.rows ? row_mask(p.mask, b, p.T, (R0 + i) / p.G) : 0ull;
-      }
-    }
-  }
-  __syncthreads();
-
-  const uint32_t stage_base = tc::smem_u32(smem);
-  if (warp == kTWarps) {
-    // ------------------------------------------------------ producer warp --
-    if (lane == 0) {
-      bool ok = true;
-      int issued = 0;
-      int64_t pb = (p.head_blk + t_begin * kTWarps) % p.nbc;
-      for (int it = 0; it < ntiles && ok; ++it) {
-        const int s = it % kTStages;
-        if (it >= kTStages)
-          ok = tc::mbar_wait(empty0 + 8 * s, ((it / kTStages) - 1) & 1, p.err, 41);
-        if (!ok) break;
-        const int64_t j0 = (t_begin + it) * kTWarps;
-        const int nb = nlb_b - j0 < kTWarps ? (int)(nlb_b - j0) : kTWarps;
-        tc::mbar_arrive_expect_tx(full0 + 8 * s, nb * kRecBytes);
-        const uint32_t sb = stage_base + s * kTStageBytes;
-        if (p.table) {
-          for (int i = 0; i < nb; ++i) {  // a bad table entry reads page 0 and is reported
-            int64_t pg = checked_page(p.table, b * p.tstride + j0 + i, p.n_pages, p.err, 1008);
-            if (pg < 0) pg = 0;
-            tc::bulk_g2s(sb + i * kRecBytes, p.blocks + (pg * p.Hkv + kvh) * kRecWords, kRecBytes,
-                         full0 + 8 * s);
-          }
-        } else {
-          const int n1 = pb + nb <= p.nbc ? nb : (int)(p.nbc - pb);
-          tc::bulk_g2s(sb, p.blocks + (row * p.nbc + pb) * kRecWords, n1 * kRecBytes,
-                       full0 + 8 * s);
-          if (n1 < nb)
-            tc::bulk_g2s(sb + n1 * kRecBytes, p.blocks + row * p.nbc * kRecWords,
-                         (nb - n1) * kRecBytes, full0 + 8 * s);
-          pb += nb;
-          if (pb >= p.nbc) pb -= p.nbc;
-        }
-        ++issued;
-      }
-      // the copies of the last stages must land before the CTA may exit
-      for (int it = issued - kTStages < 0 ? 0 : issued - kTStages; it < issued; ++it)
-        tc::mbar_wait(full0 + 8 * (it % kTStages), (it / kTStages) & 1, p.err, 42);
-    }
-    return;
-  }
-
-  // -------------------------------------------------------- compute warps --
-  // rows g and g + 8 of the group (index h); slots r + 4a + 8bb + 16i of a block
-  const float qsum[2] = {qinfo[g], qinfo[g + 8]};
-  const float qscale[2] = {qinfo[kRows + g], qinfo[kRows + g + 8]};
-  float m_run[2] = {-INFINITY, -INFINITY}, Mref[2] = {-INFINITY, -INFINITY};
-  float wbound[2] = {0.0f, 0.0f};
-  float l_part[2] = {0.0f, 0.0f}, vm_part[2] = {0.0f, 0.0f};
-  int ew[2] = {0, 0};
-  float o[16][4];
-#pragma unroll
-  for (int n = 0; n < 16; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[n][c] = 0.0f;
-  bool ok = true;
-  // 32-bit slot arithmetic: the host keeps head_off + len below 2^31 - 64
-  const int nlb32 = (int)nlb_b, hoff = p.table ? 0 : (int)p.head_off, len32 = (int)len_b;
-  const int P = len32 - p.T;  // prefix length; negative: the first drafts do not exist
-  int j = (int)(t_begin * kTWarps) + warp;
-  for (int it = 0; it < ntiles; ++it, j += kTWarps) {
-    const int s = it % kTStages;
-    if (ok) ok = tc::mbar_wait(full0 + 8 * s, (it / kTStages) & 1, p.err, 43);
-    if (ok && j < nlb32) {
-      const uint32_t* rec =
-          reinterpret_cast<const uint32_t*>(smem + s * kTStageBytes + warp * kRecBytes);
-      // ---- scores.  Column n = g of tile (a, bb) is slot (g >> 1) + 4a + 8bb +
-      // 16 (g & 1), so that a lane's columns 2r, 2r+1 are the slots that its V
-      // words pair in one half2
-      float sc[2][2][4];
-      uint32_t kw[2][6];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const uint2* kp = reinterpret_cast<const uint2*>(rec + 12 * (4 * ((g >> 1) + 4 * a) + r) +
-                                                         6 * (g & 1));
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const uint2 x = kp[i];
-          kw[a][2 * i] = x.x;
-          kw[a][2 * i + 1] = x.y;
-        }
-#pragma unroll
-        for (int bb = 0; bb < 2; ++bb)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sc[a][bb][c] = 0.0f;
-      }
-      // (products of one sum are kept four apart: each waits for the one before)
-#define FT_TREE_KSTEP(Q)                                                                  \
-  {                                                                                       \
-    const uint4 ah = qf[(Q) * 32 + lane], al = qf[(8 + (Q)) * 32 + lane];                 \
-    uint32_t b0[2][2], b1[2][2];                                                          \
-    _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) { \
-      const uint32_t w0 = kw[a][3 * bb], w1 = kw[a][3 * bb + 1], w2 = kw[a][3 * bb + 2];  \
-      b0[a][bb] = quad_centred<Q, 0>(w0, w1, w2);                                         \
-      b1[a][bb] = quad_centred<Q, 1>(w0, w1, w2);                                         \
-      mma_f16(sc[a][bb], ah, b0[a][bb], b1[a][bb]);                                       \
-    }                                                                                     \
-    _Pragma("unroll") for (int a = 0; a < 2; ++a) _Pragma("unroll") for (int bb = 0; bb < 2; ++bb) \
-      mma_f16(sc[a][bb], al, b0[a][bb], b1[a][bb]);                                       \
-  }
-      FT_TREE_KSTEP(0) FT_TREE_KSTEP(1) FT_TREE_KSTEP(2) FT_TREE_KSTEP(3)
-      FT_TREE_KSTEP(4) FT_TREE_KSTEP(5) FT_TREE_KSTEP(6) FT_TREE_KSTEP(7)
-#undef FT_TREE_KSTEP
-      // ---- x = scale * q . k in the log2 domain; vs, vn: st and the constant part of V
-      float vs[2][2][2], vn[2][2][2];  // [a][bb][i]
-      const float4* kmm = reinterpret_cast<const float4*>(rec + kRecKmm);
-      const float4* vmm = reinterpret_cast<const float4*>(rec + kRecVmm);
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 km = kmm[(r + 4 * a) * 2 + i], vm = vmm[(r + 4 * a) * 2 + i];
-#pragma unroll
-          for (int bb = 0; bb < 2; ++bb) {
-            const float kmin = bb ? km.z : km.x, kmax = bb ? km.w : km.y;
-            const float vmin = bb ? vm.z : vm.x, vmax = bb ? vm.w : vm.y;
-            const float ks = (kmax - kmin) * 0.14285714285714285f;
-            vs[a][bb][i] = (vmax - vmin) * 0.14285714285714285f;
-            vn[a][bb][i] = fmaf(3.5f, vs[a][bb][i], vmin);
-            const float kc = fmaf(3.5f, ks, kmin);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              sc[a][bb][2 * h + i] =
-                  fmaf(kc, qsum[h], ks * (sc[a][bb][2 * h + i] * qscale[h]));
-          }
-        }
-      const int base = j * kBlk - hoff;
-      // blocks of the prefix are seen whole; the others slot by slot
-      const bool part = base < 0 || base + kBlk > P;
-      float mt[2], vx[2];
-      if (!part) {
-        float v = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) mt[h] = -INFINITY;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int bb = 0; bb < 2; ++bb)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              v = fmaxf(v, vs[a][bb][i] < INFINITY ? vs[a][bb][i] : 0.0f);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) mt[h] = fmaxf(mt[h], sc[a][bb][2 * h + i]);
-            }
-        vx[0] = vx[1] = v;
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint64_t mask = qmask[g + 8 * h];
-          mt[h] = -INFINITY;
-          vx[h] = 0.0f;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int bb = 0; bb < 2; ++bb)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int pos = base + r + 4 * a + 8 * bb + 16 * i;
-                const bool sees =
-                    pos >= 0 && pos < len32 && (pos < P || ((mask >> (pos - P)) & 1ull));
-                float& x = sc[a][bb][2 * h + i];
-                x = sees ? x : -INFINITY;
-                mt[h] = fmaxf(mt[h], x);
-                if (sees && vs[a][bb][i] < INFINITY) vx[h] = fmaxf(vx[h], vs[a][bb][i]);
-              }
-        }
-      }
-      // ---- running maximum and reference of the two rows
-      bool grow = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mt[h] = fmaxf(mt[h], __shfl_xor_sync(0xffffffffu, mt[h], 1));
-        mt[h] = fmaxf(mt[h], __shfl_xor_sync(0xffffffffu, mt[h], 2));
-        grow |= mt[h] > m_run[h] || vx[h] >= wbound[h];
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          vx[h] = fmaxf(vx[h], __shfl_xor_sync(0xffffffffu, vx[h], 1));
-          vx[h] = fmaxf(vx[h], __shfl_xor_sync(0xffffffffu, vx[h], 2));
-          if (vx[h] >= wbound[h]) {
-            const int e = bound_exp(vx[h]);
-            ew[h] = 15 - e;
-            wbound[h] = pow2i(e);
-          }
-          m_run[h] = fmaxf(m_run[h], mt[h]);
-          const float Mn = m_run[h] - (float)ew[h];
-          const float alpha = Mref[h] == -INFINITY ? 0.0f : exp2f(Mref[h] - Mn);
-          Mref[h] = Mn;
-          l_part[h] *= alpha;
-          vm_part[h] *= alpha;
-#pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            o[n][2 * h] *= alpha;
-            o[n][2 * h + 1] *= alpha;
-          }
-        }
-      }
-      // ---- weights w = p vs as A fragments of the two 16-slot steps a
-      uint4 ph[2], pl[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float M = Mref[h] == -INFINITY ? 0.0f : Mref[h];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int bb = 0; bb < 2; ++bb) {
-            float w[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float x = sc[a][bb][2 * h + i];
-              const float pr = ex2(x - M);
-              l_part[h] += pr;
-              w[i] = pr * vs[a][bb][i];
-              float vmv = pr * vn[a][bb][i];
-              if (part && x == -INFINITY) w[i] = vmv = 0.0f;  // whatever V holds there
-              vm_part[h] += vmv;
-            }
-            const uint32_t hi = pack_half2(w[0], w[1]);
-            // register of the fragment: row half h, k half bb
-            uint32_t& dst = bb ? (h ? ph[a].w : ph[a].z) : (h ? ph[a].y : ph[a].x);
-            dst = hi;
-            const float2 f = unpack_half2(hi);
-            uint32_t& dl = bb ? (h ? pl[a].w : pl[a].z) : (h ? pl[a].y : pl[a].x);
-            dl = pack_half2(w[0] - f.x, w[1] - f.y);
-          }
-      }
-      // ---- P.V: column n = g of n-tile 4m + jj is dim 8 (4m + jj) + g
-      const uint4* vp = reinterpret_cast<const uint4*>(rec + kRecV) + lane * 3;
-      uint32_t vw[12];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const uint4 x = vp[i];
-        vw[4 * i] = x.x;
-        vw[4 * i + 1] = x.y;
-        vw[4 * i + 2] = x.z;
-        vw[4 * i + 3] = x.w;
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const uint32_t w0 = vw[3 * m], w1 = vw[3 * m + 1], w2 = vw[3 * m + 2];
-        uint32_t bv[4][4];
-        float t[4][4];
-#define FT_TREE_VSTEP(JJ)                                      \
-  bv[JJ][0] = quad_centred<2 * (JJ), 0>(w0, w1, w2);           \
-  bv[JJ][1] = quad_centred<2 * (JJ), 1>(w0, w1, w2);           \
-  bv[JJ][2] = quad_centred<2 * (JJ) + 1, 0>(w0, w1, w2);       \
-  bv[JJ][3] = quad_centred<2 * (JJ) + 1, 1>(w0, w1, w2);       \
-  t[JJ][0] = t[JJ][1] = t[JJ][2] = t[JJ][3] = 0.0f;            \
-  mma_f16(t[JJ], ph[0], bv[JJ][0], bv[JJ][1]);
-        FT_TREE_VSTEP(0) FT_TREE_VSTEP(1) FT_TREE_VSTEP(2) FT_TREE_VSTEP(3)
-#undef FT_TREE_VSTEP
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], pl[0], bv[jj][0], bv[jj][1]);
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], ph[1], bv[jj][2], bv[jj][3]);
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) mma_f16(t[jj], pl[1], bv[jj][2], bv[jj][3]);
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[4 * m + jj][c] += t[jj][c];
-      }
-    }
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(empty0 + 8 * s);
-  }
-  // ---- the four warps merge in the stage buffers (every copy has been consumed)
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-      l_part[h] += __shfl_xor_sync(0xffffffffu, l_part[h], x);
-      vm_part[h] += __shfl_xor_sync(0xffffffffu, vm_part[h], x);
-    }
-    // scores that were all NaN leave no maximum but a NaN sum: keep the row
-    if (Mref[h] == -INFINITY && l_part[h] != l_part[h]) Mref[h] = 0.0f;
-  }
-  asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
-  float* red = reinterpret_cast<float*>(smem);  // [warp][row][2]: M, l
-  float* num = red + kTWarps * kRows * 2;        // [warp][row][128]
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = warp * kRows + g + 8 * h;
-    if (r == 0) {
-      red[2 * at] = Mref[h];
-      red[2 * at + 1] = l_part[h];
-    }
-#pragma unroll
-    for (int n = 0; n < 16; ++n)
-      *reinterpret_cast<float2*>(num + at * kD + 8 * n + 2 * r) =
-          make_float2(fmaf(o[n][2 * h], 8.0f, vm_part[h]),
-                      fmaf(o[n][2 * h + 1], 8.0f, vm_part[h]));
-  }
-  asm volatile("bar.sync 1, %0;" ::"r"(kTWarps * 32) : "memory");
-  for (int i = warp; i < kRows && R0 + i < p.rows; i += kTWarps) {
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kTWarps; ++w) M = fmaxf(M, red[2 * (w * kRows + i)]);
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kTWarps; ++w) {
-      const int at = w * kRows + i;
-      if (red[2 * at] == -INFINITY) continue;
-      const float f = exp2f(red[2 * at] - M);
-      l = fmaf(f, red[2 * at + 1], l);
-      const float4 v = reinterpret_cast<const float4*>(num + at * kD)[lane];
-      acc[0] = fmaf(f, v.x, acc[0]);
-      acc[1] = fmaf(f, v.y, acc[1]);
-      acc[2] = fmaf(f, v.z, acc[2]);
-      acc[3] = fmaf(f, v.w, acc[3]);
-    }
-    float* pp = p.part + ((row * p.rows + R0 + i) * p.nparts + split) * kTPart;
-    if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(M, l);
-    float2* pn = reinterpret_cast<float2*>(pp + 2) + 2 * lane;  // records are 8-byte aligned
-    pn[0] = make_float2(acc[0], acc[1]);
-    pn[1] = make_float2(acc[2], acc[3]);
-  }
-}
-
-// ------------------------------------------------- bf16 queries on tcgen05 --
+// ---------------------------------------------------------------- tiles --
 // S = Q K' (128 query rows x 128 positions a tile), then O += P V', on the
 // 5th-generation tensor core, K' and V' being the tile's codes as fp16.
 //
@@ -608,16 +189,20 @@ __global__ void __launch_bounds__((kTWarps + 1) * 32, 2)
 // so w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; M starts 8 below that
 // and moves only when a score passes the bound, by a power of two that the sums,
 // the P columns already written and O in TMEM are then scaled by.
-// O is summed in TMEM over the whole split: the tensor core truncates, 2^-25 of O
-// a step on average, 2^-14 after 2048 steps, against 2^-9 of the bf16 output; fp32
-// queries use tree_decode_kernel.
+// kTerms 1: bf16 queries, q and w as one fp16 each; 2: fp32 queries, hi and lo of
+// both, twice the products; P's hi and lo of a record take the columns of its
+// scores.  O is summed in TMEM over the whole split, where the tensor core
+// truncates, 2^-25 of O a product on average: 2^-14 after 2048 products, against
+// 2^-9 of the bf16 output; for fp32 a split has at most 8 tiles (64 products a
+// group: 2^-19 at most, 1e-6 as measured), the splits being merged in fp32.
 constexpr int kPreRows = 128;
 constexpr int kPreWarps = 28;
 constexpr int kPreRaw = 3;
 constexpr int kOperand = 128 * 128 * 2;  // bytes of Q, K' or V' (two swizzled panels)
-constexpr int kPreOffK = kOperand;
-constexpr int kPreOffV = kPreOffK + 2 * kOperand;
-constexpr int kPreOffRaw = kPreOffV + 2 * kOperand;
+// bf16 queries: Q, two K', two V'; fp32 queries: Q hi and lo, two K', one V'
+__host__ __device__ constexpr int off_k(int terms) { return terms * kOperand; }
+__host__ __device__ constexpr int off_v(int terms) { return (terms + 2) * kOperand; }
+constexpr int kPreOffRaw = 5 * kOperand;
 constexpr int kPreOffFac = kPreOffRaw + kPreRaw * kTStageBytes;
 constexpr int kFacBytes = 64 * 32 + 16;  // per position pair {st, st, kc, kc} {vst, vst, vc, vc}; e per record
 constexpr int kPreOffQinfo = kPreOffFac + 4 * kFacBytes;  // [128] sum term, [128] factor
@@ -625,7 +210,7 @@ constexpr int kPreOffMask = kPreOffQinfo + kPreRows * 8;  // [128] draft bits
 constexpr int kPreOffBars = kPreOffMask + kPreRows * 8;
 // what tree_query_kernel prepares for a row tile: the operand as it lies in shared
 // memory, then the row sums, factors and draft bits
-constexpr int kQImage = kOperand + kPreRows * 16;
+__host__ __device__ constexpr int q_image(int terms) { return terms * kOperand + kPreRows * 16; }
 static_assert(kPreOffMask == kPreOffQinfo + kPreRows * 8, "one copy brings both");
 constexpr int kPreBars = 2 * kPreRaw + 5 * 2 + 2 * 4 + 2;
 constexpr int kPreSmem = kPreOffBars + kPreBars * 8 + 16 + 1024;  // 1024: alignment
@@ -682,6 +267,7 @@ __device__ __forceinline__ int row_lane(int i) {
 // its own: every split of the positions needs the same operand, and its code,
 // fetched anew by each launch, took longer in the big kernel than here.
 constexpr int kQueryRows = 32;
+template <int kTerms>
 __global__ void __launch_bounds__(256) tree_query_kernel(const __grid_constant__ TreeParams p) {
   tc::pdl_launch_dependents();  // the tile kernel may start to load the cache
   const int64_t tile = blockIdx.x / (kPreRows / kQueryRows);  // (row, row tile)
@@ -689,7 +275,7 @@ __global__ void __launch_bounds__(256) tree_query_kernel(const __grid_constant__
   const int R0 = (int)(tile % p.rgroups) * kPreRows;
   const int i0 = (blockIdx.x % (kPreRows / kQueryRows)) * kQueryRows + (threadIdx.x >> 5) * 4;
   const int lane = threadIdx.x & 31;
-  uint8_t* img = p.qimg + tile * (int64_t)kQImage;
+  uint8_t* img = p.qimg + tile * (int64_t)q_image(kTerms);
   uint4 raw[4];
 #pragma unroll
   for (int y = 0; y < 4; ++y)
@@ -709,13 +295,20 @@ __global__ void __launch_bounds__(256) tree_query_kernel(const __grid_constant__
     const uint32_t h0 = pack_half2(v[0], v[2]), h1 = pack_half2(v[1], v[3]);
     const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
     float sum = (f0.x + f0.y) + (f1.x + f1.y);  // of the q that the products take
+    const int Q = lane >> 2, c = 4 * ((Q >> 1) & 1) + (lane & 3), at = row_lane(i);
+    uint8_t* to = img + (Q >> 2) * (kOperand / 2) + at * 128 + ((c ^ (at & 7)) << 4) + (Q & 1) * 8;
+    *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
+    if (kTerms == 2) {
+      const uint32_t l0 = pack_half2(v[0] - f0.x, v[2] - f0.y);
+      const uint32_t l1 = pack_half2(v[1] - f1.x, v[3] - f1.y);
+      const float2 d0 = unpack_half2(l0), d1 = unpack_half2(l1);
+      sum += (d0.x + d0.y) + (d1.x + d1.y);
+      *reinterpret_cast<uint2*>(to + kOperand) = make_uint2(l0, l1);
+    }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const int Q = lane >> 2, c = 4 * ((Q >> 1) & 1) + (lane & 3), at = row_lane(i);
-    *reinterpret_cast<uint2*>(img + (Q >> 2) * (kOperand / 2) + at * 128 + ((c ^ (at & 7)) << 4) +
-                              (Q & 1) * 8) = make_uint2(h0, h1);
     if (lane == y) {
-      float* info = reinterpret_cast<float*>(img + kOperand);
+      float* info = reinterpret_cast<float*>(img + kTerms * kOperand);
       info[at] = sum * ldexpf(p.qk_log2, -sh);
       info[kPreRows + at] = ldexpf(p.qk_log2, 3 - sh);
       reinterpret_cast<uint64_t*>(info + 2 * kPreRows)[at] = mask;
@@ -728,6 +321,7 @@ struct Masked {
   static constexpr bool value = kValue;
 };
 
+template <int kTerms>
 __global__ void __launch_bounds__(kPreWarps * 32, 1)
     tree_tile_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -810,10 +404,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             // the first records are on their way; the queries come from the
             // kernel before this one
             tc::pdl_wait();
-            const uint8_t* img = p.qimg + ((row * p.rgroups + R0 / kPreRows) * (int64_t)kQImage);
-            tc::mbar_arrive_expect_tx(q_full, kQImage);
-            tc::bulk_g2s(sbase, img, kOperand, q_full);
-            tc::bulk_g2s(sbase + kPreOffQinfo, img + kOperand, kQImage - kOperand, q_full);
+            const uint8_t* img =
+                p.qimg + (row * p.rgroups + R0 / kPreRows) * (int64_t)q_image(kTerms);
+            tc::mbar_arrive_expect_tx(q_full, q_image(kTerms));
+            tc::bulk_g2s(sbase, img, kTerms * kOperand, q_full);
+            tc::bulk_g2s(sbase + kPreOffQinfo, img + kTerms * kOperand, kPreRows * 16, q_full);
           }
           const int s = j % kPreRaw;
           if (j >= kPreRaw)
@@ -861,12 +456,13 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
         ok = tc::mbar_wait_sleep(k_full + 8 * s, (j >> 1) & 1, p.err, 53);
         if (!ok) return;
         tc::tc_fence_after();
-        const uint64_t kd = tc::smem_desc_sw128(sbase + kPreOffK + s * kOperand);
+        const uint64_t kd = tc::smem_desc_sw128(sbase + off_k(kTerms) + s * kOperand);
         if (tc::elect_one(leader)) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
-            tc::mma_f16_ss(tS + 128 * s, qd + at, kd + at, idesc, k > 0);
+          for (int k = 0; k < 8 * kTerms; ++k) {  // hi, then lo
+            const uint64_t at = (uint64_t)(((k >> 2) & 1) * (kOperand / 2) + (k & 3) * 32) >> 4;
+            tc::mma_f16_ss(tS + 128 * s, qd + at + (uint64_t)(k >> 3) * (kOperand >> 4), kd + at,
+                           idesc, k > 0);
           }
           tc::mma_commit(qk_done + 8 * s);
         }
@@ -875,15 +471,21 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       auto pv = [&](int j) {
         const int s = j & 1;
         ok = tc::mbar_wait_sleep(p_full + 8 * s, (j >> 1) & 1, p.err, 54) &&
-             tc::mbar_wait_sleep(v_full + 8 * s, (j >> 1) & 1, p.err, 55);
+             (kTerms == 1 ? tc::mbar_wait_sleep(v_full + 8 * s, (j >> 1) & 1, p.err, 55)
+                          : tc::mbar_wait_sleep(v_full, j & 1, p.err, 55));
         if (!ok) return;
         tc::tc_fence_after();
-        const uint64_t vd = tc::smem_desc_sw128(sbase + kPreOffV + s * kOperand);
+        const uint64_t vd =
+            tc::smem_desc_sw128(sbase + off_v(kTerms) + (kTerms == 1 ? s * kOperand : 0));
         if (tc::elect_one(leader)) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
-            tc::mma_f16_ts(tO + 128 * s, tS + 128 * s + 8 * k, vd + at, idesc, j >= 2 || k > 0);
+            // P of 16 positions: 8 columns; with two terms a record's hi and lo lie in the
+            // 32 columns of its scores
+            const uint32_t pc = tS + 128 * s + (kTerms == 1 ? 8 * k : 32 * (k >> 1) + 8 * (k & 1));
+            tc::mma_f16_ts(tO + 128 * s, pc, vd + at, idesc, j >= 2 || k > 0);
+            if (kTerms == 2) tc::mma_f16_ts(tO + 128 * s, pc + 16, vd + at, idesc, 1);
           }
           tc::mma_commit(pv_done + 8 * s);
         }
@@ -902,7 +504,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       tc::mbar_wait_sleep(fin, 0, p.err, 56);
     } else {
       // ----------------------------------------------------- factor warps --
-      // scores are st x product + kc x sum(q) (a code enters as 1 + c/8), values
+      // scores are st x product + kc x sum(q) (K' is 1 + c/8, or centred), values
       // vst x product + vc x sum(p) (as (c - 3.5)/8)
       const int half = warp - 26;
       bool ok = true;
@@ -925,7 +527,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
                           (oe == 1 ? 2 : (oe == 2 ? 1 : oe));
           float* fp = fac + (col >> 1) * 8 + (col & 1);
           fp[0] = ks;
-          fp[2] = fmaf(-8.0f, ks, km.x);
+          fp[2] = fmaf(kTerms == 1 ? -8.0f : 3.5f, ks, km.x);
           fp[4] = vs;
           fp[6] = fmaf(3.5f, vs, vm.x);
           int e = bound_exp(vs < INFINITY ? vs : 0.0f);
@@ -965,12 +567,17 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(raw_empty + 8 * (j % kPreRaw));
-      if (j >= 2) ok = tc::mbar_wait_sleep(done + 8 * (j & 1), ((j >> 1) - 1) & 1, p.err, 60);
+      // the operand's buffer: K' j - 2 multiplied, V' j - 2, or j - 1 where there is one
+      if (kTerms == 2 && isv) {
+        if (j >= 1) ok = tc::mbar_wait_sleep(done + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1, p.err, 60);
+      } else if (j >= 2) {
+        ok = tc::mbar_wait_sleep(done + 8 * (j & 1), ((j >> 1) - 1) & 1, p.err, 60);
+      }
       if (!ok) break;
       if (isv) {
         // triple m: dim 8 (4m + J) + g is row 8 (4m + J) + gk; chunk 4 (w % 2) + r of panel w / 2
-        uint8_t* at = smem + kPreOffV + (j & 1) * kOperand + (w >> 1) * (kOperand / 2) + gk * 128 +
-                      (((4 * (w & 1) + r) ^ gk) << 4);
+        uint8_t* at = smem + off_v(kTerms) + (kTerms == 1 ? (j & 1) * kOperand : 0) +
+                      (w >> 1) * (kOperand / 2) + gk * 128 + (((4 * (w & 1) + r) ^ gk) << 4);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const uint32_t w0 = wd[3 * m], w1 = wd[3 * m + 1], w2 = wd[3 * m + 2];
@@ -984,7 +591,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       } else {
         // slot gk + 8e is row 32w + 8 (gk % 4) + 4 (gk / 4) + (0 2 1 3)[e]; quads 2J, 2J + 1 go to
         // chunk 4 (J % 2) + r of panel J / 2
-        uint8_t* op = smem + kPreOffK + (j & 1) * kOperand + (32 * w + 8 * (gk & 3)) * 128;
+        uint8_t* op = smem + off_k(kTerms) + (j & 1) * kOperand + (32 * w + 8 * (gk & 3)) * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t w0 = wd[3 * e], w1 = wd[3 * e + 1], w2 = wd[3 * e + 2];
@@ -993,15 +600,21 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
           uint8_t* a1 = op + sub * 128 + (((r + 4) ^ sub) << 4);
 #define FT_PRE_K(J, AT)                                                                  \
   *reinterpret_cast<uint4*>(AT) =                                                         \
-      make_uint4(quad_half2<2 * (J), 0>(w0, w1, w2), quad_half2<2 * (J), 1>(w0, w1, w2),  \
-                 quad_half2<2 * (J) + 1, 0>(w0, w1, w2), quad_half2<2 * (J) + 1, 1>(w0, w1, w2));
+      kTerms == 1                                                                         \
+          ? make_uint4(quad_half2<2 * (J), 0>(w0, w1, w2), quad_half2<2 * (J), 1>(w0, w1, w2), \
+                       quad_half2<2 * (J) + 1, 0>(w0, w1, w2),                            \
+                       quad_half2<2 * (J) + 1, 1>(w0, w1, w2))                            \
+          : make_uint4(quad_centred<2 * (J), 0>(w0, w1, w2),                              \
+                       quad_centred<2 * (J), 1>(w0, w1, w2),                              \
+                       quad_centred<2 * (J) + 1, 0>(w0, w1, w2),                          \
+                       quad_centred<2 * (J) + 1, 1>(w0, w1, w2));
           FT_PRE_K(0, a0) FT_PRE_K(1, a1) FT_PRE_K(2, a0 + kOperand / 2) FT_PRE_K(3, a1 + kOperand / 2)
 #undef FT_PRE_K
         }
       }
       tc::fence_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(full + 8 * (j & 1));
+      if (lane == 0) tc::mbar_arrive(full + (kTerms == 2 && isv ? 0 : 8 * (j & 1)));
     }
   } else {
     // ------------------------------------------------------- softmax warps --
@@ -1118,7 +731,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             tc::tmem_wait_ld();
             tc::tmem_wait_st();
 #pragma unroll 1
-            for (int k = 0; k < c; ++k) {  // P columns of this tile
+            for (int k = 0; k < kTerms * c; ++k) {  // P columns of this tile
               uint32_t t[8];
               tc::tmem_ld_16x256b_x2(ts + 16 * k, t);
               tc::tmem_wait_ld();
@@ -1147,7 +760,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             tc::tmem_wait_st();
           }
         }
-        uint32_t pw[8];
+        uint32_t pw[8], pl[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float4 vf = f4[8 * k + 1];
@@ -1167,9 +780,14 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
               vm2[i] = add2(vm2[i], pair(vt.x, vt.y));
             }
             pw[2 * k + i] = pack_half2(wt.x, wt.y);
+            if (kTerms == 2) {
+              const float2 hi = unpack_half2(pw[2 * k + i]);
+              pl[2 * k + i] = pack_half2(wt.x - hi.x, wt.y - hi.y);
+            }
           }
         }
-        tc::tmem_st_16x128b_x4(ts + 16 * c, pw);
+        tc::tmem_st_16x128b_x4(ts + 16 * kTerms * c, pw);
+        if (kTerms == 2) tc::tmem_st_16x128b_x4(ts + 32 * c + 16, pl);
       }
       tc::tmem_wait_st();
     };
@@ -1275,6 +893,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nsplit = p.nparts;
   const int64_t R = blockIdx.x;
   const float* pp = p.part + R * nsplit * kTPart;
+  tc::pdl_wait();  // the tiles' partials
   float M = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int s = warp; s < nsplit; s += kCombineWarps) {
@@ -1339,22 +958,13 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
   }
 }
 
-// Opts the kernels into their dynamic shared memory (once per device) and
-// returns the resident CTAs per SM.
-int tree_occupancy(int device) {
-  static int cached[64] = {0};
-  if (device >= 0 && device < 64 && cached[device]) return cached[device];
-  cudaFuncSetAttribute(tree_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       kTreeSmem);
-  cudaFuncSetAttribute(tree_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
-  int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, tree_decode_kernel,
-                                                    (kTWarps + 1) * 32,
-                                                    kTreeSmem) != cudaSuccess ||
-      occ < 1)
-    occ = 1;
-  if (device >= 0 && device < 64) cached[device] = occ;
-  return occ;
+// Opts the kernels into their dynamic shared memory, once per device.
+void tree_opt_in(int device) {
+  static bool done[64] = {false};
+  if (device >= 0 && device < 64 && done[device]) return;
+  cudaFuncSetAttribute(tree_tile_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
+  cudaFuncSetAttribute(tree_tile_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
+  if (device >= 0 && device < 64) done[device] = true;
 }
 
 // Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost in
@@ -1379,6 +989,26 @@ int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t ove
 }
 
 constexpr int64_t kPreOverhead = 3;
+constexpr int64_t kTermTiles = 8;  // fp32 queries: most tiles of a split
+
+// Launch that may start before the kernel in front of it has ended; the kernel
+// waits for that one itself (griddepcontrol).
+template <class Kernel, class... Args>
+int launch_early(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  FT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  FT_LAUNCH_CHECK();
+  return FT_OK;
+}
 
 template <class Cache>
 int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_draft,
@@ -1409,48 +1039,34 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
   p.err = ctx->err_word;
   const int64_t total = batch * p.Hkv * p.rows;
   const int64_t ntiles = ceil_div(p.nlb, (int64_t)kTWarps);
-  const int occ = tree_occupancy(ctx->device);
-  const int crows = q_is_bf16 ? kPreRows : kRows;
-  p.rgroups = (p.rows + crows - 1) / crows;
+  tree_opt_in(ctx->device);
+  const int terms = q_is_bf16 ? 1 : 2;
+  p.rgroups = (p.rows + kPreRows - 1) / kPreRows;
   FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
            "decode grid too large");
-  p.tiles_per = q_is_bf16
-                    ? split_tiles(batch * p.Hkv * p.rgroups, ntiles, ctx->num_sms, kPreOverhead,
-                                  p.table != nullptr)
-                    : split_tiles(batch * p.Hkv * p.rgroups, ntiles, (int64_t)occ * ctx->num_sms, 2,
-                                  p.table != nullptr);
-  p.nparts = (int)ceil_div(ntiles, p.tiles_per);
   const int64_t tiles = batch * p.Hkv * p.rgroups;
-  const size_t images = q_is_bf16 ? (size_t)tiles * kQImage : 0;
+  p.tiles_per = split_tiles(tiles, ntiles, ctx->num_sms, kPreOverhead, p.table != nullptr);
+  if (terms == 2 && p.tiles_per > kTermTiles) p.tiles_per = kTermTiles;
+  p.nparts = (int)ceil_div(ntiles, p.tiles_per);
+  const size_t images = (size_t)tiles * q_image(terms);
   FT_CHECK(total < INT32_MAX && tiles < INT32_MAX / 4, FT_ERR_UNSUPPORTED, "too many query rows");
-  const int rc = ensure_ws(c->tree, images + (size_t)(total * p.nparts * kTPart) * 4, s,
-                           "tree decode", c->retired);
+  int rc = ensure_ws(c->tree, images + (size_t)(total * p.nparts * kTPart) * 4, s, "tree decode",
+                     c->retired);
   if (rc != FT_OK) return rc;
   p.qimg = static_cast<uint8_t*>(c->tree.ptr);
   p.part = reinterpret_cast<float*>(p.qimg + images);
-  dim3 grid((unsigned)p.nparts, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
-  if (q_is_bf16) {
-    tree_query_kernel<<<(unsigned)(tiles * (kPreRows / kQueryRows)), 256, 0, s>>>(p);
-    FT_LAUNCH_CHECK();
-    // starts while the query kernel runs, and waits for it before it reads the images
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(kPreWarps * 32);
-    cfg.dynamicSmemBytes = kPreSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    FT_CUDA(cudaLaunchKernelEx(&cfg, tree_tile_kernel, p));
-  } else {
-    tree_decode_kernel<<<grid, (kTWarps + 1) * 32, kTreeSmem, s>>>(p);
-  }
+  const unsigned qgrid = (unsigned)(tiles * (kPreRows / kQueryRows));
+  if (terms == 1)
+    tree_query_kernel<1><<<qgrid, 256, 0, s>>>(p);
+  else
+    tree_query_kernel<2><<<qgrid, 256, 0, s>>>(p);
   FT_LAUNCH_CHECK();
-  tree_combine_kernel<<<(unsigned)total, 32 * kCombineWarps, 0, s>>>(p, out_dev);
-  FT_LAUNCH_CHECK();
-  return FT_OK;
+  const dim3 grid((unsigned)p.nparts, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
+  rc = launch_early(terms == 1 ? tree_tile_kernel<1> : tree_tile_kernel<2>, grid, kPreWarps * 32,
+                    kPreSmem, s, p);
+  if (rc != FT_OK) return rc;
+  return launch_early(tree_combine_kernel, dim3((unsigned)total), 32 * kCombineWarps, 0, s, p,
+                      out_dev);
 }
 
 }  // namespace
