@@ -264,7 +264,13 @@ __global__ void __launch_bounds__(kD) kv3_append_kernel(AppendParams p) {
 // operations a lane and block, in the shadow of its 3584 bytes in and out.
 constexpr int kMoveWarps = 4;
 __device__ __forceinline__ uint32_t spread12(uint32_t f) {  // four 3-bit codes to four bytes
-  return (f & 7u) | (f & 0x38u) << 5 | (f & 0x1C0u) << 10 | (f & 0xE00u) << 15;
+  const uint32_t t = (f | f << 10) & 0x003F003Fu;
+  return (t | t << 5) & 0x07070707u;
+}
+__device__ __forceinline__ uint32_t gather12(uint32_t x) {  // and back (other bits ignored)
+  x &= 0x07070707u;
+  const uint32_t t = (x | x >> 5) & 0x003F003Fu;
+  return (t | t >> 10) & 0xFFFu;
 }
 
 // 48 bytes of a stream as 12 words; vec: the address is 16-byte aligned
@@ -498,103 +504,164 @@ __global__ void kv3_rotate_kernel(const float* __restrict__ in, float* __restric
 
 // The reference's stored form: codes [B][n][Hkv*48] bytes (pack_3bit over the
 // whole kv_dim vector) and (min, max) [B][n][Hkv][2].  One warp per (block of
-// the range, row), warps of a CTA on neighbouring kv heads; the record is read
-// into shared memory once and lane u rebuilds slot u's two streams from it
-// (the maps of kv3_append_packed_kernel, backwards).
-__global__ void __launch_bounds__(32 * kMoveWarps)
-    kv3_export_kernel(RangeParams p, int64_t nblk, int64_t total, uint8_t* __restrict__ kbytes,
+// the range, row), a CTA taking up to 8 neighbouring kv heads of one block: a
+// warp reads its record into shared memory, lane u rebuilds slot u's two streams
+// from it (the maps of kv3_append_packed_kernel, backwards), and the CTA writes
+// them out in order (each lane writing its own 48 bytes touched 32 lines a store:
+// 143 us for 16384 positions of 128 rows).
+constexpr int kExportHeads = 8;
+constexpr int kExportPad = 16;  // bytes after a position's streams: eight banks apart
+__host__ __device__ constexpr int export_stride(int heads) { return heads * kRec + kExportPad; }
+__host__ __device__ constexpr int export_smem(int heads) {
+  return heads * kRecBytes + 2 * kBlk * export_stride(heads);
+}
+__global__ void __launch_bounds__(32 * kExportHeads)
+    kv3_export_kernel(RangeParams p, int64_t nblk, uint8_t* __restrict__ kbytes,
                       float* __restrict__ kmm_out, uint8_t* __restrict__ vbytes,
                       float* __restrict__ vmm_out) {
-  __shared__ __align__(16) uint32_t stage[kMoveWarps][kRecWords];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * kMoveWarps + warp;
-  if (unit >= total) return;
-  const int64_t h = unit % p.Hkv, x = unit / p.Hkv % nblk, b = unit / (p.Hkv * nblk);
+  extern __shared__ __align__(16) uint8_t export_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = blockDim.x >> 5;
+  const int groups = (int)((p.Hkv + heads - 1) / heads);
+  const int64_t x = blockIdx.x / groups, b = blockIdx.y, h0 = blockIdx.x % groups * (int64_t)heads;
+  const int nh = p.Hkv - h0 < heads ? (int)(p.Hkv - h0) : heads;
   const int64_t off = p.table ? 0 : p.head % kBlk;
-  const int64_t lb = (p.start + off) / kBlk + x;  // logical block
-  const int64_t pos = lb * kBlk + lane - off - p.start;  // of lane's slot, within the range
-  const uint32_t* rec;
+  const int64_t lb = (p.start + off) / kBlk + x;    // logical block
+  const int64_t pos0 = lb * kBlk - off - p.start;   // of slot 0, within the range
+  const uint32_t* page = nullptr;                   // record of head 0
+  int64_t per_head = kRecWords;
   if (p.table) {
     const int64_t pg = checked_page(p.table, b * p.tstride + lb, p.n_pages, p.err, 1003);
-    if (pg < 0) return;
-    rec = p.blocks + (pg * p.Hkv + h) * kRecWords;
+    if (pg < 0) return;  // uniform over the block
+    page = p.blocks + pg * p.Hkv * kRecWords;
   } else {
-    rec = p.blocks + ((b * p.Hkv + h) * p.nbc + (p.head / kBlk + lb) % p.nbc) * kRecWords;
+    page = p.blocks + (b * p.Hkv * p.nbc + (p.head / kBlk + lb) % p.nbc) * kRecWords;
+    per_head = p.nbc * kRecWords;
   }
-  uint32_t* st = stage[warp];
-#pragma unroll
-  for (int i = 0; i < kRecBytes / 512; ++i)
-    reinterpret_cast<uint4*>(st)[32 * i + lane] = reinterpret_cast<const uint4*>(rec)[32 * i + lane];
-  __syncwarp();
-  if (pos < 0 || pos >= p.n) return;
-  const int64_t vec = (b * p.n + pos) * p.Hkv + h;
+  const int stride = export_stride(heads);
+  uint32_t* st = reinterpret_cast<uint32_t*>(export_sm) + warp * kRecWords;
+  uint8_t* outs = export_sm + heads * kRecBytes;  // [K, V][slot][head][48]
   uint32_t w[12];
-  auto store = [&](uint8_t* dst) {
-    if (((uintptr_t)dst & 15) == 0) {
+  auto store = [&](int which) {
+    uint4* dst = reinterpret_cast<uint4*>(outs + (which * kBlk + lane) * stride + warp * kRec);
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
-        reinterpret_cast<uint4*>(dst)[i] =
-            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else {
-      for (int i = 0; i < 12; ++i)
-        for (int k = 0; k < 4; ++k) dst[4 * i + k] = (uint8_t)(w[i] >> (8 * k));
-    }
+    for (int i = 0; i < 3; ++i)
+      dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   };
-  // K: the slot's triples lie in lanes 4(u % 8) + r
-  uint32_t f[4][8];
+  if (warp < nh) {
+    const uint32_t* rec = page + (h0 + warp) * per_head;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const uint32_t* t = st + (4 * (lane & 7) + r) * 12 + 3 * (lane >> 3);
-    const uint32_t w0 = t[0], w1 = t[1], w2 = t[2];
-    uint32_t q[8] = {w0, w0 >> 3, w1, w1 >> 3, w2, w2 >> 3, 0, 0};
-    q[6] = ((w0 >> 6) & 0x03030303u) | ((w2 >> 4) & 0x04040404u);
-    q[7] = ((w1 >> 6) & 0x03030303u) | ((w2 >> 5) & 0x04040404u);
+    for (int i = 0; i < kRecBytes / 512; ++i)
+      reinterpret_cast<uint4*>(st)[32 * i + lane] = reinterpret_cast<const uint4*>(rec)[32 * i + lane];
+    __syncwarp();
+    // K: the slot's triples lie in lanes 4(u % 8) + r
+    uint32_t f[4][8];
 #pragma unroll
-    for (int Q = 0; Q < 8; ++Q)
-      f[r][Q] = (q[Q] & 7u) | (q[Q] >> 5 & 0x38u) | (q[Q] >> 10 & 0x1C0u) | (q[Q] >> 15 & 0xE00u);
-  }
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t* t = st + (4 * (lane & 7) + r) * 12 + 3 * (lane >> 3);
+      const uint32_t w0 = t[0], w1 = t[1], w2 = t[2];
+      uint32_t q[8] = {w0, w0 >> 3, w1, w1 >> 3, w2, w2 >> 3, 0, 0};
+      q[6] = ((w0 >> 6) & 0x03030303u) | ((w2 >> 4) & 0x04040404u);
+      q[7] = ((w1 >> 6) & 0x03030303u) | ((w2 >> 5) & 0x04040404u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // 96 bits: the 12-bit fields of quads 2i and 2i + 1
-    w[3 * i] = f[0][2 * i] | f[1][2 * i] << 12 | f[2][2 * i] << 24;
-    w[3 * i + 1] = f[2][2 * i] >> 8 | f[3][2 * i] << 4 | f[0][2 * i + 1] << 16 | f[1][2 * i + 1] << 28;
-    w[3 * i + 2] = f[1][2 * i + 1] >> 4 | f[2][2 * i + 1] << 8 | f[3][2 * i + 1] << 20;
-  }
-  store(kbytes + vec * kRec);
-  // V: byte b, half a of the triples of lanes 4g + r
-  const int a = (lane >> 2) & 1, sb = 8 * (lane >> 3);
+      for (int Q = 0; Q < 8; ++Q)
+        f[r][Q] = gather12(q[Q]);
+    }
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    uint32_t G[4] = {0, 0, 0, 0};  // the 24-bit groups 4m + j
+    for (int i = 0; i < 4; ++i) {  // 96 bits: the 12-bit fields of quads 2i and 2i + 1
+      w[3 * i] = f[0][2 * i] | f[1][2 * i] << 12 | f[2][2 * i] << 24;
+      w[3 * i + 1] = f[2][2 * i] >> 8 | f[3][2 * i] << 4 | f[0][2 * i + 1] << 16 | f[1][2 * i + 1] << 28;
+      w[3 * i + 2] = f[1][2 * i + 1] >> 4 | f[2][2 * i + 1] << 8 | f[3][2 * i + 1] << 20;
+    }
+    store(0);
+    // V: byte b, half a of the triples of lanes 4g + r.  All four triples m at once:
+    // byte m of c[j] is the code of the 24-bit group 4m + j; the codes of two g make
+    // six bits of a byte, four such pairs a group.
+    const int a = (lane >> 2) & 1;
+    const uint32_t sel = (uint32_t)(lane >> 3) * 0x11u + 0x40u;
+    uint32_t pr[4][4];  // [pair of g][j]
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
-      const uint32_t* t = st + kRecV + (4 * g + (lane & 3)) * 12 + 3 * m;
-      const uint32_t y0 = t[0] >> sb, y1 = t[1] >> sb, y2 = t[2] >> sb;
-      G[0] |= ((y0 >> (3 * a)) & 7u) << (3 * g);
-      G[1] |= ((y1 >> (3 * a)) & 7u) << (3 * g);
-      G[2] |= ((y2 >> (3 * a)) & 7u) << (3 * g);
-      G[3] |= ((((a ? y1 : y0) >> 6) & 3u) | ((y2 >> (6 + a)) & 1u) << 2) << (3 * g);
+      const uint4* t4 = reinterpret_cast<const uint4*>(st + kRecV + (4 * g + (lane & 3)) * 12);
+      const uint4 t0 = t4[0], t1 = t4[1], t2 = t4[2];
+      const uint32_t y0 = __byte_perm(__byte_perm(t0.x, t0.w, sel), __byte_perm(t1.z, t2.y, sel), 0x5410);
+      const uint32_t y1 = __byte_perm(__byte_perm(t0.y, t1.x, sel), __byte_perm(t1.w, t2.z, sel), 0x5410);
+      const uint32_t y2 = __byte_perm(__byte_perm(t0.z, t1.y, sel), __byte_perm(t2.x, t2.w, sel), 0x5410);
+      const uint32_t c[4] = {(y0 >> (3 * a)) & 0x07070707u, (y1 >> (3 * a)) & 0x07070707u,
+                             (y2 >> (3 * a)) & 0x07070707u,
+                             (((a ? y1 : y0) >> 6) & 0x03030303u) |
+                                 ((y2 >> (4 + a)) & 0x04040404u)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (g & 1) pr[g >> 1][j] |= c[j] << 3;
+        else pr[g >> 1][j] = c[j];
+      }
     }
-    w[3 * m] = G[0] | G[1] << 24;
-    w[3 * m + 1] = G[1] >> 8 | G[2] << 16;
-    w[3 * m + 2] = G[2] >> 16 | G[3] << 8;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      uint32_t G[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        G[j] = ((pr[0][j] >> (8 * m)) & 63u) | ((pr[1][j] >> (8 * m)) & 63u) << 6 |
+               ((pr[2][j] >> (8 * m)) & 63u) << 12 | ((pr[3][j] >> (8 * m)) & 63u) << 18;
+      w[3 * m] = G[0] | G[1] << 24;
+      w[3 * m + 1] = G[1] >> 8 | G[2] << 16;
+      w[3 * m + 2] = G[2] >> 16 | G[3] << 8;
+    }
+    store(1);
   }
-  store(vbytes + vec * kRec);
-  const float2 km = reinterpret_cast<const float2*>(st + kRecKmm)[mm_index(lane)];
-  const float2 vm = reinterpret_cast<const float2*>(st + kRecVmm)[mm_index(lane)];
-  kmm_out[vec * 2] = km.x;
-  kmm_out[vec * 2 + 1] = km.y;
-  vmm_out[vec * 2] = vm.x;
-  vmm_out[vec * 2 + 1] = vm.y;
+  __syncthreads();
+  const bool vec = (((uintptr_t)kbytes | (uintptr_t)vbytes) & 15) == 0;
+  const int chunks = 3 * nh;
+  for (int i = threadIdx.x; i < kBlk * chunks; i += blockDim.x) {
+    const int u = i / chunks, c = i - u * chunks;
+    const int64_t pos = pos0 + u;
+    if (pos < 0 || pos >= p.n) continue;
+    const int64_t at = ((b * p.n + pos) * p.Hkv + h0) * kRec + 16 * c;
+    const uint4 k = *reinterpret_cast<const uint4*>(outs + u * stride + 16 * c);
+    const uint4 v = *reinterpret_cast<const uint4*>(outs + (kBlk + u) * stride + 16 * c);
+    if (vec) {
+      *reinterpret_cast<uint4*>(kbytes + at) = k;
+      *reinterpret_cast<uint4*>(vbytes + at) = v;
+    } else {
+      const uint32_t kk[4] = {k.x, k.y, k.z, k.w}, vv[4] = {v.x, v.y, v.z, v.w};
+      for (int y = 0; y < 16; ++y) {
+        kbytes[at + y] = (uint8_t)(kk[y >> 2] >> (8 * (y & 3)));
+        vbytes[at + y] = (uint8_t)(vv[y >> 2] >> (8 * (y & 3)));
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < kBlk * nh; i += blockDim.x) {
+    const int u = i / nh, h = i - u * nh;
+    const int64_t pos = pos0 + u;
+    if (pos < 0 || pos >= p.n) continue;
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(export_sm) + h * kRecWords;
+    const float2 km = reinterpret_cast<const float2*>(r + kRecKmm)[mm_index(u)];
+    const float2 vm = reinterpret_cast<const float2*>(r + kRecVmm)[mm_index(u)];
+    const int64_t at = ((b * p.n + pos) * p.Hkv + h0 + h) * 2;
+    kmm_out[at] = km.x;
+    kmm_out[at + 1] = km.y;
+    vmm_out[at] = vm.x;
+    vmm_out[at + 1] = vm.y;
+  }
 }
 
 int launch_export(const RangeParams& p, uint8_t* k, float* kmm, uint8_t* v, float* vmm,
                   cudaStream_t s) {
   const int64_t off = p.table ? 0 : p.head % kBlk;
   const int64_t nblk = (p.start + p.n + off + kBlk - 1) / kBlk - (p.start + off) / kBlk;
-  const int64_t total = p.B * nblk * p.Hkv;
-  FT_CHECK(ceil_div(total, kMoveWarps) < INT32_MAX, FT_ERR_UNSUPPORTED, "range too long");
-  kv3_export_kernel<<<(unsigned)ceil_div(total, kMoveWarps), 32 * kMoveWarps, 0, s>>>(
-      p, nblk, total, k, kmm, v, vmm);
+  const int heads = p.Hkv < kExportHeads ? (int)p.Hkv : kExportHeads;
+  const int64_t grid = nblk * ceil_div(p.Hkv, (int64_t)heads);
+  FT_CHECK(grid < INT32_MAX && p.B <= 65535, FT_ERR_UNSUPPORTED, "range too long");
+  static bool opted[64] = {false};  // once per device
+  int dev = 0;
+  FT_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !opted[dev]) {
+    FT_CUDA(cudaFuncSetAttribute(kv3_export_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 export_smem(kExportHeads)));
+    if (dev < 64) opted[dev] = true;
+  }
+  kv3_export_kernel<<<dim3((unsigned)grid, (unsigned)p.B), 32 * heads, export_smem(heads), s>>>(
+      p, nblk, k, kmm, v, vmm);
   FT_LAUNCH_CHECK();
   return FT_OK;
 }

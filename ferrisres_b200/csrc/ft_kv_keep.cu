@@ -35,7 +35,7 @@ struct SelectParams {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBins = 2048;
-static_assert(kSelBins == 2 * kSelThreads, "two bins a thread");
+static_assert(kSelBins == 2 * kSelThreads && kSelWarps == 32, "two bins a thread, a warp sum a lane");
 constexpr int kSelKeys = 40960;  // keys held in shared memory; further ones are read again
 constexpr int kSelSmem = kSelBins * 4 + 4 * 64 * 4;
 
@@ -133,8 +133,7 @@ __global__ void __launch_bounds__(kSelThreads)
     }
     if (lane == 0) red[warp] = inc;
     __syncthreads();
-    uint32_t above = inc - sum;
-    for (int k = warp + 1; k < kSelWarps; ++k) above += red[k];
+    const uint32_t above = inc - sum + __reduce_add_sync(0xffffffffu, lane > warp ? red[lane] : 0u);
     if (above < need && need <= above + sum) {  // exactly one thread
       const bool low = above + own[1] < need;
       bc[0] = (uint32_t)(2 * tid + (low ? 0 : 1));
@@ -165,14 +164,13 @@ __global__ void __launch_bounds__(kSelThreads)
     red[32 + warp] = eq;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0, e = 0;
-    for (int k = 0; k < kSelWarps; ++k) {
-      a += red[k];
-      e += red[32 + k];
+  if (warp == 0) {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, red[lane]);
+    const uint32_t e = __reduce_add_sync(0xffffffffu, red[32 + lane]);
+    if (lane == 0) {
+      bc[2] = a;
+      bc[3] = e;
     }
-    bc[2] = a;
-    bc[3] = e;
   }
   meet();
   uint32_t gt_before = 0, eq_before = 0;
@@ -180,10 +178,8 @@ __global__ void __launch_bounds__(kSelThreads)
     gt_before += cl.map_shared_rank(bc, c)[2];
     eq_before += cl.map_shared_rank(bc, c)[3];
   }
-  for (int k = 0; k < warp; ++k) {
-    gt_before += red[k];
-    eq_before += red[32 + k];
-  }
+  gt_before += __reduce_add_sync(0xffffffffu, lane < warp ? red[lane] : 0u);
+  eq_before += __reduce_add_sync(0xffffffffu, lane < warp ? red[32 + lane] : 0u);
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
     const uint32_t k = i < s1 ? key_at(i) : 0u;
@@ -348,101 +344,101 @@ __global__ void __launch_bounds__(32 * kKeepWarps, 2)
     uint32_t* home = lb < blk1 ? record(lb) : nullptr;
     const bool write = __any_sync(0xffffffffu, moved) && home != nullptr;
     if (write) {
-        const int sblk = (int)((src + off) / kBlk);
-        const uint32_t* mine = home;
-        if (moved) {
-          mine = record(sblk);
-          if (mine && staged)
-            mine = assembled + (kKeepWarps + at * kKeepSpan + sblk - lo) * kRecWords;
-        }
-        const bool bad = mine == nullptr;
-        if (bad) mine = home;  // reported; the slot keeps what it holds
-        const int slot = bad ? lane : (int)((src + off) % kBlk);
-        const unsigned long long base = (unsigned long long)mine;
-        reinterpret_cast<float2*>(buf + kRecKmm)[mm_index(lane)] =
-            reinterpret_cast<const float2*>(mine + kRecKmm)[mm_index(slot)];
-        reinterpret_cast<float2*>(buf + kRecVmm)[mm_index(lane)] =
-            reinterpret_cast<const float2*>(mine + kRecVmm)[mm_index(slot)];
-        // K: lane (g, r) assembles the triples of slots g + 8e
-        uint4* k4 = reinterpret_cast<uint4*>(buf + lane * 12);
-        uint32_t kd[12];
+      const int sblk = (int)((src + off) / kBlk);
+      const uint32_t* mine = home;
+      if (moved) {
+        mine = record(sblk);
+        if (mine && staged)
+          mine = assembled + (kKeepWarps + at * kKeepSpan + sblk - lo) * kRecWords;
+      }
+      const bool bad = mine == nullptr;
+      if (bad) mine = home;  // reported; the slot keeps what it holds
+      const int slot = bad ? lane : (int)((src + off) % kBlk);
+      const unsigned long long base = (unsigned long long)mine;
+      reinterpret_cast<float2*>(buf + kRecKmm)[mm_index(lane)] =
+          reinterpret_cast<const float2*>(mine + kRecKmm)[mm_index(slot)];
+      reinterpret_cast<float2*>(buf + kRecVmm)[mm_index(lane)] =
+          reinterpret_cast<const float2*>(mine + kRecVmm)[mm_index(slot)];
+      // K: lane (g, r) assembles the triples of slots g + 8e
+      uint4* k4 = reinterpret_cast<uint4*>(buf + lane * 12);
+      uint32_t kd[12];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, g + 8 * e);
-          const int t = __shfl_sync(0xffffffffu, slot, g + 8 * e);
-          const uint32_t* k = rec + (4 * (t & 7) + r) * 12 + 3 * (t >> 3);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t* rec = (const uint32_t*)__shfl_sync(0xffffffffu, base, g + 8 * e);
+        const int t = __shfl_sync(0xffffffffu, slot, g + 8 * e);
+        const uint32_t* k = rec + (4 * (t & 7) + r) * 12 + 3 * (t >> 3);
 #pragma unroll
-          for (int y = 0; y < 3; ++y) kd[3 * e + y] = k[y];
-        }
+        for (int y = 0; y < 3; ++y) kd[3 * e + y] = k[y];
+      }
 #pragma unroll
-        for (int y = 0; y < 3; ++y)
-          k4[y] = make_uint4(kd[4 * y], kd[4 * y + 1], kd[4 * y + 2], kd[4 * y + 3]);
-        // V: lane (g, r) assembles slots u = r + 4a + 8bb, byte bb of its words, from
-        // lane 4g + t % 4 of the source's record.  Positions that keep their distance
-        // share that lane, so its 48 bytes are loaded when they change.
-        // The work is done on the four triples m at once: z[w][bb] holds word w's byte
-        // of triple m in byte m, and is transposed at the end.
-        uint32_t x[12], z[3][4];
-        unsigned long long have = 0;
+      for (int y = 0; y < 3; ++y)
+        k4[y] = make_uint4(kd[4 * y], kd[4 * y + 1], kd[4 * y + 2], kd[4 * y + 3]);
+      // V: lane (g, r) assembles slots u = r + 4a + 8bb, byte bb of its words, from
+      // lane 4g + t % 4 of the source's record.  Positions that keep their distance
+      // share that lane, so its 48 bytes are loaded when they change.
+      // The work is done on the four triples m at once: z[w][bb] holds word w's byte
+      // of triple m in byte m, and is transposed at the end.
+      uint32_t x[12], z[3][4];
+      unsigned long long have = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int a = q & 1, bb = q >> 1, u = r + 4 * q;
-          const unsigned long long rb = __shfl_sync(0xffffffffu, base, u);
-          const int t = __shfl_sync(0xffffffffu, slot, u);
-          const unsigned long long from = rb + 4 * (kRecV + (4 * g + (t & 3)) * 12);
-          if (from != have) {
-            have = from;
-            const uint4* v4 = reinterpret_cast<const uint4*>(from);
+      for (int q = 0; q < 8; ++q) {
+        const int a = q & 1, bb = q >> 1, u = r + 4 * q;
+        const unsigned long long rb = __shfl_sync(0xffffffffu, base, u);
+        const int t = __shfl_sync(0xffffffffu, slot, u);
+        const unsigned long long from = rb + 4 * (kRecV + (4 * g + (t & 3)) * 12);
+        if (from != have) {
+          have = from;
+          const uint4* v4 = reinterpret_cast<const uint4*>(from);
 #pragma unroll
-            for (int y = 0; y < 3; ++y) {
-              const uint4 v = v4[y];
-              x[4 * y] = v.x;
-              x[4 * y + 1] = v.y;
-              x[4 * y + 2] = v.z;
-              x[4 * y + 3] = v.w;
-            }
-          }
-          // byte t / 8 of word w of each triple; half a of a triple (quads 2j + a) is bits
-          // 0-2 (a = 0) or 3-5 (a = 1) of each byte, plus bits 6-7 of byte 0 or 1 and bit 6
-          // or 7 of byte 2
-          const int sa = (t >> 2) & 1;
-          const uint32_t sel = (uint32_t)(t >> 3) * 0x11u + 0x40u;
-          uint32_t y[3];
-#pragma unroll
-          for (int w = 0; w < 3; ++w)
-            y[w] = __byte_perm(__byte_perm(x[w], x[3 + w], sel), __byte_perm(x[6 + w], x[9 + w], sel),
-                               0x5410);
-          const uint32_t lo2 = ((sa ? y[1] : y[0]) >> 6) & 0x03030303u;
-          const uint32_t hi1 = (y[2] >> (6 + sa)) & 0x01010101u;
-          const uint32_t c0 = (y[0] >> (3 * sa)) & 0x07070707u;
-          const uint32_t c1 = (y[1] >> (3 * sa)) & 0x07070707u;
-          const uint32_t c2 = (y[2] >> (3 * sa)) & 0x07070707u;
-          if (a == 0) {
-            z[0][bb] = c0 | lo2 << 6;
-            z[1][bb] = c1;
-            z[2][bb] = c2 | hi1 << 6;
-          } else {
-            z[0][bb] |= c0 << 3;
-            z[1][bb] |= c1 << 3 | lo2 << 6;
-            z[2][bb] |= c2 << 3 | hi1 << 7;
+          for (int y = 0; y < 3; ++y) {
+            const uint4 v = v4[y];
+            x[4 * y] = v.x;
+            x[4 * y + 1] = v.y;
+            x[4 * y + 2] = v.z;
+            x[4 * y + 3] = v.w;
           }
         }
-        uint32_t vd[12];
+        // byte t / 8 of word w of each triple; half a of a triple (quads 2j + a) is bits
+        // 0-2 (a = 0) or 3-5 (a = 1) of each byte, plus bits 6-7 of byte 0 or 1 and bit 6
+        // or 7 of byte 2
+        const int sa = (t >> 2) & 1;
+        const uint32_t sel = (uint32_t)(t >> 3) * 0x11u + 0x40u;
+        uint32_t y[3];
 #pragma unroll
-        for (int w = 0; w < 3; ++w) {  // 4 x 4 bytes: (bb, m) to (m, bb)
-          const uint32_t p01l = __byte_perm(z[w][0], z[w][1], 0x5140);
-          const uint32_t p01h = __byte_perm(z[w][0], z[w][1], 0x7362);
-          const uint32_t p23l = __byte_perm(z[w][2], z[w][3], 0x5140);
-          const uint32_t p23h = __byte_perm(z[w][2], z[w][3], 0x7362);
-          vd[w] = __byte_perm(p01l, p23l, 0x5410);
-          vd[3 + w] = __byte_perm(p01l, p23l, 0x7632);
-          vd[6 + w] = __byte_perm(p01h, p23h, 0x5410);
-          vd[9 + w] = __byte_perm(p01h, p23h, 0x7632);
+        for (int w = 0; w < 3; ++w)
+          y[w] = __byte_perm(__byte_perm(x[w], x[3 + w], sel), __byte_perm(x[6 + w], x[9 + w], sel),
+                             0x5410);
+        const uint32_t lo2 = ((sa ? y[1] : y[0]) >> 6) & 0x03030303u;
+        const uint32_t hi1 = (y[2] >> (6 + sa)) & 0x01010101u;
+        const uint32_t c0 = (y[0] >> (3 * sa)) & 0x07070707u;
+        const uint32_t c1 = (y[1] >> (3 * sa)) & 0x07070707u;
+        const uint32_t c2 = (y[2] >> (3 * sa)) & 0x07070707u;
+        if (a == 0) {
+          z[0][bb] = c0 | lo2 << 6;
+          z[1][bb] = c1;
+          z[2][bb] = c2 | hi1 << 6;
+        } else {
+          z[0][bb] |= c0 << 3;
+          z[1][bb] |= c1 << 3 | lo2 << 6;
+          z[2][bb] |= c2 << 3 | hi1 << 7;
         }
-        uint4* v4 = reinterpret_cast<uint4*>(buf + kRecV + lane * 12);
+      }
+      uint32_t vd[12];
 #pragma unroll
-        for (int y = 0; y < 3; ++y)
-          v4[y] = make_uint4(vd[4 * y], vd[4 * y + 1], vd[4 * y + 2], vd[4 * y + 3]);
+      for (int w = 0; w < 3; ++w) {  // 4 x 4 bytes: (bb, m) to (m, bb)
+        const uint32_t p01l = __byte_perm(z[w][0], z[w][1], 0x5140);
+        const uint32_t p01h = __byte_perm(z[w][0], z[w][1], 0x7362);
+        const uint32_t p23l = __byte_perm(z[w][2], z[w][3], 0x5140);
+        const uint32_t p23h = __byte_perm(z[w][2], z[w][3], 0x7362);
+        vd[w] = __byte_perm(p01l, p23l, 0x5410);
+        vd[3 + w] = __byte_perm(p01l, p23l, 0x7632);
+        vd[6 + w] = __byte_perm(p01h, p23h, 0x5410);
+        vd[9 + w] = __byte_perm(p01h, p23h, 0x7632);
+      }
+      uint4* v4 = reinterpret_cast<uint4*>(buf + kRecV + lane * 12);
+#pragma unroll
+      for (int y = 0; y < 3; ++y)
+        v4[y] = make_uint4(vd[4 * y], vd[4 * y + 1], vd[4 * y + 2], vd[4 * y + 3]);
     }
     tc::fence_async_smem();
     if (C > 1) cl.sync();
@@ -473,6 +469,11 @@ template <class Kernel, class... Args>
 int launch_cluster(Kernel kernel, int64_t rows, int cluster, int threads, size_t smem,
                    cudaStream_t s, Args... args) {
   FT_CHECK(rows * cluster < INT32_MAX, FT_ERR_UNSUPPORTED, "too many (sequence, head) rows");
+  if (cluster == 1) {  // a plain launch is a cluster of one, and cheaper
+    kernel<<<(unsigned)rows, threads, smem, s>>>(args...);
+    FT_LAUNCH_CHECK();
+    return FT_OK;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
   cfg.blockDim = dim3((unsigned)threads);

@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
     const uint32_t lanes = (uint32_t)(32 * quad + 16 * half) << 16;
     const int row0 = 32 * quad + 16 * half + g;
     const bool live = 64 * half + 16 * quad < nrows;  // this warp's rows exist
-    // 32-bit slot arithmetic: the host keeps head_off + len below 2^31 - 64
+    // 32-bit slot arithmetic: the host keeps len below 2^31 - 512
     const int hoff = p.table ? 0 : (int)p.head_off, len32 = (int)len_b;
     const int P = len32 - p.T;  // prefix length; negative: the first drafts do not exist
     uint64_t qsum[2], qfac[2], l2[2], vm2[2], negM[2];
@@ -1082,7 +1082,7 @@ int ft_kv3_tree_decode(ft_ctx* ctx, ft_kv3* c, int64_t n_draft, const void* q_de
   FT_CHECK(ctx && c && q_dev && out_dev, FT_ERR_SHAPE, "null argument");
   FT_CHECK(n_draft <= c->len, FT_ERR_SHAPE, "%lld drafts in a cache of %lld positions",
            (long long)n_draft, (long long)c->len);
-  FT_CHECK(c->len + kBlk < (int64_t)INT32_MAX - 64, FT_ERR_UNSUPPORTED,
+  FT_CHECK(c->len < (int64_t)INT32_MAX - 512, FT_ERR_UNSUPPORTED,
            "cache too long for the decode's 32-bit slot arithmetic");
   DeviceScope scope(c->device);
   TreeParams p{};
@@ -1104,7 +1104,7 @@ int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tab
                max_seq_len <= table_stride * kBlk,
            FT_ERR_SHAPE, "bad decode shape (batch %lld, max_seq_len %lld, table stride %lld)",
            (long long)batch, (long long)max_seq_len, (long long)table_stride);
-  FT_CHECK(max_seq_len + kBlk < (int64_t)INT32_MAX - 64, FT_ERR_UNSUPPORTED,
+  FT_CHECK(max_seq_len < (int64_t)INT32_MAX - 512, FT_ERR_UNSUPPORTED,
            "sequence too long for the decode's 32-bit slot arithmetic");
   DeviceScope scope(c->device);
   TreeParams p{};

@@ -84,8 +84,8 @@ def select_heavy(weights: torch.Tensor, n_keep: int, n_recent: int = 0, length: 
     n_keep, n_recent = int(n_keep), int(n_recent)
     if n_keep < 1 or not 0 <= n_recent <= n_keep:
         raise ShapeError("0 <= n_recent <= n_keep and n_keep >= 1 are expected")
-    idx = torch.empty((B, H, n_keep), dtype=torch.int32, device=dev)
-    out = torch.empty((B, H, W), dtype=torch.float32, device=dev)
+    idx = weights.new_empty((B, H, n_keep), dtype=torch.int32)
+    out = weights.new_empty((B, H, W))
     if B == 0:
         return idx, out
     lens = None if seq_lens is None else seq_lens.contiguous()
@@ -307,7 +307,9 @@ class Kv3Cache:
         [batch, kv_heads, >= len] stay (``select_heavy``).  Returns (idx, weights): the
         kept old positions and the weights that belong to the new ones."""
         n = len(self)
-        _row_stride(weights, (self.batch, self.kv_heads), n, "weights", self.device)
+        if tuple(weights.shape[:2]) != (self.batch, self.kv_heads) or weights.device != self.device:
+            raise ShapeError(f"weights must be fp32 [{self.batch}, {self.kv_heads}, >= {n}] "
+                             f"on {self.device}")
         idx, out = select_heavy(weights, n_keep, n_recent, length=n, stream=stream)
         if n > int(n_keep):
             self._keep(idx, int(n_keep), self.kv_heads * int(n_keep), int(n_keep), 0, stream)

@@ -322,6 +322,50 @@ def test_keep_list_forms_and_refusals(kv):
     c.close()
 
 
+def test_keep_nothing_and_evict_nothing(kv):
+    g = generator(40)
+    c = kv.Kv3Cache(2, 2, 64)
+    x = rand(g, 2, 40, 2, D)
+    none = torch.empty((2, 2, 0), dtype=torch.int32, device="cuda")
+    idx, w = c.evict_heavy(torch.zeros((2, 2, 8), device="cuda"), 4, 2)  # an empty cache
+    assert bool((idx == -1).all()) and bool((w == 0).all()) and len(c) == 0
+    c.append(x, x)
+    before = stored(c, 0, 40)
+    c.keep(none, start=33)  # rejected drafts: the cache is cut
+    assert len(c) == 33
+    for a, b in zip(stored(c, 0, 33), before):
+        assert (a == b[:, :33]).all()
+    c.keep(none)
+    assert len(c) == 0
+    c.append(x, x)
+    for a, b in zip(stored(c, 0, 40), before):
+        assert (a == b).all()
+    c.ctx.check()
+    c.close()
+
+
+@pytest.mark.parametrize("share", [0.97, 0.6, 0.2, 0.03])
+def test_keep_shares(kv, share):
+    """Sources that span few records, many, and far more than are staged at once."""
+    rng, g = np.random.default_rng(int(100 * share)), generator(41)
+    B, H, n = 2, 3, 6000
+    c = kv.Kv3Cache(B, H, n)
+    c.append(rand(g, B, n, H, D), rand(g, B, n, H, D))
+    before = stored(c, 0, n)
+    idx = random_lists(rng, B, H, n, int(n * share))
+    c.keep(torch.from_numpy(idx).cuda())
+    assert_store(stored(c, 0, idx.shape[2]), gather(before, idx, H))
+    # not ascending, but no entry below its place
+    m = idx.shape[2] // 2
+    free = np.stack([np.stack([rng.integers(np.arange(m), idx.shape[2]) for _ in range(H)])
+                     for _ in range(B)]).astype(np.int32)
+    before = stored(c, 0, idx.shape[2])
+    c.keep(torch.from_numpy(free).cuda())
+    assert_store(stored(c, 0, m), gather(before, free, H))
+    c.ctx.check()
+    c.close()
+
+
 def test_evict_heavy(kv):
     g, rng = generator(5), np.random.default_rng(5)
     B, H, n, keep, recent = 2, 2, 1000, 600, 64

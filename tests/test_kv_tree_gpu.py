@@ -367,6 +367,34 @@ def test_short_empty_and_bad_sequences(paged):
     c.close()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_and_a_graph(kv, dtype):
+    """Caches of their own on streams of their own, one call captured: results as one by one."""
+    g = generator(30)
+    caches, qs, refs = [], [], []
+    for i, n in enumerate((900, 2600)):
+        c = kv.Kv3Cache(2, 2, n)
+        c.append(rand(g, 2, n, 2, D), rand(g, 2, n, 2, D))
+        caches.append(c)
+        qs.append((2 * rand(g, 2, 40, 8, D)).to(dtype))
+        refs.append(c.tree_decode(qs[i]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    out = torch.empty_like(qs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caches[0].tree_decode(qs[0], out=out)
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        got = caches[1].tree_decode(qs[1], stream=streams[1])
+    torch.cuda.synchronize()
+    assert torch.equal(out, refs[0]) and torch.equal(got, refs[1])
+    for c in caches:
+        c.ctx.check()
+        c.close()
+
+
 def test_refusals(kv, paged):
     from ferrisres_b200._lib import ShapeError, UnsupportedError
     c = kv.Kv3Cache(1, 2, 64)
