@@ -226,8 +226,8 @@ constexpr int kKeepSmem = (2 * kKeepSpan + kKeepWarps) * kRecBytes;
 // The sources of a CTA's 256 positions span few blocks when most positions stay:
 // up to kKeepSpan records come in by one bulk copy, each read once, while the round
 // before is assembled; a wider span is gathered from global memory.  (16384 of 17408
-// positions of 128 rows: all gathers from global memory 171 us, staged without the
-// overlap 180.)
+// positions of 128 rows: 133 us; all gathers from global memory 171 us, staged without
+// the overlap 180.)
 // Gathering one slot: its K codes are 4 triples (one a lane r, copied as they
 // are); its V codes are one byte lane of three words in each of 8 lanes and 4
 // triples, 6 bits of 8 x 3, which move to the byte and the half (a) of the
@@ -552,7 +552,7 @@ int ft_kv_select_heavy(ft_ctx* ctx, int64_t batch, int64_t kv_heads, const float
   p.err = ctx->err_word;
   const int64_t rows = batch * kv_heads;
   // one CTA a row up to 32 keys a thread: the cluster's barriers cost more than they
-  // save (16384 keys a row, 128 rows: 50 us on clusters of four)
+  // save (16384 keys a row, 128 rows: 50 us on clusters of four, 22.5 so)
   const int c = cluster_size(ctx->num_sms, rows, max_seq_len, 32 * kSelThreads);
   // keys that do not fit shared memory are read from global memory again
   const int64_t share = ceil_div(max_seq_len, c);

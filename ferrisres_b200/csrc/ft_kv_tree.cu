@@ -23,9 +23,9 @@
 // aligns a product by the operands' exponents and drops the low bits: 2^-12 of
 // the result were lost.)  Softmax statistics, the sum terms and the merge of the
 // splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
-// With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 24
-// drafts of 6 sequences took 104 us where tree_tile_kernel takes 47, and 64 drafts
-// over 8 x 32768 positions 1868 us where it takes 541.
+// With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 32
+// drafts over 8192 positions took 86 us where this takes 43 (32 q heads, bf16), and
+// 64 drafts over 8 x 32768 positions 1868 us where it takes 538.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -884,8 +884,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 }
 
 // Merges the split partials of a row: one CTA a row, its warps share the splits
-// (so that all loads are in flight at once; a warp a row took 13 us over 512 rows x
-// 17 splits, this 4), 4 dims a lane; mode T: the output is rotated back.
+// (so that more loads are in flight at once: with a warp a row the decode of 32 drafts
+// over 8192 positions takes 49.5 us, so 45.5), 4 dims a lane; mode T: the output is rotated back.
 constexpr int kCombineWarps = 4;
 __global__ void __launch_bounds__(32 * kCombineWarps)
     tree_combine_kernel(const __grid_constant__ TreeParams p, void* __restrict__ out) {
@@ -967,17 +967,22 @@ void tree_opt_in(int device) {
   if (device >= 0 && device < 64) done[device] = true;
 }
 
-// Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost in
-// tiles).  Paged sequences differ in length, which only the device knows: there the
-// splits are made small enough for three waves, down to four tiles, so that CTAs of
-// short sequences make room (6 sequences of 2006 to 8191 positions, 24 drafts: 104 us
-// with splits for equal lengths).
+// Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost, which
+// is about three tiles' time: counted as 1 or 6 of them, 64 drafts over 8 x 32768
+// positions take 547 or 556 us, as 3 they take 544).  Paged sequences differ in length,
+// which only the device knows: there the splits are made small enough for three waves,
+// down to eight tiles, so that CTAs of short sequences make room.  64 drafts over 8
+// sequences of 500 to 11469 positions: 163 us, 235 with splits for equal lengths, 182
+// with two waves; down to four tiles, 24 drafts over 6 sequences of 2006 to 8191
+// positions take 61 us in the tile kernel where they take 55.
+constexpr int64_t kPreOverhead = 3;
+constexpr int64_t kFineTiles = 8;
 int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t overhead,
                     bool ragged) {
   int64_t best_cost = INT64_MAX, best = ntiles;
   for (int64_t sp = 1; sp <= 256 && sp <= ntiles; ++sp) {
     const int64_t per = ceil_div(ntiles, sp), ctas = units * ceil_div(ntiles, per);
-    if (ragged && per > 4 && ctas < 3 * resident && sp < 256 && sp < ntiles) continue;
+    if (ragged && per > kFineTiles && ctas < 3 * resident && sp < 256 && sp < ntiles) continue;
     const int64_t waves = ceil_div(ctas, resident);
     const int64_t cost = waves * (per + overhead);
     if (cost < best_cost) {
@@ -988,7 +993,6 @@ int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t ove
   return best;
 }
 
-constexpr int64_t kPreOverhead = 3;
 constexpr int64_t kTermTiles = 8;  // fp32 queries: most tiles of a split
 
 // Launch that may start before the kernel in front of it has ended; the kernel

@@ -72,22 +72,25 @@ def select_heavy(weights: torch.Tensor, n_keep: int, n_recent: int = 0, length: 
     (idx, weights): idx int32 [batch, kv_heads, n_keep], ascending, -1 where a sequence
     has fewer positions; a new weights tensor of the same shape with the kept
     positions' weights in front and zeros behind."""
-    if weights.dim() != 3 or not weights.is_cuda:
+    if not isinstance(weights, torch.Tensor) or weights.dim() != 3 or not weights.is_cuda:
         raise ShapeError("weights must be fp32 [batch, kv_heads, positions] on a GPU")
     B, H, W = weights.shape
     length = W if length is None else int(length)
     dev = weights.device
+    if length < 0:
+        raise ShapeError("a length is not negative")
     step = _row_stride(weights, (B, H), length, "weights", dev)
-    if seq_lens is not None and (seq_lens.dtype != torch.int32 or seq_lens.device != dev or
-                                 tuple(seq_lens.shape) != (B,)):
+    if seq_lens is not None and (not isinstance(seq_lens, torch.Tensor) or
+                                 seq_lens.dtype != torch.int32 or
+                                 seq_lens.device != dev or tuple(seq_lens.shape) != (B,)):
         raise ShapeError(f"seq_lens must be int32 [{B}] on {dev}")
     n_keep, n_recent = int(n_keep), int(n_recent)
     if n_keep < 1 or not 0 <= n_recent <= n_keep:
         raise ShapeError("0 <= n_recent <= n_keep and n_keep >= 1 are expected")
     idx = weights.new_empty((B, H, n_keep), dtype=torch.int32)
     out = weights.new_empty((B, H, W))
-    if B == 0:
-        return idx, out
+    if B == 0 or W == 0:
+        return idx.fill_(-1), out
     lens = None if seq_lens is None else seq_lens.contiguous()
     call("ft_kv_select_heavy", get_context(dev.index).handle, B, H, C.c_void_p(weights.data_ptr()),
          step, None if lens is None else _dptr(lens), length, n_keep, n_recent, _dptr(idx),
@@ -123,16 +126,16 @@ def _tree_args(q: torch.Tensor, mask, batch: int, device, out):
     if q.data_ptr() % 16:  # a view that starts inside a row of its storage
         q = q.clone()
     if mask is not None:
-        if mask.device != device or mask.dtype != torch.int64 or \
-                mask.shape not in ((T,), (batch, T)):
+        if not isinstance(mask, torch.Tensor) or mask.device != device or mask.dtype != torch.int64 \
+                or mask.shape not in ((T,), (batch, T)):
             raise ShapeError(f"mask must be int64 [{T}] or [{batch}, {T}] on {device}")
         if mask.dim() == 1:
             mask = mask.expand(batch, T)
         mask = mask.contiguous()
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or \
-            not out.is_contiguous() or out.data_ptr() % 16:
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or \
+            out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ShapeError("out must be contiguous, 16-byte aligned and like q")
     return q, mask, out
 
@@ -293,7 +296,9 @@ class Kv3Cache:
         position start + i is old position idx[..., i] for each sequence and kv head
         (idx [n], [batch, n] or [batch, kv_heads, n], ascending from ``start`` on).  After
         a tree decode: the accepted path.  An entry outside [start + i, len) is skipped
-        and reported by ``ctx.check()``."""
+        and reported by ``ctx.check()``.  (A ring that is full from the middle of a block
+        on may be laid out anew, as by an append that grows it: graphs captured before
+        then no longer hold.)"""
         idx, n, (ib, ih) = _index_list(idx, self.batch, self.kv_heads, self.device)
         self._keep(idx, n, ib, ih, int(start), stream)
 
@@ -307,7 +312,8 @@ class Kv3Cache:
         [batch, kv_heads, >= len] stay (``select_heavy``).  Returns (idx, weights): the
         kept old positions and the weights that belong to the new ones."""
         n = len(self)
-        if tuple(weights.shape[:2]) != (self.batch, self.kv_heads) or weights.device != self.device:
+        if not isinstance(weights, torch.Tensor) or weights.device != self.device or \
+                tuple(weights.shape[:2]) != (self.batch, self.kv_heads):
             raise ShapeError(f"weights must be fp32 [{self.batch}, {self.kv_heads}, >= {n}] "
                              f"on {self.device}")
         idx, out = select_heavy(weights, n_keep, n_recent, length=n, stream=stream)

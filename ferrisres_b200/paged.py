@@ -23,7 +23,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-from ._lib import OOMError, ShapeError, call
+from ._lib import OOMError, ShapeError, UnsupportedError, call
 from .gpu import _call_stream, _dptr, _stream_ptr, get_context
 from .kv import _index_list, _row_stride, _tree_args, select_heavy
 
@@ -355,6 +355,12 @@ class PagedKv3Cache:
             a[i, :len(t)] = t
         return torch.from_numpy(a).to(self.device), stride
 
+    @staticmethod
+    def _not_captured():
+        if torch.cuda.is_current_stream_capturing():
+            raise UnsupportedError("block tables are uploaded per call: not while a stream is "
+                                   "being captured")
+
     def _upload(self, layer: int, rids, *rows):
         """The block tables and further int32 rows [len(rids)] in one copy to the device:
         (tables, table stride, *rows)."""
@@ -432,6 +438,7 @@ class PagedKv3Cache:
                                  "fp32 [requests, n_pos, kv_heads, 2] on the cache's device")
         if n_pos == 0 or not rids:
             return
+        self._not_captured()
         copies = []
         starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
         self._copy_pages(copies, stream)
@@ -467,6 +474,7 @@ class PagedKv3Cache:
         if not rids:
             return out
         lens = [self.seq_len(r, layer) for r in rids]
+        self._not_captured()
         if min(lens) < q.shape[1]:
             raise ShapeError(f"{q.shape[1]} drafts in a request of {min(lens)} positions")
         tables, stride, lens_dev = self._upload(layer, rids, lens)
@@ -501,6 +509,7 @@ class PagedKv3Cache:
                                  f"and a request of {length}")
         if not rids:
             return
+        self._not_captured()
         # private copies of the shared pages that the call writes
         alloc = self.manager.allocator
         tabs = [self._state(r).layer_table(layer).table() for r in rids]
@@ -540,6 +549,7 @@ class PagedKv3Cache:
         lens = [self.seq_len(r, layer) for r in rids]
         longest = max(lens, default=0)
         _row_stride(weights, (len(rids), self.kv_heads), longest, "weights", self.device)
+        self._not_captured()
         lens_dev = torch.tensor(lens, dtype=torch.int32).to(self.device)
         idx, out = select_heavy(weights, n_keep, n_recent, length=longest, seq_lens=lens_dev,
                                 stream=stream)

@@ -329,6 +329,8 @@ def test_keep_nothing_and_evict_nothing(kv):
     none = torch.empty((2, 2, 0), dtype=torch.int32, device="cuda")
     idx, w = c.evict_heavy(torch.zeros((2, 2, 8), device="cuda"), 4, 2)  # an empty cache
     assert bool((idx == -1).all()) and bool((w == 0).all()) and len(c) == 0
+    idx, w = c.evict_heavy(torch.zeros((2, 2, 0), device="cuda"), 4, 2)
+    assert bool((idx == -1).all()) and w.shape == (2, 2, 0)
     c.append(x, x)
     before = stored(c, 0, 40)
     c.keep(none, start=33)  # rejected drafts: the cache is cut

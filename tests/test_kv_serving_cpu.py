@@ -103,5 +103,15 @@ def test_entry_points_refuse_null():
 
 
 def test_select_needs_a_gpu_tensor():
+    for bad in (torch.zeros((1, 1, 8)), [[[0.0] * 8]], None):
+        with pytest.raises(ShapeError):
+            kv.select_heavy(bad, 4)
+
+
+def test_tree_arguments_of_other_kinds():
+    q = torch.zeros((2, 3, 4, 128))
+    for mask in ([[1, 2, 4]] * 2, 7):
+        with pytest.raises(ShapeError):
+            kv._tree_args(q, mask, 2, CPU, None)
     with pytest.raises(ShapeError):
-        kv.select_heavy(torch.zeros((1, 1, 8)), 4)
+        kv._tree_args(q, None, 2, CPU, q.numpy())

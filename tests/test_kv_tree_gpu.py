@@ -422,6 +422,44 @@ def test_refusals(kv, paged):
     p.close()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_splits(kv, dtype):
+    """One kv head over 40007 positions: every CTA of the GPU takes a split."""
+    g = generator(31)
+    n, T, Hq = 40007, 5, 2
+    c = kv.Kv3Cache(1, 1, n)
+    c.append(rand(g, 1, n, 1, D), rand(g, 1, n, 1, D))
+    q = (2 * rand(g, 1, T, Hq, D)).to(dtype)
+    mask, bits = rand_mask(g, 1, T)
+    k, v = c.get_range(0, n)
+    check(c.tree_decode(q, mask)[0], exact(q[0], k[0], v[0], bits[0]), dtype, "R", n)
+    c.close()
+
+
+def test_paged_calls_refuse_a_capture(paged):
+    from ferrisres_b200._lib import UnsupportedError
+    g = generator(32)
+    p = paged.PagedKv3Cache(1, 12, 2)
+    r = p.create_request()
+    x = rand(g, 1, 70, 2, D)
+    p.append(0, [r], x, x)
+    f = p.fork_request(r)
+    q = rand(g, 2, 4, 4, D)
+    want = p.tree_decode(0, [r, f], q)
+    idx = torch.arange(40, 60, dtype=torch.int32, device="cuda")
+    w = torch.zeros((2, 2, 70), device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for refused in (lambda: p.tree_decode(0, [r, f], q), lambda: p.keep(0, [f], idx),
+                        lambda: p.evict_heavy(0, [r, f], w, 40)):
+            with pytest.raises(UnsupportedError):
+                refused()
+    assert torch.equal(p.tree_decode(0, [r, f], q), want)
+    p.ctx.check()
+    p.close()
+
+
 def test_captured_and_replayed(kv):
     g = generator(14)
     c = kv.Kv3Cache(2, 2, 600)
