@@ -23,9 +23,9 @@
 // aligns a product by the operands' exponents and drops the low bits: 2^-12 of
 // the result were lost.)  Softmax statistics, the sum terms and the merge of the
 // splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
-// With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 32
-// drafts over 8192 positions took 86 us where this takes 43 (32 q heads, bf16), and
-// 64 drafts over 8 x 32768 positions 1868 us where it takes 538.
+// With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 16
+// drafts over 32768 positions took 86 us where this takes 41 (32 q and 8 kv heads,
+// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 538.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -262,6 +262,14 @@ __device__ __forceinline__ int row_lane(int i) {
   return 32 * ((i >> 4) & 3) + 16 * (i >> 6) + (i & 15);
 }
 
+// With at most 64 rows (kDup) the row tile holds each row twice, as i and i + 64: the
+// first takes the first two records of each tile, the second the others, so that all
+// softmax warps work and each for half as long.  Their weights are 0 in the records
+// that the other takes, their sums are merged like those of the two groups.  (5 drafts
+// over 517 positions, 2 kv heads: 18.4 -> 16.4 us; 16 over 32768, 8 kv heads: 43.0 ->
+// 41.1.  Without the rows' second copies half the softmax warps have nothing to do.)
+__host__ __device__ constexpr bool twice(int rows) { return rows <= kPreRows / 2; }
+
 // The query operand of tree_tile_kernel, 32 rows a CTA, four a warp: fp16 in the
 // swizzled K-major layout, the rows' sums, factors and draft bits.  A kernel of
 // its own: every split of the positions needs the same operand, and its code,
@@ -276,13 +284,13 @@ __global__ void __launch_bounds__(256) tree_query_kernel(const __grid_constant__
   const int i0 = (blockIdx.x % (kPreRows / kQueryRows)) * kQueryRows + (threadIdx.x >> 5) * 4;
   const int lane = threadIdx.x & 31;
   uint8_t* img = p.qimg + tile * (int64_t)q_image(kTerms);
+  const int from = R0 + (twice(p.rows) ? i0 & 63 : i0);
   uint4 raw[4];
 #pragma unroll
   for (int y = 0; y < 4; ++y)
-    raw[y] = R0 + i0 + y < p.rows ? load_q_raw(p, b, kvh, R0 + i0 + y, lane)
-                                  : make_uint4(0, 0, 0, 0);
+    raw[y] = from + y < p.rows ? load_q_raw(p, b, kvh, from + y, lane) : make_uint4(0, 0, 0, 0);
   uint64_t mask = 0;
-  if (lane < 4 && R0 + i0 + lane < p.rows) mask = row_mask(p.mask, b, p.T, (R0 + i0 + lane) / p.G);
+  if (lane < 4 && from + lane < p.rows) mask = row_mask(p.mask, b, p.T, (from + lane) / p.G);
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
     const int i = i0 + y;
@@ -321,7 +329,7 @@ struct Masked {
   static constexpr bool value = kValue;
 };
 
-template <int kTerms>
+template <int kTerms, bool kDup>
 __global__ void __launch_bounds__(kPreWarps * 32, 1)
     tree_tile_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -626,7 +634,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
     const int st = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
     const uint32_t lanes = (uint32_t)(32 * quad + 16 * half) << 16;
     const int row0 = 32 * quad + 16 * half + g;
-    const bool live = 64 * half + 16 * quad < nrows;  // this warp's rows exist
+    const bool live = (kDup ? 0 : 64 * half) + 16 * quad < nrows;  // this warp's rows exist
+    const int c0 = kDup ? 2 * half : 0, c1 = kDup ? c0 + 2 : 4;    // its records of a tile
     // 32-bit slot arithmetic: the host keeps len below 2^31 - 512
     const int hoff = p.table ? 0 : (int)p.head_off, len32 = (int)len_b;
     const int P = len32 - p.T;  // prefix length; negative: the first drafts do not exist
@@ -648,9 +657,9 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       const uint32_t ts = tS + 128 * st + lanes;
       const float* fac = reinterpret_cast<const float*>(smem + kPreOffFac + (j & 3) * kFacBytes);
       uint32_t sv[16];
-      tc::tmem_ld_16x256b_x4(ts, sv);
+      tc::tmem_ld_16x256b_x4(ts + 32 * c0, sv);
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = c0; c < c1; ++c) {
         // 32 positions (a record); x[k][i]: row i, positions 8k + 2r, + 1
         const float4* f4 = reinterpret_cast<const float4*>(fac) + (16 * c + r) * 2;
         const float eb = (float)(15 - reinterpret_cast<const int*>(fac + 64 * 8)[c]);
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             x[k][i] = fma2(ks, mul2(s2, qfac[i]), fma2(kc, qsum[i], negM[i]));
           }
         }
-        if (c < 3) tc::tmem_ld_16x256b_x4(ts + 32 * (c + 1), sv);  // the next record's scores
+        if (c + 1 < c1) tc::tmem_ld_16x256b_x4(ts + 32 * (c + 1), sv);  // the next record's scores
         float bound[2] = {eb, eb}, m[2];
         if (kMasked) {
           // position 8k + 2r + o of the record is slot k + 4 (r / 2) + 8 (r % 2) + 16 o
@@ -731,7 +740,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             tc::tmem_wait_ld();
             tc::tmem_wait_st();
 #pragma unroll 1
-            for (int k = 0; k < kTerms * c; ++k) {  // P columns of this tile
+            for (int k = kTerms * c0; k < kTerms * c; ++k) {  // P columns of this tile
               uint32_t t[8];
               tc::tmem_ld_16x256b_x2(ts + 16 * k, t);
               tc::tmem_wait_ld();
@@ -789,6 +798,12 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
         tc::tmem_st_16x128b_x4(ts + 16 * kTerms * c, pw);
         if (kTerms == 2) tc::tmem_st_16x128b_x4(ts + 32 * c + 16, pl);
       }
+      if (kDup) {  // nothing of the records that the row's other copy takes
+        const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 2 * kTerms; ++k)
+          tc::tmem_st_16x128b_x4(ts + 16 * (kTerms * (2 - c0) + k), zero);
+      }
       tc::tmem_wait_st();
     };
     for (int j = st; j < n; j += 2) {
@@ -833,7 +848,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
     const int myrow = 32 * quad + lane;  // here a warp takes 32 rows and half the dims
     if (16 * quad < nrows) {
       const float* mine = stats + (st * kPreRows + myrow) * 3;
-      const float Mx = fmaxf(stats[myrow * 3], stats[(kPreRows + myrow) * 3]);
+      float Mx = fmaxf(stats[myrow * 3], stats[(kPreRows + myrow) * 3]);
+      if (kDup) Mx = fmaxf(Mx, __shfl_xor_sync(0xffffffffu, Mx, 16));
       const bool some = st < n && mine[0] != -INFINITY;
       const float f = some ? exp2f(mine[0] - Mx) : 0.0f, vterm = mine[2];
       float* arow = reinterpret_cast<float*>(smem) + st * kMergeArea + myrow * kMergeStride;
@@ -862,18 +878,25 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
     // partial records, one warp a row
     for (int i = warp; i < nrows; i += 16) {
       const int at = row_lane(i);
-      const float* t0 = stats + at * 3;
-      const float* t1 = t0 + kPreRows * 3;
-      const float mx = fmaxf(t0[0], t1[0]);
-      const float a0 = t0[0] == -INFINITY ? 0.0f : exp2f(t0[0] - mx) * t0[1];
-      const float a1 = t1[0] == -INFINITY ? 0.0f : exp2f(t1[0] - mx) * t1[1];
+      const int last = at + (kDup ? 16 : 0);  // row_lane(i + 64): its other copy
+      float mx = -INFINITY, l = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int y = at; y <= last; y += 16)
+        mx = fmaxf(mx, fmaxf(stats[y * 3], stats[(kPreRows + y) * 3]));
+      for (int y = at; y <= last; y += 16)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float* t = stats + (x * kPreRows + y) * 3;
+          if (t[0] != -INFINITY) l += exp2f(t[0] - mx) * t[1];
+          const float4 w =
+              reinterpret_cast<const float4*>(smem)[(x * kMergeArea + y * kMergeStride) / 4 + lane];
+          v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+        }
       float* pp = part + (int64_t)i * p.nparts * kTPart;
-      if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(mx, a0 + a1);
-      const float4* a = reinterpret_cast<const float4*>(smem) + at * (kMergeStride / 4) + lane;
-      const float4 v = a[0], w = a[kMergeArea / 4];
+      if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(mx, l);
       float2* pn = reinterpret_cast<float2*>(pp + 2) + 2 * lane;
-      pn[0] = make_float2(v.x + w.x, v.y + w.y);
-      pn[1] = make_float2(v.z + w.z, v.w + w.w);
+      pn[0] = make_float2(v.x, v.y);
+      pn[1] = make_float2(v.z, v.w);
     }
   }
   __syncthreads();
@@ -884,8 +907,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 }
 
 // Merges the split partials of a row: one CTA a row, its warps share the splits
-// (so that more loads are in flight at once: with a warp a row the decode of 32 drafts
-// over 8192 positions takes 49.5 us, so 45.5), 4 dims a lane; mode T: the output is rotated back.
+// (so that more loads are in flight at once: with a warp a row the decode of 16 drafts
+// over 32768 positions takes 49.5 us, so 45.5), 4 dims a lane; mode T: the output is rotated back.
 constexpr int kCombineWarps = 4;
 __global__ void __launch_bounds__(32 * kCombineWarps)
     tree_combine_kernel(const __grid_constant__ TreeParams p, void* __restrict__ out) {
@@ -962,8 +985,9 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
 void tree_opt_in(int device) {
   static bool done[64] = {false};
   if (device >= 0 && device < 64 && done[device]) return;
-  cudaFuncSetAttribute(tree_tile_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
-  cudaFuncSetAttribute(tree_tile_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
+  for (auto kernel : {tree_tile_kernel<1, false>, tree_tile_kernel<1, true>,
+                      tree_tile_kernel<2, false>, tree_tile_kernel<2, true>})
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPreSmem);
   if (device >= 0 && device < 64) done[device] = true;
 }
 
@@ -1066,8 +1090,10 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
     tree_query_kernel<2><<<qgrid, 256, 0, s>>>(p);
   FT_LAUNCH_CHECK();
   const dim3 grid((unsigned)p.nparts, (unsigned)(p.Hkv * p.rgroups), (unsigned)batch);
-  rc = launch_early(terms == 1 ? tree_tile_kernel<1> : tree_tile_kernel<2>, grid, kPreWarps * 32,
-                    kPreSmem, s, p);
+  const auto kernel = twice(p.rows)
+                          ? (terms == 1 ? tree_tile_kernel<1, true> : tree_tile_kernel<2, true>)
+                          : (terms == 1 ? tree_tile_kernel<1, false> : tree_tile_kernel<2, false>);
+  rc = launch_early(kernel, grid, kPreWarps * 32, kPreSmem, s, p);
   if (rc != FT_OK) return rc;
   return launch_early(tree_combine_kernel, dim3((unsigned)total), 32 * kCombineWarps, 0, s, p,
                       out_dev);
