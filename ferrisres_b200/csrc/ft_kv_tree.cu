@@ -181,6 +181,8 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // compute each position's factors; one thread issues the MMAs; two groups of eight
 // softmax warps (16 rows each) take the even and the odd tiles, each with its own S
 // and O in TMEM and its own running statistics, and merge at the end.  P overwrites S.
+// The waits of the chain S -> P -> O poll, all others suspend the warp: 64 drafts over
+// 8 x 32768 positions take 535 us, 543 when these suspend it too.
 // The K index of the first product is dims in the order 32 (Q/2) + 8r + 4 (Q%2)
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       const uint64_t qd = tc::smem_desc_sw128(sbase);
       auto qk = [&](int j) {
         const int s = j & 1;
-        ok = tc::mbar_wait_sleep(k_full + 8 * s, (j >> 1) & 1, p.err, 53);
+        ok = tc::mbar_wait(k_full + 8 * s, (j >> 1) & 1, p.err, 53);
         if (!ok) return;
         tc::tc_fence_after();
         const uint64_t kd = tc::smem_desc_sw128(sbase + off_k(kTerms) + s * kOperand);
@@ -478,9 +480,9 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       };
       auto pv = [&](int j) {
         const int s = j & 1;
-        ok = tc::mbar_wait_sleep(p_full + 8 * s, (j >> 1) & 1, p.err, 54) &&
-             (kTerms == 1 ? tc::mbar_wait_sleep(v_full + 8 * s, (j >> 1) & 1, p.err, 55)
-                          : tc::mbar_wait_sleep(v_full, j & 1, p.err, 55));
+        ok = tc::mbar_wait(p_full + 8 * s, (j >> 1) & 1, p.err, 54) &&
+             (kTerms == 1 ? tc::mbar_wait(v_full + 8 * s, (j >> 1) & 1, p.err, 55)
+                          : tc::mbar_wait(v_full, j & 1, p.err, 55));
         if (!ok) return;
         tc::tc_fence_after();
         const uint64_t vd =
@@ -807,8 +809,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       tc::tmem_wait_st();
     };
     for (int j = st; j < n; j += 2) {
-      ok = ok && tc::mbar_wait_sleep(fac_full + 8 * (j & 3), (j >> 2) & 1, p.err, 63) &&
-           tc::mbar_wait_sleep(qk_done + 8 * st, (j >> 1) & 1, p.err, 64);
+      ok = ok && tc::mbar_wait(fac_full + 8 * (j & 3), (j >> 2) & 1, p.err, 63) &&
+           tc::mbar_wait(qk_done + 8 * st, (j >> 1) & 1, p.err, 64);
       if (!ok) break;
       tc::tc_fence_after();
       if (live) {
