@@ -25,7 +25,7 @@
 // splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
 // With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 16
 // drafts over 32768 positions took 86 us where this takes 41 (32 q and 8 kv heads,
-// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 538.
+// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 531.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -995,7 +995,7 @@ void tree_opt_in(int device) {
 
 // Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost, which
 // is about three tiles' time: counted as 1 or 6 of them, 64 drafts over 8 x 32768
-// positions take 547 or 556 us, as 3 they take 544).  Paged sequences differ in length,
+// positions take 547 or 556 us, as 3 they take 544, all measured in one run).  Paged sequences differ in length,
 // which only the device knows: there the splits are made small enough for three waves,
 // down to eight tiles, so that CTAs of short sequences make room.  64 drafts over 8
 // sequences of 500 to 11469 positions: 163 us, 235 with splits for equal lengths, 182
