@@ -127,7 +127,7 @@ SIGNATURES = {
     "ft_kvp_flash_decode": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, C.c_float, _p, _p],
     "ft_kvp_flash_decode_weights": [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, C.c_float, _p, _p,
                                     _i64, _p],
-    "ft_kvp_tree_decode": [_p, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i, _i64, _p, C.c_float,
+    "ft_kvp_tree_decode": [_p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, C.c_float,
                            _p, _p],
     "ft_kvp_keep": [_p, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p],
 }

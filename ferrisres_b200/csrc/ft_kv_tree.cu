@@ -29,6 +29,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "ft_kv3.cuh"
 #include "ft_tc.cuh"
 
@@ -993,24 +995,32 @@ void tree_opt_in(int device) {
   if (device >= 0 && device < 64) done[device] = true;
 }
 
-// Tiles per split: fewest waves of `resident` CTAs x (tiles + a CTA's own cost, which
-// is about three tiles' time: counted as 1 or 6 of them, 64 drafts over 8 x 32768
-// positions take 547 or 556 us, as 3 they take 544, all measured in one run).  Paged sequences differ in length,
-// which only the device knows: there the splits are made small enough for three waves,
-// down to eight tiles, so that CTAs of short sequences make room.  64 drafts over 8
-// sequences of 500 to 11469 positions: 163 us, 235 with splits for equal lengths, 182
-// with two waves; down to four tiles, 24 drafts over 6 sequences of 2006 to 8191
-// positions take 61 us in the tile kernel where they take 55.
+// Tiles per split, at most `most`: fewest waves of `resident` CTAs x (tiles + a CTA's
+// own cost, which is about three tiles' time: counted as 1 or 6 of them, 64 drafts over
+// 8 x 32768 positions took 547 or 556 us, as 3 they took 544, all measured in one run).
+// `rows` row tiles a sequence; `all` tiles of the batch's sequences together, of which
+// the longest has ntiles.  Unequal sequences: CTAs that would start behind a sequence's
+// end return at once and are not counted (each sequence's last split is taken as half
+// full), and where more CTAs work than are resident the time is their work evenly
+// shared and a quarter of a split.  24 drafts over 6 sequences of 2006 to 8191
+// positions, 4 kv heads: 69 us, 77 with splits for equal lengths; 64 drafts over 8
+// sequences of 500 to 11469, 8 kv heads: 162 and 235 (half a split: 171, an eighth: 181);
+// over 24 of 200 to 29352: 429 and 431 (443, 417).
 constexpr int64_t kPreOverhead = 3;
-constexpr int64_t kFineTiles = 8;
-int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t overhead,
-                    bool ragged) {
-  int64_t best_cost = INT64_MAX, best = ntiles;
-  for (int64_t sp = 1; sp <= 256 && sp <= ntiles; ++sp) {
-    const int64_t per = ceil_div(ntiles, sp), ctas = units * ceil_div(ntiles, per);
-    if (ragged && per > kFineTiles && ctas < 3 * resident && sp < 256 && sp < ntiles) continue;
-    const int64_t waves = ceil_div(ctas, resident);
-    const int64_t cost = waves * (per + overhead);
+constexpr int64_t kTailParts = 4;  // of a split
+constexpr int64_t kTermTiles = 8;  // fp32 queries: most tiles of a split
+int64_t split_tiles(int64_t batch, int64_t rows, int64_t ntiles, int64_t all, int64_t resident,
+                    int64_t most) {
+  int64_t best_cost = INT64_MAX, best = most < ntiles ? most : ntiles;
+  for (int64_t sp = ceil_div(ntiles, best); sp <= 256 && sp <= ntiles; ++sp) {
+    const int64_t per = ceil_div(ntiles, sp);
+    const int64_t one = per + kPreOverhead;
+    const bool equal = all == batch * ntiles;
+    const int64_t splits = equal ? batch * ceil_div(ntiles, per)
+                                 : ceil_div(2 * all + batch * (per - 1), 2 * per);
+    const int64_t cost = equal || rows * splits <= resident
+                             ? kTailParts * ceil_div(rows * splits, resident) * one
+                             : kTailParts * rows * (all + splits * kPreOverhead) / resident + one;
     if (cost < best_cost) {
       best_cost = cost;
       best = per;
@@ -1018,8 +1028,6 @@ int64_t split_tiles(int64_t units, int64_t ntiles, int64_t resident, int64_t ove
   }
   return best;
 }
-
-constexpr int64_t kTermTiles = 8;  // fp32 queries: most tiles of a split
 
 // Launch that may start before the kernel in front of it has ended; the kernel
 // waits for that one itself (griddepcontrol).
@@ -1041,7 +1049,8 @@ int launch_early(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_
 }
 
 template <class Cache>
-int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_draft,
+int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t total_len,
+                int64_t n_draft,
                 const void* q_dev, int q_is_bf16, int64_t q_heads, const uint64_t* mask_dev,
                 float scale, void* out_dev, cudaStream_t s) {
   FT_CHECK(q_heads > 0 && q_heads % c->kv_heads == 0, FT_ERR_SHAPE,
@@ -1075,8 +1084,11 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t n_dr
   FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
            "decode grid too large");
   const int64_t tiles = batch * p.Hkv * p.rgroups;
-  p.tiles_per = split_tiles(tiles, ntiles, ctx->num_sms, kPreOverhead, p.table != nullptr);
-  if (terms == 2 && p.tiles_per > kTermTiles) p.tiles_per = kTermTiles;
+  int64_t all = batch * ntiles;
+  if (total_len > 0 && total_len < batch * p.len)
+    all = std::min(all, ceil_div(total_len + batch * (kTWarps * kBlk / 2), kTWarps * kBlk));
+  p.tiles_per = split_tiles(batch, p.Hkv * p.rgroups, ntiles, all, ctx->num_sms,
+                            terms == 2 ? kTermTiles : INT64_MAX);
   p.nparts = (int)ceil_div(ntiles, p.tiles_per);
   const size_t images = (size_t)tiles * q_image(terms);
   FT_CHECK(total < INT32_MAX && tiles < INT32_MAX / 4, FT_ERR_UNSUPPORTED, "too many query rows");
@@ -1122,17 +1134,18 @@ int ft_kv3_tree_decode(ft_ctx* ctx, ft_kv3* c, int64_t n_draft, const void* q_de
   p.head_off = c->head % kBlk;
   p.head_blk = c->head / kBlk;
   p.len = c->len;
-  return launch_tree(ctx, c, p, c->batch, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
+  return launch_tree(ctx, c, p, c->batch, 0, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
                      out_dev, static_cast<cudaStream_t>(stream));
 }
 
 int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tables_dev,
                        int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
-                       int64_t n_draft, const void* q_dev, int q_is_bf16, int64_t q_heads,
-                       const uint64_t* mask_dev, float scale, void* out_dev, void* stream) {
+                       int64_t total_len, int64_t n_draft, const void* q_dev, int q_is_bf16,
+                       int64_t q_heads, const uint64_t* mask_dev, float scale, void* out_dev,
+                       void* stream) {
   FT_CHECK(ctx && c && tables_dev && seq_lens_dev && q_dev && out_dev, FT_ERR_SHAPE,
            "null argument");
-  FT_CHECK(batch > 0 && max_seq_len > 0 && table_stride > 0 &&
+  FT_CHECK(batch > 0 && max_seq_len > 0 && total_len >= 0 && table_stride > 0 &&
                max_seq_len <= table_stride * kBlk,
            FT_ERR_SHAPE, "bad decode shape (batch %lld, max_seq_len %lld, table stride %lld)",
            (long long)batch, (long long)max_seq_len, (long long)table_stride);
@@ -1146,7 +1159,7 @@ int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* c, int64_t batch, const int32_t* tab
   p.seq_lens = seq_lens_dev;
   p.tstride = table_stride;
   p.n_pages = c->n_pages;
-  return launch_tree(ctx, c, p, batch, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
+  return launch_tree(ctx, c, p, batch, total_len, n_draft, q_dev, q_is_bf16, q_heads, mask_dev, scale,
                      out_dev, static_cast<cudaStream_t>(stream));
 }
 

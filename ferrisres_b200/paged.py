@@ -479,7 +479,7 @@ class PagedKv3Cache:
             raise ShapeError(f"{q.shape[1]} drafts in a request of {min(lens)} positions")
         tables, stride, lens_dev = self._upload(layer, rids, lens)
         call("ft_kvp_tree_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
-             _dptr(lens_dev), max(lens), int(q.shape[1]), _dptr(q),
+             _dptr(lens_dev), max(lens), sum(lens), int(q.shape[1]), _dptr(q),
              int(q.dtype == torch.bfloat16), int(q.shape[2]), None if mask is None else _dptr(mask),
              float(scale), _dptr(out),
              _call_stream(self.device, stream, tables, lens_dev, q, out, mask))

@@ -486,11 +486,14 @@ int ft_kvp_flash_decode_weights(ft_ctx* ctx, ft_kvp* pool, int64_t batch,
                                 const float* q_dev, int64_t q_heads, float scale, float* out_dev,
                                 float* weights_dev, int64_t weights_stride, void* stream);
 /* seq_lens[b] counts the drafts; a sequence shorter than n_draft has only the
- * last seq_lens[b] of them (an empty one gives 0 everywhere). */
+ * last seq_lens[b] of them (an empty one gives 0 everywhere).  total_len, the sum
+ * of the lengths as far as the host knows it (0: batch * max_seq_len), only guides
+ * how the positions are split. */
 int ft_kvp_tree_decode(ft_ctx* ctx, ft_kvp* pool, int64_t batch, const int32_t* tables_dev,
                        int64_t table_stride, const int32_t* seq_lens_dev, int64_t max_seq_len,
-                       int64_t n_draft, const void* q_dev, int q_is_bf16, int64_t q_heads,
-                       const uint64_t* mask_dev, float scale, void* out_dev, void* stream);
+                       int64_t total_len, int64_t n_draft, const void* q_dev, int q_is_bf16,
+                       int64_t q_heads, const uint64_t* mask_dev, float scale, void* out_dev,
+                       void* stream);
 /* Sequence b keeps count_dev[b] <= max_count positions from start_dev[b] on
  * (int32 on the device; start + count <= seq_lens[b], otherwise the sequence is
  * skipped and reported).  The pages from start on must belong to that sequence

@@ -106,6 +106,6 @@ extern "C" {
     pub fn ft_kvp_export_range(ctx: *mut ft_ctx, pool: *const ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, start: i64, end: i64, k_codes_dev: *mut u8, k_minmax_dev: *mut f32, v_codes_dev: *mut u8, v_minmax_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_flash_decode(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_flash_decode_weights(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, q_dev: *const f32, q_heads: i64, scale: f32, out_dev: *mut f32, weights_dev: *mut f32, weights_stride: i64, stream: *mut c_void) -> c_int;
-    pub fn ft_kvp_tree_decode(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, n_draft: i64, q_dev: *const c_void, q_is_bf16: c_int, q_heads: i64, mask_dev: *const u64, scale: f32, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ft_kvp_tree_decode(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, max_seq_len: i64, total_len: i64, n_draft: i64, q_dev: *const c_void, q_is_bf16: c_int, q_heads: i64, mask_dev: *const u64, scale: f32, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn ft_kvp_keep(ctx: *mut ft_ctx, pool: *mut ft_kvp, batch: i64, tables_dev: *const i32, table_stride: i64, seq_lens_dev: *const i32, start_dev: *const i32, count_dev: *const i32, max_count: i64, idx_dev: *const i32, idx_batch_stride: i64, idx_head_stride: i64, stream: *mut c_void) -> c_int;
 }

@@ -97,7 +97,7 @@ def test_entry_points_refuse_null():
                L.ft_kv_select_heavy(n, 1, 1, n, 1, n, 1, 1, 0, n, n, 0, n),
                L.ft_kv3_keep(n, n, 0, 1, n, 0, 0, n),
                L.ft_kvp_flash_decode_weights(n, n, 1, n, 1, n, 1, n, 1, f, n, n, 1, n),
-               L.ft_kvp_tree_decode(n, n, 1, n, 1, n, 1, 1, n, 0, 1, n, f, n, n),
+               L.ft_kvp_tree_decode(n, n, 1, n, 1, n, 1, 1, 1, n, 0, 1, n, f, n, n),
                L.ft_kvp_keep(n, n, 1, n, 1, n, n, n, 1, n, 0, 0, n)):
         assert rc == 1 and b"null" in L.ft_last_error_string()
 

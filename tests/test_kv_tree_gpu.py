@@ -343,7 +343,7 @@ def test_short_empty_and_bad_sequences(paged):
     out = torch.full_like(q, 7.0)
 
     def go(tables, lens):
-        call("ft_kvp_tree_decode", c.ctx.handle, c.handle, 3, _dptr(tables), 2, _dptr(lens), 40, T,
+        call("ft_kvp_tree_decode", c.ctx.handle, c.handle, 3, _dptr(tables), 2, _dptr(lens), 40, 0, T,
              _dptr(q), 0, 2, None, C.c_float(0.0), _dptr(out), _stream_ptr())
 
     go(tables, lens)
