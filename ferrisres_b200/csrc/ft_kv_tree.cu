@@ -1003,7 +1003,7 @@ void tree_opt_in(int device) {
 // end return at once and are not counted (each sequence's last split is taken as half
 // full), and where more CTAs work than are resident the time is their work evenly
 // shared and a quarter of a split.  24 drafts over 6 sequences of 2006 to 8191
-// positions, 4 kv heads: 69 us, 77 with splits for equal lengths; 64 drafts over 8
+// positions, 4 kv heads: 66 us, 77 with splits for equal lengths; 64 drafts over 8
 // sequences of 500 to 11469, 8 kv heads: 162 and 235 (half a split: 171, an eighth: 181);
 // over 24 of 200 to 29352: 429 and 431 (443, 417).
 constexpr int64_t kPreOverhead = 3;
