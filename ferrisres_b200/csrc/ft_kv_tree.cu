@@ -15,17 +15,19 @@
 // st = (max - min)/7, so q . k is a multiple of sum(q) plus 8 st times a product
 // of fp16 matrices.  q enters as fp16 hi + lo of q * 2^sh (sh puts the row's
 // absmax in [2^14, 2^15)): hi alone holds a bf16 q exactly down to 2^-29 of the
-// absmax, hi + lo hold 22 bits of an fp32 q.  p . v likewise: w = p st as fp16
-// (bf16 q: relative rounding 2^-12, an eighth of the output's own) or fp16 hi +
-// lo (fp32 q).  The centred form keeps the products' sums near zero, where the
-// two parts of v do not cancel; the scores of a bf16 q do without it.  (As
+// absmax, hi + lo hold 22 bits of an fp32 q or of a rotated one (mode T), which is
+// no bf16 value.  p . v likewise: w = p st as fp16 hi + lo, 22 bits.  (hi alone, 11
+// bits, took 532 us where 64 drafts over 8 x 32768 positions now take 604, but one
+// bf16 output in twenty came out a step off.)  The centred form keeps the products'
+// sums near zero, where the two parts of v do not cancel; the scores of a bf16 q do
+// without it.  (As
 // fp16 subnormals the codes would cost one operation less, but the tensor core
 // aligns a product by the operands' exponents and drops the low bits: 2^-12 of
 // the result were lost.)  Softmax statistics, the sum terms and the merge of the
 // splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
 // With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 16
-// drafts over 32768 positions took 86 us where this takes 41 (32 q and 8 kv heads,
-// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 531.
+// drafts over 32768 positions took 86 us where this takes 44 (32 q and 8 kv heads,
+// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 604.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -193,17 +195,16 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // so w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; M starts 8 below that
 // and moves only when a score passes the bound, by a power of two that the sums,
 // the P columns already written and O in TMEM are then scaled by.
-// kTerms 1: bf16 queries, q and w as one fp16 each; 2: fp32 queries, hi and lo of
-// both, twice the products; P's hi and lo of a record take the columns of its
-// scores.  O is summed in TMEM over the whole split, where the tensor core
+// kTerms 1: bf16 queries (mode R), q as one fp16; 2: fp32 or rotated queries, hi and lo.
+// P's hi and lo of a record take the columns of its scores.  O is summed in TMEM over the whole split, where the tensor core
 // truncates, 2^-25 of O a product on average: 2^-14 after 2048 products, against
 // 2^-9 of the bf16 output; for fp32 a split has at most 8 tiles (64 products a
-// group: 2^-19 at most, 1e-6 as measured), the splits being merged in fp32.
+// group: 2^-19 expected, 1e-6 as measured), the splits being merged in fp32.
 constexpr int kPreRows = 128;
 constexpr int kPreWarps = 28;
 constexpr int kPreRaw = 3;
 constexpr int kOperand = 128 * 128 * 2;  // bytes of Q, K' or V' (two swizzled panels)
-// bf16 queries: Q, two K', two V'; fp32 queries: Q hi and lo, two K', one V'
+// one term of q: Q, two K', two V'; two terms: Q hi and lo, two K', one V'
 __host__ __device__ constexpr int off_k(int terms) { return terms * kOperand; }
 __host__ __device__ constexpr int off_v(int terms) { return (terms + 2) * kOperand; }
 constexpr int kPreOffRaw = 5 * kOperand;
@@ -493,11 +494,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t at = (uint64_t)((k >> 2) * (kOperand / 2) + (k & 3) * 32) >> 4;
-            // P of 16 positions: 8 columns; with two terms a record's hi and lo lie in the
-            // 32 columns of its scores
-            const uint32_t pc = tS + 128 * s + (kTerms == 1 ? 8 * k : 32 * (k >> 1) + 8 * (k & 1));
+            // P of 16 positions: 8 columns; a record's hi and lo lie in the 32 columns of
+            // its scores
+            const uint32_t pc = tS + 128 * s + 32 * (k >> 1) + 8 * (k & 1);
             tc::mma_f16_ts(tO + 128 * s, pc, vd + at, idesc, j >= 2 || k > 0);
-            if (kTerms == 2) tc::mma_f16_ts(tO + 128 * s, pc + 16, vd + at, idesc, 1);
+            tc::mma_f16_ts(tO + 128 * s, pc + 16, vd + at, idesc, 1);
           }
           tc::mma_commit(pv_done + 8 * s);
         }
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             tc::tmem_wait_ld();
             tc::tmem_wait_st();
 #pragma unroll 1
-            for (int k = kTerms * c0; k < kTerms * c; ++k) {  // P columns of this tile
+            for (int k = 2 * c0; k < 2 * c; ++k) {  // P columns of this tile
               uint32_t t[8];
               tc::tmem_ld_16x256b_x2(ts + 16 * k, t);
               tc::tmem_wait_ld();
@@ -793,20 +794,17 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
               vm2[i] = add2(vm2[i], pair(vt.x, vt.y));
             }
             pw[2 * k + i] = pack_half2(wt.x, wt.y);
-            if (kTerms == 2) {
-              const float2 hi = unpack_half2(pw[2 * k + i]);
-              pl[2 * k + i] = pack_half2(wt.x - hi.x, wt.y - hi.y);
-            }
+            const float2 hi = unpack_half2(pw[2 * k + i]);
+            pl[2 * k + i] = pack_half2(wt.x - hi.x, wt.y - hi.y);
           }
         }
-        tc::tmem_st_16x128b_x4(ts + 16 * kTerms * c, pw);
-        if (kTerms == 2) tc::tmem_st_16x128b_x4(ts + 32 * c + 16, pl);
+        tc::tmem_st_16x128b_x4(ts + 32 * c, pw);
+        tc::tmem_st_16x128b_x4(ts + 32 * c + 16, pl);
       }
       if (kDup) {  // nothing of the records that the row's other copy takes
         const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 2 * kTerms; ++k)
-          tc::tmem_st_16x128b_x4(ts + 16 * (kTerms * (2 - c0) + k), zero);
+        for (int k = 0; k < 4; ++k) tc::tmem_st_16x128b_x4(ts + 32 * (2 - c0) + 16 * k, zero);
       }
       tc::tmem_wait_st();
     };
@@ -1079,7 +1077,7 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t tota
   const int64_t total = batch * p.Hkv * p.rows;
   const int64_t ntiles = ceil_div(p.nlb, (int64_t)kTWarps);
   tree_opt_in(ctx->device);
-  const int terms = q_is_bf16 ? 1 : 2;
+  const int terms = q_is_bf16 && !p.signs ? 1 : 2;  // a rotated bf16 q is no bf16 value
   p.rgroups = (p.rows + kPreRows - 1) / kPreRows;
   FT_CHECK(p.Hkv * p.rgroups <= 65535 && batch <= 65535, FT_ERR_UNSUPPORTED,
            "decode grid too large");
@@ -1088,7 +1086,7 @@ int launch_tree(ft_ctx* ctx, Cache* c, TreeParams p, int64_t batch, int64_t tota
   if (total_len > 0 && total_len < batch * p.len)
     all = std::min(all, ceil_div(total_len + batch * (kTWarps * kBlk / 2), kTWarps * kBlk));
   p.tiles_per = split_tiles(batch, p.Hkv * p.rgroups, ntiles, all, ctx->num_sms,
-                            terms == 2 ? kTermTiles : INT64_MAX);
+                            q_is_bf16 ? INT64_MAX : kTermTiles);
   p.nparts = (int)ceil_div(ntiles, p.tiles_per);
   const size_t images = (size_t)tiles * q_image(terms);
   FT_CHECK(total < INT32_MAX && tiles < INT32_MAX / 4, FT_ERR_UNSUPPORTED, "too many query rows");

@@ -1,0 +1,71 @@
+"""Where the tree decode's 16-bit operands could lose bits or overflow: results against attention in 64
+bits over the stored values (``exact`` and its X, V are those of test_kv_tree_gpu).
+
+Bounds, each an upper limit of the roundings that the formula needs:
+  scores: K vectors here are a level plus little noise, so that a score is level * sum(q) (fp32: qsum, the
+    factor and the product, 4 roundings of 2^-24 and the sum of 128 terms, 2^-22 together) plus a small
+    product of codes: below 2^-20 * X.  p is off by twice that, X <= 40 in these tests where nothing else
+    is said: 2^-19 * 40 / 4 in the 2-norm (rounding errors of both signs) = 2e-5 at most; where X <= 20, 1e-5.
+  weights: fp16 hi + lo of p (max - min)/7: relative 2^-22, absolute 2^-25 of a largest of at least 2^5.
+  bf16 output: half a step, 2^(floor(log2 |out|) - 8), plus the fp32 error before it.
+"""
+import pytest
+import torch
+
+from test_kv_tree_gpu import D, causal_bits, exact, generator, kv, paged, rand  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def ring(kv, k, v, mode="R", seed=3):
+    c = kv.Kv3Cache(k.shape[0], k.shape[2], k.shape[1], mode=mode, seed=seed)
+    c.append(k, v)
+    return c
+
+
+def near(got, ref, rel):
+    out = ref[0]
+    assert bool(torch.isfinite(got.float()).all())
+    err = float((got.double() - out).norm() / out.norm())
+    assert err <= rel, err
+
+
+def half_step(x):
+    """Half a step of bf16 at |x| (x in 64 bits)."""
+    return torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(1e-30))) - 8)
+
+
+# ------------------------------------------------------------ bf16 queries --
+@pytest.mark.parametrize("n", [64, 66, 200, 1500])
+def test_bf16_output_is_rounded_once(kv, n):
+    """bf16 queries: the output is the fp32 result rounded once.  Small scores (X about 1.3) make the fp32
+    error small: 2 * 3 X 2^-20 of the scores, 2^-18 and 2^-21 of the exponentials and weights, sums of
+    (n / 32 + 16) 2^-24 of 3 V.  An output may differ from the rounded exact result only where that lies
+    within the error of a rounding border, which of m outputs happens to sum(error / half step) at most."""
+    g = generator(n)
+    T, Hq, H = 64, 8, 2
+    c = ring(kv, rand(g, 1, n, H, D), rand(g, 1, n, H, D))
+    q = (0.05 * rand(g, 1, T, Hq, D)).bfloat16()
+    bits = torch.eye(T, dtype=torch.bool, device="cuda")  # a draft sees the prefix and itself
+    mask = torch.ones(T, dtype=torch.int64, device="cuda") << torch.arange(T, device="cuda")
+    got = c.tree_decode(q, mask)[0].double()
+    k, v = c.get_range(0, n)
+    out, X, V = exact(q[0], k[0], v[0], bits)
+    tol = V * (6 * X * 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -21 + 3 * (n / 32 + 16) * 2.0 ** -24)
+    half = half_step(out.abs() + tol)
+    assert bool(((got - out).abs() <= half + tol).all())
+    differ = int((got != out.float().bfloat16().double()).sum())
+    expected = float((tol / half_step(out)).clamp_max(1).sum())
+    assert differ <= expected + 6 * expected ** 0.5, (differ, expected, got.numel())
+    c.close()
+
+
+@pytest.mark.parametrize("n,T,Hq,H", [(5, 5, 8, 2), (64, 64, 8, 8), (128, 21, 10, 2), (100, 64, 16, 1)])
+def test_bf16_queries_in_mode_t(kv, n, T, Hq, H):
+    """The rotated query is no bf16 value: it is taken with the bits of an fp32 one.  The same q as fp32
+    gives the same result before the one rounding (one tile of positions: one split either way)."""
+    g = generator(n + T)
+    c = ring(kv, rand(g, 2, n, H, D), rand(g, 2, n, H, D), mode="T")
+    q = (2 * rand(g, 2, T, Hq, D)).bfloat16()
+    assert torch.equal(c.tree_decode(q), c.tree_decode(q.float()).bfloat16())
+    c.close()
