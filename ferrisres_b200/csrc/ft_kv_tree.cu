@@ -745,17 +745,24 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             tc::tmem_wait_ld();
             tc::tmem_wait_st();
 #pragma unroll 1
-            for (int k = 2 * c0; k < 2 * c; ++k) {  // P columns of this tile
-              uint32_t t[8];
-              tc::tmem_ld_16x256b_x2(ts + 16 * k, t);
+            for (int k = 2 * c0; k < 2 * c; ++k) {
+              // P columns of this tile, 16 positions: hi + lo, scaled in fp32 (alpha as
+              // fp16 would be 0 below 2^-25, where the weights still count) and split anew
+              const uint32_t at = ts + 32 * (k >> 1) + 8 * (k & 1);
+              uint32_t h[4], l[4];
+              tc::tmem_ld_16x256b_x1(at, h);
+              tc::tmem_ld_16x256b_x1(at + 16, l);
               tc::tmem_wait_ld();
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&t[q]),
-                                          __float2half2_rn(alpha[(q >> 1) & 1]));
-                t[q] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int q = 0; q < 4; ++q) {
+                const float2 a = unpack_half2(h[q]), b = unpack_half2(l[q]);
+                const float u = (a.x + b.x) * alpha[q >> 1], v = (a.y + b.y) * alpha[q >> 1];
+                h[q] = pack_half2(u, v);
+                const float2 hi = unpack_half2(h[q]);
+                l[q] = pack_half2(u - hi.x, v - hi.y);
               }
-              tc::tmem_st_16x256b_x2(ts + 16 * k, t);
+              tc::tmem_st_16x256b_x1(at, h);
+              tc::tmem_st_16x256b_x1(at + 16, l);
             }
             if (j >= 2) {  // O, once the product of tile j - 2 is in it
               ok = ok && tc::mbar_wait_sleep(pv_done + 8 * st, ((j >> 1) - 1) & 1, p.err, 65);

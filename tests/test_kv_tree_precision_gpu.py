@@ -69,3 +69,30 @@ def test_bf16_queries_in_mode_t(kv, n, T, Hq, H):
     q = (2 * rand(g, 2, T, Hq, D)).bfloat16()
     assert torch.equal(c.tree_decode(q), c.tree_decode(q.float()).bfloat16())
     c.close()
+
+
+# ------------------------------------------------- references of the softmax --
+def levels(g, n, H, at):
+    """K whose score is level * sum(q): at [n] in units of log2 for a q of ones, and q rows near ones."""
+    unit = 1.4426950408889634 * D ** 0.5  # log2 of a score per unit of level, sum(q) = 128
+    return (at / unit)[None, :, None, None] + 0.01 * rand(g, 1, n, H, D)
+
+
+def test_weights_that_fall_by_2_to_26_within_a_tile(kv):
+    """One record grows the reference's headroom, the next passes it by 2^18: what the records before hold
+    in 16 bits is scaled by 2^-26, and counts for 64 * 2^-18 of the result."""
+    g = generator(41)
+    n, T, H, Hq = 128, 1, 1, 80  # above 64 rows a row takes all records of a tile
+    at = torch.zeros(n, device="cuda")
+    at[32:96] = 7.3
+    at[96:] = -10.0
+    at[100] = 7.3 + 18.9
+    k = levels(g, n, H, at)
+    v = rand(g, 1, n, H, D)
+    v[:, 32:96] = rand(g, 1, 1, H, D)
+    c = ring(kv, k, v)
+    q = 1 + 0.02 * rand(g, 1, T, Hq, D)
+    kk, vv = c.get_range(0, n)
+    ref = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
+    near(c.tree_decode(q)[0], ref, 1e-5)
+    c.close()
