@@ -191,10 +191,15 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
 // 16 bytes it holds, and eight lanes of a store meet eight banks.
-// References: integer M per row with x - M <= 15 - e wherever (max - min)/7 < 2^e,
-// so w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; M starts 8 below that
-// and moves only when a score passes the bound, by a power of two that the sums,
-// the P columns already written and O in TMEM are then scaled by.
+// References: integer M per row with x - M + e <= 15 wherever (max - min)/7 < 2^e,
+// so w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; the largest x - M + e
+// starts at 7 and M moves only when one passes 15, by a power of two that the sums,
+// the P columns already written and O in TMEM are then scaled by.  So the largest w of
+// a row has at least 2^5, and a w at 2^-k of it is off by 2^-25 or 2^(k - 30) of itself,
+// whatever the largest p belongs to (a sink with values near 0) and whatever ranges
+// positions of little weight have.  A record's scores are compared with 15 minus the
+// e of its largest range first; only where one passes that does each position's own e
+// count.
 // kTerms 1: bf16 queries (mode R), q as one fp16; 2: fp32 or rotated queries, hi and lo.
 // P's hi and lo of a record take the columns of its scores.  O is summed in TMEM over the whole split, where the tensor core
 // truncates, 2^-25 of O a product on average: 2^-14 after 2048 products, against
@@ -682,29 +687,20 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
           }
         }
         if (c + 1 < c1) tc::tmem_ld_16x256b_x4(ts + 32 * (c + 1), sv);  // the next record's scores
-        float bound[2] = {eb, eb}, m[2];
         if (kMasked) {
           // position 8k + 2r + o of the record is slot k + 4 (r / 2) + 8 (r % 2) + 16 o
           const int base = ((int)(t_begin + j) * kTWarps + c) * kBlk - hoff;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint64_t mask = qmask[row0 + 8 * i];
-            int e = -85;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 f = unpair(x[k][i]);
-              const float4 vf = f4[8 * k + 1];
               const int p0 = base + k + 4 * (r >> 1) + 8 * (r & 1), p1 = p0 + 16;
               const bool s0 = p0 >= 0 && p0 < len32 && (p0 < P || ((mask >> (p0 - P)) & 1ull));
               const bool s1 = p1 >= 0 && p1 < len32 && (p1 < P || ((mask >> (p1 - P)) & 1ull));
-              if (s0) e = max(e, bound_exp(vf.x < INFINITY ? vf.x : 0.0f));
-              if (s1) e = max(e, bound_exp(vf.y < INFINITY ? vf.y : 0.0f));
               x[k][i] = pair(s0 ? f.x : -INFINITY, s1 ? f.y : -INFINITY);
             }
-            // what a row sees bounds it, not what masked places hold
-            e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-            e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-            bound[i] = (float)(15 - e);
           }
         }
         bool above = unset;
@@ -716,19 +712,30 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             const float2 f = unpair(x[k][i]);
             t[k] = fmaxf(f.x, f.y);
           }
-          m[i] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-          above |= m[i] > bound[i];
+          above |= fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) > eb;
         }
         if (__builtin_expect(__any_sync(0xffffffffu, above), 0)) {
-          // a score above its row's bound, or a row's first: new references
-          float alpha[2];
+          // a score that may be above its row's bound, or a row's first: each position's
+          // own e decides (masked places have x = -infinity)
+          float top[2] = {-INFINITY, -INFINITY}, alpha[2];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 vf = f4[8 * k + 1];
+            const float e0 = (float)bound_exp(vf.x < INFINITY ? vf.x : 0.0f);
+            const float e1 = (float)bound_exp(vf.y < INFINITY ? vf.y : 0.0f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 f = unpair(x[k][i]);
+              top[i] = fmaxf(top[i], fmaxf(f.x + e0, f.y + e1));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
-            m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 2));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
             const bool first = !((have >> i) & 1u);
-            // x - M so far; up by the whole steps that put the maximum 8 below the bound
-            float up = first || m[i] > bound[i] ? ceilf(m[i] - (bound[i] - 8.0f)) : 0.0f;
+            // x - M + e so far; up by the whole steps that put its maximum at 7 at most
+            float up = first || top[i] > 15.0f ? ceilf(top[i] - 7.0f) : 0.0f;
             // nothing seen yet, or NaN or infinite scores (the row then ends NaN)
             if (!(fabsf(up) < 1e30f)) up = 0.0f;
             else if (first) have |= 1u << i;

@@ -96,3 +96,84 @@ def test_weights_that_fall_by_2_to_26_within_a_tile(kv):
     ref = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
     near(c.tree_decode(q)[0], ref, 1e-5)
     c.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [12, 17, 22, 27, 40])
+def test_values_of_one_position_far_above_the_others(kv, power, dtype):
+    """A position whose values are 2^power times its neighbours' and whose weight is 2^-60: it takes no
+    bits from theirs."""
+    g = generator(power)
+    n, T, H, Hq = 300, 2, 2, 8
+    at = torch.zeros(n, device="cuda")
+    at[32:] = 8.0
+    at[70] = at[150] = -56.0
+    k, v = levels(g, n, H, at), rand(g, 1, n, H, D)
+    for i in (70, 150):
+        v[:, i] *= 2.0 ** power
+    c = ring(kv, k, v)
+    q = (1 + 0.02 * rand(g, 1, T, Hq, D)).to(dtype)
+    kk, vv = c.get_range(0, n)
+    ref = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
+    near(c.tree_decode(q)[0], ref, 2e-5 if dtype == torch.float32 else 0.6 * 2.0 ** -8)
+    c.close()
+
+
+@pytest.mark.parametrize("size", [0.0, 1e-4, 1e-2])
+@pytest.mark.parametrize("share", [6, 10, 14, 20])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_sink(kv, dtype, share, size):
+    """Position 0 takes all but 2^-share of the weight and has values of `size`: the others' weights keep
+    their bits."""
+    g = generator(share)
+    n, T, H, Hq = 512, 1, 2, 8
+    at = torch.zeros(n, device="cuda")
+    at[0] = share + 9
+    k, v = levels(g, n, H, at), rand(g, 1, n, H, D)
+    v[:, 0] *= size
+    c = ring(kv, k, v)
+    q = (1 + 0.02 * rand(g, 1, T, Hq, D)).to(dtype)
+    kk, vv = c.get_range(0, n)
+    ref = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
+    near(c.tree_decode(q)[0], ref, 2e-5 if dtype == torch.float32 else 0.6 * 2.0 ** -8)
+    c.close()
+
+
+@pytest.mark.parametrize("kind", ["rise", "fall", "steps", "huge", "values", "constant", "jumps", "spikes"])
+def test_references_that_move_fp32(kv, kind):
+    """fp32 queries: scores and value ranges that move by a little and by a lot, between tiles and between
+    the records of one.  p is off by twice 3 X 2^-20 at most (the scores' bound); terms add up to 2 V."""
+    g = generator(22)
+    n, T, Hq, H = 2500, 6, 8, 2
+    k, v = rand(g, 1, n, H, D), rand(g, 1, n, H, D)
+    q = 2 * rand(g, 1, T, Hq, D)
+    at = torch.arange(n, device="cuda")[None, :, None, None]
+    along = torch.nn.functional.normalize(q.mean((1, 2)), dim=-1)  # moves every row's score
+    if kind == "rise":
+        k = k + along * at * 0.03
+    elif kind == "fall":
+        k = k - along * at * 0.03
+    elif kind == "steps":
+        k = k + along * (at // 300 * 37 % 90)
+    elif kind == "huge":
+        k = k * 40
+    elif kind == "values":
+        v = v * torch.exp2(torch.div(at, 128, rounding_mode="floor").float())
+    elif kind == "constant":
+        v[:, ::2] = 0.5
+        v[:, 1200:1600] = 0.0
+        k[:, 700] = 1.0
+    elif kind == "jumps":  # score and range change by up to 2^30 between records of a tile
+        k = k + along * (at // 32 * 7 % 5)
+        v = v * torch.exp2((at // 32 * 17 % 30).float())
+    else:
+        v[:, 5::97] *= 2.0 ** 20
+        k[:, 5::97] -= along * 8
+    c = ring(kv, k, v)
+    got = c.tree_decode(q)[0].double()
+    c.ctx.check()
+    kk, vv = c.get_range(0, n)
+    out, X, V = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
+    tol = V * (6 * X * 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -21 + 3 * (n / 32 + 16) * 2.0 ** -24)
+    assert bool(((got - out).abs() <= tol).all())
+    c.close()
