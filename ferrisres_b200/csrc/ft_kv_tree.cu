@@ -173,6 +173,14 @@ __device__ __forceinline__ int bound_exp(float v) {
   return min(max(e, -85), 128);
 }
 
+// e of a position's value factors: vs < 2^e and |vc| < 2^(e + 85), so that with
+// x - M + e <= 15 the weights stay below 2^15 and the terms of the sums below 2^100;
+// an infinity or NaN bounds nothing.
+__device__ __forceinline__ int value_exp(float vs, float vc) {
+  const float v = fmaxf(vs, fabsf(vc) * 0x1p-85f);
+  return bound_exp(v < INFINITY ? v : 0.0f);
+}
+
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // ---------------------------------------------------------------- tiles --
@@ -191,8 +199,9 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
 // 16 bytes it holds, and eight lanes of a store meet eight banks.
-// References: integer M per row with x - M + e <= 15 wherever (max - min)/7 < 2^e,
-// so w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; the largest x - M + e
+// References: integer M per row with x - M + e <= 15 for the e of each position
+// (value_exp), so that neither the sum terms overflow, those of constant vectors among
+// them, nor w: w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; the largest x - M + e
 // starts at 7 and M moves only when one passes 15, by a power of two that the sums,
 // the P columns already written and O in TMEM are then scaled by.  So the largest w of
 // a row has at least 2^5, and a w at 2^-k of it is off by 2^-25 or 2^(k - 30) of itself,
@@ -546,11 +555,10 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
           float* fp = fac + (col >> 1) * 8 + (col & 1);
           fp[0] = ks;
           fp[2] = fmaf(kTerms == 1 ? -8.0f : 3.5f, ks, km.x);
+          const float vc = fmaf(3.5f, vs, vm.x);
           fp[4] = vs;
-          fp[6] = fmaf(3.5f, vs, vm.x);
-          int e = bound_exp(vs < INFINITY ? vs : 0.0f);
-#pragma unroll
-          for (int x = 16; x > 0; x >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, x));
+          fp[6] = vc;
+          const int e = __reduce_max_sync(0xffffffffu, value_exp(vs, vc));
           if (lane == 0) reinterpret_cast<int*>(fac + 64 * 8)[w] = e;
         }
         __syncwarp();
@@ -721,8 +729,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float4 vf = f4[8 * k + 1];
-            const float e0 = (float)bound_exp(vf.x < INFINITY ? vf.x : 0.0f);
-            const float e1 = (float)bound_exp(vf.y < INFINITY ? vf.y : 0.0f);
+            const float e0 = (float)value_exp(vf.x, vf.z), e1 = (float)value_exp(vf.y, vf.w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float2 f = unpair(x[k][i]);

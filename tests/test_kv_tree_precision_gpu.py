@@ -139,6 +139,22 @@ def test_a_sink(kv, dtype, share, size):
     c.close()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 31, 1024])
+@pytest.mark.parametrize("value", [3.0, 1e9, 1e11, -1e20, 1e30, 1e38, 1e-20])
+def test_constant_values_of_any_size(kv, value, n, dtype):
+    """V vectors without a range (step 0): the result is the value, for all sizes that have one."""
+    g = generator(n)
+    k = rand(g, 1, n, 2, D)
+    c = ring(kv, k, torch.full_like(k, value))
+    q = rand(g, 1, 1, 4, D).to(dtype)
+    got = c.tree_decode(q).double()
+    kk, vv = c.get_range(0, n)
+    want = vv.double().mean()
+    assert float((got - want).abs().max()) <= (1e-5 if dtype == torch.float32 else 2.0 ** -8) * abs(float(want))
+    c.close()
+
+
 @pytest.mark.parametrize("kind", ["rise", "fall", "steps", "huge", "values", "constant", "jumps", "spikes"])
 def test_references_that_move_fp32(kv, kind):
     """fp32 queries: scores and value ranges that move by a little and by a lot, between tiles and between
