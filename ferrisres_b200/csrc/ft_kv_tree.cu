@@ -183,6 +183,14 @@ __device__ __forceinline__ int value_exp(float vs, float vc) {
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// v * 2^(2 h): references are even and lie up to 2^200 apart, beyond one factor's range
+__device__ __forceinline__ float scale2(float v, float half_pow) { return v * half_pow * half_pow; }
+
+// The tile kernel takes V as V * 2^-16, so that with the largest ranges (e = 112) exp2(x - M)
+// is at least 2^-107 for the heaviest position, 2^19 above the smallest normal float;
+// the combine kernel scales back.
+constexpr float kValueScale = 0x1p-16f;
+
 // ---------------------------------------------------------------- tiles --
 // S = Q K' (128 query rows x 128 positions a tile), then O += P V', on the
 // 5th-generation tensor core, K' and V' being the tile's codes as fp16.
@@ -199,12 +207,12 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
 // 16 bytes it holds, and eight lanes of a store meet eight banks.
-// References: integer M per row with x - M + e <= 15 for the e of each position
+// References: even integer M per row with x - M + e <= 15 for the e of each position
 // (value_exp), so that neither the sum terms overflow, those of constant vectors among
 // them, nor w: w = exp2(x - M)(max - min)/7 stays below 2^15 in fp16; the largest x - M + e
-// starts at 7 and M moves only when one passes 15, by a power of two that the sums,
+// starts in (5, 7] and M moves only when one passes 15, by a power of two that the sums,
 // the P columns already written and O in TMEM are then scaled by.  So the largest w of
-// a row has at least 2^5, and a w at 2^-k of it is off by 2^-25 or 2^(k - 30) of itself,
+// a row has at least 2^4, and a w at 2^-k of it is off by 2^-25 or 2^(k - 29) of itself,
 // whatever the largest p belongs to (a sink with values near 0) and whatever ranges
 // positions of little weight have.  A record's scores are compared with 15 minus the
 // e of its largest range first; only where one passes that does each position's own e
@@ -548,14 +556,14 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
           const float2 km = reinterpret_cast<const float2*>(rec + kRecKmm)[mm_index(lane)];
           const float2 vm = reinterpret_cast<const float2*>(rec + kRecVmm)[mm_index(lane)];
           const float ks = (km.y - km.x) * 0.14285714285714285f;
-          const float vs = (vm.y - vm.x) * 0.14285714285714285f;
+          const float vs = (vm.y - vm.x) * 0.14285714285714285f * kValueScale;
           const int oe = lane >> 3;
           const int col = 32 * w + 8 * (lane & 3) + 4 * ((lane >> 2) & 1) +
                           (oe == 1 ? 2 : (oe == 2 ? 1 : oe));
           float* fp = fac + (col >> 1) * 8 + (col & 1);
           fp[0] = ks;
           fp[2] = fmaf(kTerms == 1 ? -8.0f : 3.5f, ks, km.x);
-          const float vc = fmaf(3.5f, vs, vm.x);
+          const float vc = fmaf(3.5f, vs, vm.x * kValueScale);
           fp[4] = vs;
           fp[6] = vc;
           const int e = __reduce_max_sync(0xffffffffu, value_exp(vs, vc));
@@ -741,16 +749,17 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
             const bool first = !((have >> i) & 1u);
-            // x - M + e so far; up by the whole steps that put its maximum at 7 at most
-            float up = first || top[i] > 15.0f ? ceilf(top[i] - 7.0f) : 0.0f;
+            // x - M + e so far; up by the even number that puts its maximum at 7 at most
+            float up = first || top[i] > 15.0f ? 2.0f * ceilf(0.5f * top[i] - 3.5f) : 0.0f;
             // nothing seen yet, or NaN or infinite scores (the row then ends NaN)
             if (!(fabsf(up) < 1e30f)) up = 0.0f;
             else if (first) have |= 1u << i;
-            alpha[i] = first ? 1.0f : exp2f(-up);  // nothing is summed before the first
+            // half of the factor's exponent; nothing is summed before the first
+            alpha[i] = first ? 1.0f : exp2f(-0.5f * up);
             const uint64_t a2 = pair(alpha[i], alpha[i]), u2 = pair(-up, -up);
             negM[i] = add2(negM[i], u2);
-            l2[i] = mul2(l2[i], a2);
-            vm2[i] = mul2(vm2[i], a2);
+            l2[i] = mul2(mul2(l2[i], a2), a2);
+            vm2[i] = mul2(mul2(vm2[i], a2), a2);
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k][i] = add2(x[k][i], u2);
           }
@@ -770,7 +779,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 const float2 a = unpack_half2(h[q]), b = unpack_half2(l[q]);
-                const float u = (a.x + b.x) * alpha[q >> 1], v = (a.y + b.y) * alpha[q >> 1];
+                const float u = scale2(a.x + b.x, alpha[q >> 1]), v = scale2(a.y + b.y, alpha[q >> 1]);
                 h[q] = pack_half2(u, v);
                 const float2 hi = unpack_half2(h[q]);
                 l[q] = pack_half2(u - hi.x, v - hi.y);
@@ -788,7 +797,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
                 tc::tmem_wait_ld();
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                  t[q] = __float_as_uint(__uint_as_float(t[q]) * alpha[(q >> 1) & 1]);
+                  t[q] = __float_as_uint(scale2(__uint_as_float(t[q]), alpha[(q >> 1) & 1]));
                 tc::tmem_st_16x256b_x2(tO + 128 * st + lanes + 16 * k, t);
               }
             }
@@ -874,7 +883,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
       float Mx = fmaxf(stats[myrow * 3], stats[(kPreRows + myrow) * 3]);
       if (kDup) Mx = fmaxf(Mx, __shfl_xor_sync(0xffffffffu, Mx, 16));
       const bool some = st < n && mine[0] != -INFINITY;
-      const float f = some ? exp2f(mine[0] - Mx) : 0.0f, vterm = mine[2];
+      const float f = some ? exp2f(0.5f * (mine[0] - Mx)) : 0.0f, vterm = mine[2];
       float* arow = reinterpret_cast<float*>(smem) + st * kMergeArea + myrow * kMergeStride;
 #pragma unroll 1
       for (int k = 4 * half; k < 4 * half + 4; ++k) {
@@ -888,7 +897,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
             const float v = __uint_as_float(t[8 * h + (d & 1) * 4 + (d >> 1)]);
-            o[d] = some ? f * fmaf(8.0f, v, vterm) : 0.0f;
+            o[d] = some ? scale2(fmaf(8.0f, v, vterm), f) : 0.0f;
           }
           float4* dst = reinterpret_cast<float4*>(arow + 16 * k + 8 * h);
           dst[0] = make_float4(o[0], o[1], o[2], o[3]);
@@ -910,7 +919,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float* t = stats + (x * kPreRows + y) * 3;
-          if (t[0] != -INFINITY) l += exp2f(t[0] - mx) * t[1];
+          if (t[0] != -INFINITY) l += scale2(t[1], exp2f(0.5f * (t[0] - mx)));
           const float4 w =
               reinterpret_cast<const float4*>(smem)[(x * kMergeArea + y * kMergeStride) / 4 + lane];
           v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
@@ -949,13 +958,13 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
     const float2 c = reinterpret_cast<const float2*>(ps + 2)[2 * lane + 1];
     if (ml.x == -INFINITY) continue;
     const float Mn = fmaxf(M, ml.x);
-    const float f0 = exp2f(M - Mn), f = exp2f(ml.x - Mn);  // M = -inf at first: 0
+    const float f0 = exp2f(0.5f * (M - Mn)), f = exp2f(0.5f * (ml.x - Mn));  // M = -inf at first: 0
     M = Mn;
-    l = fmaf(f, ml.y, l * f0);
-    v[0] = fmaf(f, a.x, v[0] * f0);
-    v[1] = fmaf(f, a.y, v[1] * f0);
-    v[2] = fmaf(f, c.x, v[2] * f0);
-    v[3] = fmaf(f, c.y, v[3] * f0);
+    l = scale2(ml.y, f) + scale2(l, f0);
+    v[0] = scale2(a.x, f) + scale2(v[0], f0);
+    v[1] = scale2(a.y, f) + scale2(v[1], f0);
+    v[2] = scale2(c.x, f) + scale2(v[2], f0);
+    v[3] = scale2(c.y, f) + scale2(v[3], f0);
   }
   if (lane == 0) {
     sm[warp][0] = M;
@@ -972,13 +981,14 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
 #pragma unroll
   for (int w = 0; w < kCombineWarps; ++w) {
     if (sm[w][0] == -INFINITY) continue;
-    const float f = exp2f(sm[w][0] - M);
-    l = fmaf(f, sm[w][1], l);
+    const float f = exp2f(0.5f * (sm[w][0] - M));
+    l += scale2(sm[w][1], f);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = fmaf(f, sm[w][2 + 32 * k + lane], v[k]);
+    for (int k = 0; k < 4; ++k) v[k] += scale2(sm[w][2 + 32 * k + lane], f);
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : v[k] / l;  // 0: the row saw nothing
+  for (int k = 0; k < 4; ++k)  // l = 0: the row saw nothing
+    v[k] = l == 0.0f ? 0.0f : v[k] / l * (1.0f / kValueScale);
   if (p.signs) {
     warp_fwht128(v, lane);
     const float4 sg = reinterpret_cast<const float4*>(p.signs)[lane];

@@ -155,6 +155,42 @@ def test_constant_values_of_any_size(kv, value, n, dtype):
     c.close()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-25, 1e-20, 1e30, 1e34, 1e37])
+def test_value_ranges_up_to_the_largest(kv, size, dtype):
+    """V of sizes up to the largest whose range is finite, with weights that spread over 2^20."""
+    g = generator(43)
+    n, T, H, Hq = 300, 2, 1, 4
+    at = -20 * torch.rand((n,), generator=g, device="cuda")
+    k, v = levels(g, n, H, at), rand(g, 1, n, H, D) * size
+    c = ring(kv, k, v)
+    q = (1 + 0.02 * rand(g, 1, T, Hq, D)).to(dtype)
+    kk, vv = c.get_range(0, n)
+    ref = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
+    near(c.tree_decode(q)[0], ref, 2e-5 if dtype == torch.float32 else 0.6 * 2.0 ** -8)
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("flip", [False, True])
+@pytest.mark.parametrize("far", [64, 700, 3000])
+def test_constant_values_beside_very_large_ones(kv, far, flip, dtype):
+    """Half of the positions with constant values, half with a range of 1e34, equal scores: references
+    that lie 2^190 apart meet within a tile, between groups and between splits."""
+    g = generator(far)
+    n = 2 * far
+    k, v = levels(g, n, 1, torch.zeros(n, device="cuda")), torch.ones((1, n, 1, D), device="cuda")
+    v[:, :far] = rand(g, 1, far, 1, D) * 1e34
+    if flip:
+        v = v.flip(1).contiguous()
+    c = ring(kv, k, v)
+    q = (1 + 0.02 * rand(g, 1, 1, 4, D)).to(dtype)
+    kk, vv = c.get_range(0, n)
+    ref = exact(q[0], kk[0], vv[0], causal_bits(1, 1)[0])
+    near(c.tree_decode(q)[0], ref, 2e-5 if dtype == torch.float32 else 0.6 * 2.0 ** -8)
+    c.close()
+
+
 @pytest.mark.parametrize("kind", ["rise", "fall", "steps", "huge", "values", "constant", "jumps", "spikes"])
 def test_references_that_move_fp32(kv, kind):
     """fp32 queries: scores and value ranges that move by a little and by a lot, between tiles and between
