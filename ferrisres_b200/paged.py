@@ -185,6 +185,19 @@ class PrefixSharingManager:
     def remove_prefix(self, tokens) -> None:
         self._prefixes.pop(tuple(tokens), None)
 
+    def forget_blocks(self, changed: dict, freed=()) -> None:
+        """Drops the registrations that blocks no longer fit (no counterpart in the
+        reference, where a block's positions never change): those that name a block of
+        ``freed``, or one of ``changed`` (block -> its first slot that holds another
+        position now) with that slot among the prefix's tokens."""
+        def stale(n_tokens, layer_blocks):
+            return any(b in freed or j * self._bs + changed.get(b, n_tokens) < n_tokens
+                       for j, b in enumerate(layer_blocks))
+
+        for key in [k for k, blocks in self._prefixes.items()
+                    if any(stale(len(k), lb) for lb in blocks)]:
+            del self._prefixes[key]
+
 
 class PagedAttentionManager:
     """Requests over a shared block pool (:354-527)."""
@@ -490,7 +503,8 @@ class PagedKv3Cache:
         """Keeps chosen positions of each request in ``layer``: new position starts[i] + j is
         old position idx[i, ..., j] for j < counts[i] (idx [n], [requests, n] or
         [requests, kv_heads, n]; counts default n, starts 0, host integers), the rest is
-        dropped and its pages are freed.  A page that a fork shares is copied first."""
+        dropped and its pages are freed.  A page that a fork shares is copied first; a
+        registered prefix whose pages are rewritten or freed is forgotten."""
         rids = list(request_ids)
         if len(set(rids)) != len(rids):
             raise ShapeError("a request may appear once per call")
@@ -526,6 +540,15 @@ class PagedKv3Cache:
             old, t[j] = t[j], alloc.allocate()
             copies.append((old, t[j]))
             alloc.free(old)
+        prefixes = self.manager.prefix_manager()
+        if prefixes.num_prefixes():
+            # rewritten from start on, and free to be appended to from the new end on
+            changed = {}
+            for t, c, st, length in zip(tabs, counts, starts, lens):
+                for j in range(st // PAGE_POSITIONS, -(-(st + c) // PAGE_POSITIONS)):
+                    if c or st < length:
+                        changed[t[j]] = max(st - j * PAGE_POSITIONS, 0)
+            prefixes.forget_blocks(changed)
         self._copy_pages(copies, stream)
         if max(counts) > 0:
             tables, stride, *meta = self._upload(layer, rids, lens, starts, counts)
@@ -534,8 +557,12 @@ class PagedKv3Cache:
                  _call_stream(self.device, stream, tables, idx))
         for r, t, c, st, length in zip(rids, tabs, counts, starts, lens):
             need = -(-(st + c) // PAGE_POSITIONS)
-            while len(t) > need:
-                alloc.free(t.pop())
+            dropped = t[need:]
+            del t[need:]
+            for b in reversed(dropped):
+                alloc.free(b)
+            if dropped and prefixes.num_prefixes():
+                prefixes.forget_blocks({}, {b for b in dropped if alloc.ref_count(b) == 0})
             self._grow_by(layer, r, st + c - length)
 
     def evict_heavy(self, layer: int, request_ids, weights: torch.Tensor, n_keep: int,

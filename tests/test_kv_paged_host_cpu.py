@@ -1,0 +1,145 @@
+"""Host side of the paged cache's calls, without a GPU: pages, reference counts and registered
+prefixes around keep, append and eviction, and what a call on another stream waits for."""
+import types
+
+import pytest
+import torch
+
+from ferrisres_b200 import kv, paged
+from ferrisres_b200._lib import OOMError, ShapeError
+from ferrisres_b200.paged import PAGE_POSITIONS, PagedAttentionManager, PagedKv3Cache
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """make(num_pages): a cache on the CPU whose C calls are recorded, not made."""
+    seen = types.SimpleNamespace(calls=[], used=[], ordered=[])
+
+    def dptr(t):
+        seen.used.append(t)
+        return None
+
+    def call_stream(device, stream, *tensors):
+        seen.ordered.append((stream, [t for t in tensors if t is not None], len(seen.calls)))
+        return None
+
+    for m in (kv, paged):
+        monkeypatch.setattr(m, "call", lambda name, *a: seen.calls.append((name, a)))
+        monkeypatch.setattr(m, "_dptr", dptr)
+        monkeypatch.setattr(m, "_call_stream", call_stream)
+    monkeypatch.setattr(PagedKv3Cache, "_not_captured", staticmethod(lambda *a: None))
+
+    def make(num_pages, kv_heads=2, num_layers=1):
+        c = PagedKv3Cache.__new__(PagedKv3Cache)
+        c.manager = PagedAttentionManager(num_layers, num_pages, PAGE_POSITIONS, kv_heads * 128)
+        c.ctx = types.SimpleNamespace(handle=None)
+        c.device, c.kv_heads, c.mode, c.handle = torch.device("cpu"), kv_heads, "R", None
+        return c
+
+    make.seen = seen
+    return make
+
+
+def fill(c, n, layer=0):
+    r = c.create_request()
+    x = torch.zeros((1, n, c.kv_heads, 128))
+    c.append_packed(layer, [r], *packed(c, 1, n))
+    assert c.seq_len(r, layer) == n and x.shape[1] == n
+    return r
+
+
+def packed(c, batch, n):
+    codes = torch.zeros((batch, n, c.kv_heads * 48), dtype=torch.uint8)
+    mm = torch.zeros((batch, n, c.kv_heads, 2))
+    return codes, mm, codes.clone(), mm.clone()
+
+
+def idx(n, start=0):
+    return torch.arange(start, start + n, dtype=torch.int32)
+
+
+def state(c, rids):
+    """Everything that a refused call has to leave as it was."""
+    a = c.manager.allocator
+    return ([(c.block_table(r), c.seq_len(r)) for r in rids], list(a._ref), sorted(a._free))
+
+
+# ------------------------------------------------------- registered prefixes --
+def test_keep_forgets_a_prefix_whose_pages_it_rewrites(host):
+    c = host(8)
+    r = fill(c, 100)
+    pm = c.manager.prefix_manager()
+    tokens = list(range(64))
+    pm.register_prefix(tokens, [c.block_table(r)[:2]])
+    pm.register_prefix([7] * 32, [c.block_table(r)[:1]])
+    # positions from 70 on: neither prefix has any
+    c.keep(0, [r], idx(10, 80), starts=[70])
+    assert pm.has_prefix(tokens) and pm.has_prefix([7] * 32)
+    # from 40 on: the second page of the first
+    c.keep(0, [r], idx(20, 50), starts=[40])
+    assert pm.lookup_prefix(tokens) is None and pm.has_prefix([7] * 32)
+    c.keep(0, [r], idx(30, 20), starts=[0])
+    assert pm.lookup_prefix([7] * 32) is None
+
+
+def test_keep_forgets_a_prefix_whose_pages_it_frees(host):
+    c = host(8)
+    r = fill(c, 128)
+    pm = c.manager.prefix_manager()
+    pm.register_prefix(range(128), [c.block_table(r)])
+    pm.register_prefix(range(64), [c.block_table(r)[:2]])
+    c.keep(0, [r], idx(0), starts=[64])  # nothing moves, two pages go
+    assert pm.lookup_prefix(range(128)) is None and pm.has_prefix(range(64))
+    assert c.manager.num_free_blocks() == 6
+
+
+def test_a_partly_filled_page_keeps_its_prefix(host):
+    """A prefix of 40 positions: positions from 40 on may change in its second page."""
+    c = host(8)
+    r = fill(c, 60)
+    pm = c.manager.prefix_manager()
+    pm.register_prefix(range(40), [c.block_table(r)])
+    c.keep(0, [r], idx(5, 50), starts=[40])
+    assert pm.has_prefix(range(40))
+    c.keep(0, [r], idx(3, 41), starts=[39])
+    assert not pm.has_prefix(range(40))
+
+
+def test_a_prefix_beyond_the_new_end_is_forgotten(host):
+    """Positions 50 and up go: the next append writes over them in the second page."""
+    c = host(8)
+    r = fill(c, 64)
+    pm = c.manager.prefix_manager()
+    pages = c.block_table(r)
+    pm.register_prefix(range(64), [pages])
+    pm.register_prefix(range(50), [pages])
+    pm.register_prefix(range(32), [pages[:1]])
+    c.keep(0, [r], idx(0), starts=[64])  # all stay
+    assert pm.num_prefixes() == 3
+    c.keep(0, [r], idx(0), starts=[50])
+    assert pm.lookup_prefix(range(64)) is None and pm.has_prefix(range(50)) and pm.has_prefix(range(32))
+
+
+def test_keep_spares_a_prefix_that_others_hold(host):
+    c = host(8)
+    r = fill(c, 64)
+    pm = c.manager.prefix_manager()
+    pages = c.block_table(r)
+    pm.register_prefix(range(64), [pages])
+    assert pm.lookup_prefix(range(64)) == [pages]  # another user of the pages
+    c.keep(0, [r], idx(40, 10))
+    assert [n for n, _ in host.seen.calls][-2:] == ["ft_kvp_copy_pages", "ft_kvp_keep"]
+    assert not set(c.block_table(r)) & set(pages)
+    assert pm.lookup_prefix(range(64)) == [pages]
+
+
+def test_evict_forgets_a_prefix(host, monkeypatch):
+    c = host(8)
+    r = fill(c, 64)
+    pm = c.manager.prefix_manager()
+    pm.register_prefix(range(32), [c.block_table(r)[:1]])
+    monkeypatch.setattr(paged, "select_heavy", lambda w, n, *a, **k: (idx(n).expand(1, 2, n), w))
+    c.evict_heavy(0, [r], torch.zeros((1, 2, 64)), 64)  # nothing to evict
+    assert pm.has_prefix(range(32))
+    c.evict_heavy(0, [r], torch.zeros((1, 2, 64)), 40)
+    assert pm.lookup_prefix(range(32)) is None
