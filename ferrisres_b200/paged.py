@@ -18,7 +18,7 @@ The device block size is 32 positions (the reference's default is 16;
 from __future__ import annotations
 
 import ctypes as C
-from collections import OrderedDict
+from collections import Counter, OrderedDict
 
 import numpy as np
 import torch
@@ -360,6 +360,12 @@ class PagedKv3Cache:
             tab.append(alloc.allocate())
         return length
 
+    def _copies_needed(self, blocks) -> int:
+        """Pages to copy when a call writes ``blocks``, each listed once per request that
+        writes it: the last owner of a page needs no copy."""
+        return sum(min(k, self.manager.allocator.ref_count(b) - 1)
+                   for b, k in Counter(blocks).items())
+
     def _tables(self, layer: int, rids):
         tabs = [self._state(r).layer_table(layer).table() for r in rids]
         stride = max(1, max(len(t) for t in tabs))
@@ -530,8 +536,9 @@ class PagedKv3Cache:
         writes = [(t, j) for t, c, st in zip(tabs, counts, starts) if c
                   for j in range(st // PAGE_POSITIONS, -(-(st + c) // PAGE_POSITIONS))]
         shared = [(t, j) for t, j in writes if alloc.ref_count(t[j]) > 1]
-        if len(shared) > alloc.num_free():
-            raise OOMError(f"page pool exhausted: {len(shared)} shared pages to copy, "
+        need = self._copies_needed(t[j] for t, j in shared)
+        if need > alloc.num_free():
+            raise OOMError(f"page pool exhausted: {need} shared pages to copy, "
                            f"{alloc.num_free()} free")
         copies = []
         for t, j in shared:

@@ -143,3 +143,30 @@ def test_evict_forgets_a_prefix(host, monkeypatch):
     assert pm.has_prefix(range(32))
     c.evict_heavy(0, [r], torch.zeros((1, 2, 64)), 40)
     assert pm.lookup_prefix(range(32)) is None
+
+
+# ------------------------------------------------------------- free pages --
+def test_keep_needs_no_copy_for_the_last_owner(host):
+    """A request and its fork, both rewritten: half of their pages have to be copied."""
+    c = host(4)
+    a = fill(c, 64)
+    b = c.fork_request(a)
+    assert c.manager.num_free_blocks() == 2
+    c.keep(0, [a, b], idx(40, 10))
+    assert not set(c.block_table(a)) & set(c.block_table(b))
+    assert c.seq_len(a) == c.seq_len(b) == 40
+
+
+def test_keep_refuses_before_it_changes_anything(host):
+    c = host(4)
+    a = fill(c, 64)
+    b = c.fork_request(a)
+    d = fill(c, 10)
+    before = state(c, [a, b, d])
+    with pytest.raises(OOMError):
+        c.keep(0, [a, b], idx(40, 10))
+    with pytest.raises(OOMError):  # the other owner is not part of the call
+        c.keep(0, [b], idx(40, 10))
+    assert state(c, [a, b, d]) == before
+    c.keep(0, [b], idx(8, 3), counts=[8])  # one page to write, one free
+    assert c.seq_len(b) == 8
