@@ -360,6 +360,23 @@ class PagedKv3Cache:
             tab.append(alloc.allocate())
         return length
 
+    def _prepare_all(self, layer: int, rids, n_pos: int, copies: list):
+        """``_prepare`` of every request, their lengths as int32; refused before any table
+        changes when the pool does not hold the pages of all."""
+        alloc = self.manager.allocator
+        new, shared = 0, []
+        for r in rids:
+            t = self._state(r).layer_table(layer)
+            length, tab = t.num_tokens(), t.table()
+            new += max(0, -(-(length + n_pos) // PAGE_POSITIONS) - len(tab))
+            if length % PAGE_POSITIONS and alloc.ref_count(tab[length // PAGE_POSITIONS]) > 1:
+                shared.append(tab[length // PAGE_POSITIONS])
+        need = new + self._copies_needed(shared)
+        if need > alloc.num_free():
+            raise OOMError(f"page pool exhausted: {need} pages are needed, "
+                           f"{alloc.num_free()} free")
+        return np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
+
     def _copies_needed(self, blocks) -> int:
         """Pages to copy when a call writes ``blocks``, each listed once per request that
         writes it: the last owner of a page needs no copy."""
@@ -417,7 +434,7 @@ class PagedKv3Cache:
         if n_pos == 0 or not rids:
             return
         copies = []
-        starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
+        starts = self._prepare_all(layer, rids, n_pos, copies)
         if copies:
             src = np.array([c[0] for c in copies], np.int32)
             dst = np.array([c[1] for c in copies], np.int32)
@@ -459,7 +476,7 @@ class PagedKv3Cache:
             return
         self._not_captured()
         copies = []
-        starts = np.array([self._prepare(layer, r, n_pos, copies) for r in rids], np.int32)
+        starts = self._prepare_all(layer, rids, n_pos, copies)
         self._copy_pages(copies, stream)
         tables, stride, start_dev = self._upload(layer, rids, starts)
         call("ft_kvp_append_packed", self.ctx.handle, self.handle, len(rids), n_pos,

@@ -170,3 +170,29 @@ def test_keep_refuses_before_it_changes_anything(host):
     assert state(c, [a, b, d]) == before
     c.keep(0, [b], idx(8, 3), counts=[8])  # one page to write, one free
     assert c.seq_len(b) == 8
+
+
+# -------------------------------------------------------------------- append --
+def values(c, batch, n):
+    return torch.zeros((batch, n, c.kv_heads, 128)), torch.zeros((batch, n, c.kv_heads, 128))
+
+
+@pytest.mark.parametrize("how", ["append_packed"])
+def test_append_refuses_before_it_changes_anything(host, how):
+    c = host(4)
+    a = fill(c, 40)
+    b = c.fork_request(a)
+    d = c.create_request()
+    before, calls = state(c, [a, b, d]), len(host.seen.calls)
+    data = {"append": values, "append_packed": packed}[how]
+    with pytest.raises(OOMError):
+        # b: a copy of the shared page; d: two pages; two are free
+        getattr(c, how)(0, [b, d], *data(c, 2, 64))
+    with pytest.raises(ShapeError):
+        getattr(c, how)(0, [b, 99], *data(c, 2, 4))
+    assert state(c, [a, b, d]) == before and len(host.seen.calls) == calls
+    # a request and its fork: one of the two copies the page
+    getattr(c, how)(0, [a, b], *data(c, 2, 24))
+    assert c.seq_len(a) == c.seq_len(b) == 64
+    assert c.block_table(a)[0] == c.block_table(b)[0] and c.block_table(a)[1] != c.block_table(b)[1]
+    assert c.manager.num_free_blocks() == 1
