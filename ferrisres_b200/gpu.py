@@ -74,7 +74,8 @@ def _call_stream(device, stream, *tensors):
     it); the tensors then stay allocated until ``stream`` has passed this point."""
     if stream is None:
         return C.c_void_p(_raw_stream(device.index))
-    stream.wait_stream(torch.cuda.current_stream(device))
+    if stream.cuda_stream != _raw_stream(device.index):
+        stream.wait_stream(torch.cuda.current_stream(device))
     for t in tensors:
         if t is not None:
             t.record_stream(stream)

@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ._lib import ShapeError, UnsupportedError, call
-from .gpu import _call_stream, _dptr, _stream_ptr, get_context
+from .gpu import _call_stream, _dptr, get_context
 
 HEAD_DIM = 128
 REC_BYTES = HEAD_DIM * 3 // 8  # 48
@@ -200,7 +200,7 @@ class Kv3Cache:
             raise ShapeError("K and V must have the same shape and dtype")
         n = k.numel() // (self.batch * self.kv_heads * HEAD_DIM)
         call("ft_kv3_append", self.ctx.handle, self.handle, n, _dptr(k), _dptr(v),
-             int(k.dtype == torch.bfloat16), _stream_ptr(stream))
+             int(k.dtype == torch.bfloat16), _call_stream(self.device, stream, k, v))
 
     def append_packed(self, k_codes, k_minmax, v_codes, v_minmax, stream=None) -> None:
         """Positions in the reference's stored form: codes uint8 [batch, n, kv_heads*48],
@@ -216,7 +216,8 @@ class Kv3Cache:
         if tens[2].shape != tens[0].shape or tens[2].dtype != torch.uint8:
             raise ShapeError("K and V codes must match")
         call("ft_kv3_append_packed", self.ctx.handle, self.handle, n, _dptr(tens[0]),
-             _dptr(tens[1]), _dptr(tens[2]), _dptr(tens[3]), _stream_ptr(stream))
+             _dptr(tens[1]), _dptr(tens[2]), _dptr(tens[3]),
+             _call_stream(self.device, stream, *tens))
 
     # ---- read
     def get_range(self, start: int, end: int, stream=None):
@@ -228,7 +229,7 @@ class Kv3Cache:
         k = torch.empty(shape, dtype=torch.float32, device=self.device)
         v = torch.empty_like(k)
         call("ft_kv3_get_range", self.ctx.handle, self.handle, int(start), int(end), _dptr(k),
-             _dptr(v), _stream_ptr(stream))
+             _dptr(v), _call_stream(self.device, stream, k, v))
         return k, v
 
     def export_range(self, start: int, end: int, stream=None):
@@ -243,7 +244,8 @@ class Kv3Cache:
         km = kc.new_empty((self.batch, n, self.kv_heads, 2), dtype=torch.float32)
         vm = torch.empty_like(km)
         call("ft_kv3_export_range", self.ctx.handle, self.handle, int(start), int(end),
-             _dptr(kc), _dptr(km), _dptr(vc), _dptr(vm), _stream_ptr(stream))
+             _dptr(kc), _dptr(km), _dptr(vc), _dptr(vm),
+             _call_stream(self.device, stream, kc, km, vc, vm))
         return kc, km, vc, vm
 
     def flash_decode(self, q: torch.Tensor, scale: float = 0.0, out: torch.Tensor | None = None,
@@ -261,7 +263,7 @@ class Kv3Cache:
         if out is None:
             out = torch.empty_like(q)
         call("ft_flash_decode_3bit", self.ctx.handle, self.handle, _dptr(q), int(q.shape[1]),
-             float(scale), _dptr(out), _stream_ptr(stream))
+             float(scale), _dptr(out), _call_stream(self.device, stream, q, out))
         return out
 
     def _decode_weights(self, q, scale, out, stream, weights):

@@ -24,7 +24,7 @@ import numpy as np
 import torch
 
 from ._lib import OOMError, ShapeError, UnsupportedError, call
-from .gpu import _call_stream, _dptr, _stream_ptr, get_context
+from .gpu import _call_stream, _dptr, get_context
 from .kv import _index_list, _row_stride, _tree_args, select_heavy
 
 DEFAULT_BLOCK_SIZE = 16   # the reference's default (paged_attention.rs:21)
@@ -383,14 +383,6 @@ class PagedKv3Cache:
         return sum(min(k, self.manager.allocator.ref_count(b) - 1)
                    for b, k in Counter(blocks).items())
 
-    def _tables(self, layer: int, rids):
-        tabs = [self._state(r).layer_table(layer).table() for r in rids]
-        stride = max(1, max(len(t) for t in tabs))
-        a = np.zeros((len(rids), stride), np.int32)
-        for i, t in enumerate(tabs):
-            a[i, :len(t)] = t
-        return torch.from_numpy(a).to(self.device), stride
-
     @staticmethod
     def _not_captured():
         if torch.cuda.is_current_stream_capturing():
@@ -411,6 +403,9 @@ class PagedKv3Cache:
             b[i, :len(t)] = t
         d = torch.from_numpy(a).to(self.device)
         return (d[len(rows) * n:], stride, *(d[i * n:(i + 1) * n] for i in range(len(rows))))
+
+    def _tables(self, layer: int, rids):
+        return self._upload(layer, rids)
 
     def _kv_view(self, t: torch.Tensor, n_req: int) -> torch.Tensor:
         if t.device != self.device or t.dtype not in (torch.float32, torch.bfloat16):
@@ -435,27 +430,13 @@ class PagedKv3Cache:
             return
         copies = []
         starts = self._prepare_all(layer, rids, n_pos, copies)
-        if copies:
-            src = np.array([c[0] for c in copies], np.int32)
-            dst = np.array([c[1] for c in copies], np.int32)
-            call("ft_kvp_copy_pages", self.ctx.handle, self.handle, len(copies),
-                 src.ctypes.data_as(C.c_void_p), dst.ctypes.data_as(C.c_void_p),
-                 _stream_ptr(stream))
-        tables, stride = self._tables(layer, rids)
-        start_dev = torch.from_numpy(starts).to(self.device)
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        # the uploads above ran on the current stream; order the append after them
-        if stream is not None:
-            stream.wait_stream(torch.cuda.current_stream(self.device))
+        self._copy_pages(copies, stream)
+        tables, stride, start_dev = self._upload(layer, rids, starts)
         call("ft_kvp_append", self.ctx.handle, self.handle, len(rids), n_pos, _dptr(tables),
              stride, _dptr(start_dev), _dptr(k), _dptr(v), 1 if k.dtype == torch.bfloat16 else 0,
-             _stream_ptr(s))
-        tables.record_stream(s)
-        start_dev.record_stream(s)
+             _call_stream(self.device, stream, tables, start_dev, k, v))
         for r in rids:
-            self._state(r).layer_table(layer).add_tokens(n_pos)
-            if layer == 0:
-                self._state(r).add_tokens(n_pos)
+            self._grow_by(layer, r, n_pos)
 
     def append_packed(self, layer: int, request_ids, k_codes, k_minmax, v_codes, v_minmax,
                       stream=None):
@@ -627,31 +608,21 @@ class PagedKv3Cache:
         lens = np.array([self.seq_len(r, layer) for r in rids], np.int32)
         if lens.max(initial=0) == 0:
             raise ShapeError("flash decode over empty requests")
-        tables, stride = self._tables(layer, rids)
-        lens_dev = torch.from_numpy(lens).to(self.device)
         if out is None:
             out = torch.empty_like(q)
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        if stream is not None:
-            stream.wait_stream(torch.cuda.current_stream(self.device))
         if weights is not None:
             step = _row_stride(weights, (len(rids), self.kv_heads), int(lens.max()), "weights",
                                self.device)
             if out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
                 raise ShapeError("out must be like q")
-            call("ft_kvp_flash_decode_weights", self.ctx.handle, self.handle, len(rids),
-                 _dptr(tables), stride, _dptr(lens_dev), int(lens.max()), _dptr(q),
-                 int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
-                 _stream_ptr(s))
-            if stream is not None:
-                for t in (q, out, weights):
-                    t.record_stream(s)
+        tables, stride, lens_dev = self._upload(layer, rids, lens)
+        args = (self.ctx.handle, self.handle, len(rids), _dptr(tables), stride, _dptr(lens_dev),
+                int(lens.max()), _dptr(q), int(q.shape[1]), float(scale), _dptr(out))
+        s = _call_stream(self.device, stream, tables, lens_dev, q, out, weights)
+        if weights is not None:
+            call("ft_kvp_flash_decode_weights", *args, C.c_void_p(weights.data_ptr()), step, s)
         else:
-            call("ft_kvp_flash_decode", self.ctx.handle, self.handle, len(rids), _dptr(tables),
-                 stride, _dptr(lens_dev), int(lens.max()), _dptr(q), int(q.shape[1]),
-                 float(scale), _dptr(out), _stream_ptr(s))
-        tables.record_stream(s)
-        lens_dev.record_stream(s)
+            call("ft_kvp_flash_decode", *args, s)
         return out
 
     def _range_check(self, layer, rids, start, end):
@@ -669,7 +640,8 @@ class PagedKv3Cache:
         v = torch.empty_like(k)
         tables, stride = self._tables(layer, rids)
         call("ft_kvp_get_range", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
-             int(start), int(end), _dptr(k), _dptr(v), _stream_ptr(stream))
+             int(start), int(end), _dptr(k), _dptr(v),
+             _call_stream(self.device, stream, tables, k, v))
         return k, v
 
     def export_range(self, layer: int, request_ids, start: int, end: int, stream=None):
@@ -686,7 +658,7 @@ class PagedKv3Cache:
         tables, stride = self._tables(layer, rids)
         call("ft_kvp_export_range", self.ctx.handle, self.handle, len(rids), _dptr(tables), stride,
              int(start), int(end), _dptr(kc), _dptr(km), _dptr(vc), _dptr(vm),
-             _stream_ptr(stream))
+             _call_stream(self.device, stream, tables, kc, km, vc, vm))
         return kc, km, vc, vm
 
     def close(self):

@@ -177,7 +177,7 @@ def values(c, batch, n):
     return torch.zeros((batch, n, c.kv_heads, 128)), torch.zeros((batch, n, c.kv_heads, 128))
 
 
-@pytest.mark.parametrize("how", ["append_packed"])
+@pytest.mark.parametrize("how", ["append", "append_packed"])
 def test_append_refuses_before_it_changes_anything(host, how):
     c = host(4)
     a = fill(c, 40)
@@ -196,3 +196,75 @@ def test_append_refuses_before_it_changes_anything(host, how):
     assert c.seq_len(a) == c.seq_len(b) == 64
     assert c.block_table(a)[0] == c.block_table(b)[0] and c.block_table(a)[1] != c.block_table(b)[1]
     assert c.manager.num_free_blocks() == 1
+
+
+# ------------------------------------------------------------- other streams --
+def pool_calls(c):
+    r = fill(c, 70)
+    f = c.fork_request(r)
+    q = torch.zeros((1, 4, 128))
+    return {
+        "append": lambda s: c.append(0, [f], *(t[:, ::2] for t in values(c, 1, 8)), stream=s),
+        "append_packed": lambda s: c.append_packed(0, [f], *(t[:, ::2] for t in packed(c, 1, 8)), stream=s),
+        "keep": lambda s: c.keep(0, [f], idx(9, 40), starts=[33], stream=s),
+        "tree_decode": lambda s: c.tree_decode(0, [r], torch.zeros((1, 3, 4, 128)), stream=s),
+        "flash_decode": lambda s: c.flash_decode(0, [r], q, stream=s),
+        "weights": lambda s: c.flash_decode(0, [r], q, weights=torch.zeros((1, 2, 70)), stream=s),
+        "get_range": lambda s: c.get_range(0, [r], 3, 50, stream=s),
+        "export_range": lambda s: c.export_range(0, [r], 3, 50, stream=s),
+    }
+
+
+def ring(host):
+    c = kv.Kv3Cache.__new__(kv.Kv3Cache)
+    c.ctx = types.SimpleNamespace(handle=None)
+    c.device, c.batch, c.kv_heads, c.handle = torch.device("cpu"), 2, 2, None
+    return c
+
+
+def ring_calls(c):
+    x = torch.zeros((2, 8, 2, 128))
+    codes = torch.zeros((2, 8, 96), dtype=torch.uint8)
+    mm = torch.zeros((2, 8, 2, 2))
+    q = torch.zeros((2, 4, 128))
+    return {
+        "append": lambda s: c.append(x[:, ::2], x[:, 1::2], stream=s),
+        "append_packed": lambda s: c.append_packed(codes[:, ::2], mm[:, ::2], codes[:, 1::2], mm[:, 1::2], stream=s),
+        "get_range": lambda s: c.get_range(3, 50, stream=s),
+        "export_range": lambda s: c.export_range(3, 50, stream=s),
+        "flash_decode": lambda s: c.flash_decode(q, stream=s),
+        "tree_decode": lambda s: c.tree_decode(torch.zeros((2, 3, 4, 128)), stream=s),
+        "keep": lambda s: c.keep(idx(9), stream=s),
+    }
+
+
+@pytest.mark.parametrize("name", ["append", "append_packed", "keep", "tree_decode", "flash_decode", "weights",
+                                  "get_range", "export_range"])
+def test_paged_calls_are_ordered_behind_the_current_stream(host, name):
+    """Every tensor that a call hands over is ordered with, and held for, the stream that it runs on,
+    before anything is launched there."""
+    c = host(16)
+    go = pool_calls(c)[name]
+    host.seen.calls.clear(), host.seen.used.clear(), host.seen.ordered.clear()
+    side = object()
+    go(side)
+    check_ordered(host.seen, side)
+
+
+@pytest.mark.parametrize("name", ["append", "append_packed", "get_range", "export_range", "flash_decode", "tree_decode",
+                                  "keep"])
+def test_ring_calls_are_ordered_behind_the_current_stream(host, name):
+    go = ring_calls(ring(host))[name]
+    side = object()
+    go(side)
+    check_ordered(host.seen, side)
+
+
+def check_ordered(seen, side):
+    launches = [i for i, (n, _) in enumerate(seen.calls)]
+    assert launches and len(seen.ordered) >= 1
+    assert all(s is side for s, _, _ in seen.ordered)
+    assert len(seen.ordered) == len(launches)  # one for every launch
+    held = {t.untyped_storage().data_ptr() for _, ts, _ in seen.ordered for t in ts}
+    for t in seen.used:
+        assert t.numel() == 0 or t.untyped_storage().data_ptr() in held, tuple(t.shape)
