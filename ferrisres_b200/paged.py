@@ -384,8 +384,13 @@ class PagedKv3Cache:
                    for b, k in Counter(blocks).items())
 
     @staticmethod
-    def _not_captured():
-        if torch.cuda.is_current_stream_capturing():
+    def _not_captured(stream=None):
+        """Refuses a call whose current stream, or ``stream``, is being captured."""
+        captured = torch.cuda.is_current_stream_capturing()
+        if stream is not None and not captured:
+            with torch.cuda.stream(stream):
+                captured = torch.cuda.is_current_stream_capturing()
+        if captured:
             raise UnsupportedError("block tables are uploaded per call: not while a stream is "
                                    "being captured")
 
@@ -419,6 +424,7 @@ class PagedKv3Cache:
     def append(self, layer: int, request_ids, k: torch.Tensor, v: torch.Tensor, stream=None):
         """Appends n_pos positions to each request of ``request_ids`` in
         ``layer``: k, v [len(request_ids), n_pos, kv_heads, 128]."""
+        self._not_captured(stream)
         rids = list(request_ids)
         if len(set(rids)) != len(rids):
             raise ShapeError("a request may appear once per append")
@@ -442,6 +448,7 @@ class PagedKv3Cache:
                       stream=None):
         """Appends positions already in the reference's stored form: codes uint8
         [len(request_ids), n_pos, kv_heads*48], (min, max) fp32 [.., n_pos, kv_heads, 2]."""
+        self._not_captured(stream)
         rids = list(request_ids)
         if len(set(rids)) != len(rids):
             raise ShapeError("a request may appear once per append")
@@ -455,7 +462,6 @@ class PagedKv3Cache:
                                  "fp32 [requests, n_pos, kv_heads, 2] on the cache's device")
         if n_pos == 0 or not rids:
             return
-        self._not_captured()
         copies = []
         starts = self._prepare_all(layer, rids, n_pos, copies)
         self._copy_pages(copies, stream)
@@ -486,12 +492,12 @@ class PagedKv3Cache:
         """Attention of drafted tokens, the last n_draft positions of each request in
         ``layer``: q [len(request_ids), n_draft, q_heads, 128] fp32 or bf16 -> out of the
         same type (see ``Kv3Cache.tree_decode``)."""
+        self._not_captured(stream)
         rids = list(request_ids)
         q, mask, out = _tree_args(q, mask, len(rids), self.device, out)
         if not rids:
             return out
         lens = [self.seq_len(r, layer) for r in rids]
-        self._not_captured()
         if min(lens) < q.shape[1]:
             raise ShapeError(f"{q.shape[1]} drafts in a request of {min(lens)} positions")
         tables, stride, lens_dev = self._upload(layer, rids, lens)
@@ -509,6 +515,7 @@ class PagedKv3Cache:
         [requests, kv_heads, n]; counts default n, starts 0, host integers), the rest is
         dropped and its pages are freed.  A page that a fork shares is copied first; a
         registered prefix whose pages are rewritten or freed is forgotten."""
+        self._not_captured(stream)
         rids = list(request_ids)
         if len(set(rids)) != len(rids):
             raise ShapeError("a request may appear once per call")
@@ -527,7 +534,6 @@ class PagedKv3Cache:
                                  f"and a request of {length}")
         if not rids:
             return
-        self._not_captured()
         # private copies of the shared pages that the call writes
         alloc = self.manager.allocator
         tabs = [self._state(r).layer_table(layer).table() for r in rids]
@@ -575,13 +581,13 @@ class PagedKv3Cache:
         """Evicts each request down to ``n_keep`` positions per kv head by accumulated
         attention ``weights`` [len(request_ids), kv_heads, >= longest] (see
         ``Kv3Cache.evict_heavy``); shorter requests stay whole.  Returns (idx, weights)."""
+        self._not_captured(stream)
         rids = list(request_ids)
         if len(set(rids)) != len(rids):
             raise ShapeError("a request may appear once per call")
         lens = [self.seq_len(r, layer) for r in rids]
         longest = max(lens, default=0)
         _row_stride(weights, (len(rids), self.kv_heads), longest, "weights", self.device)
-        self._not_captured()
         lens_dev = torch.tensor(lens, dtype=torch.int32).to(self.device)
         idx, out = select_heavy(weights, n_keep, n_recent, length=longest, seq_lens=lens_dev,
                                 stream=stream)
@@ -600,6 +606,7 @@ class PagedKv3Cache:
         each request's positions in ``layer`` (ragged lengths).  ``weights``
         [len(request_ids), kv_heads, >= longest] fp32: each position's attention weight,
         summed over the q heads of its kv head, is added to it."""
+        self._not_captured(stream)
         rids = list(request_ids)
         if q.dim() != 3 or q.shape[0] != len(rids) or q.shape[2] != HEAD_DIM or \
                 q.dtype != torch.float32 or q.device != self.device:
@@ -633,6 +640,7 @@ class PagedKv3Cache:
 
     def get_range(self, layer: int, request_ids, start: int, end: int, stream=None):
         """Dequantised K, V [len(request_ids), end-start, kv_heads, 128] fp32."""
+        self._not_captured(stream)
         rids = list(request_ids)
         self._range_check(layer, rids, start, end)
         shape = (len(rids), end - start, self.kv_heads, HEAD_DIM)
@@ -647,6 +655,7 @@ class PagedKv3Cache:
     def export_range(self, layer: int, request_ids, start: int, end: int, stream=None):
         """The reference's stored form of positions [start, end): codes
         [n, end-start, kv_heads*48] uint8 and (min, max) [n, end-start, kv_heads, 2]."""
+        self._not_captured(stream)
         rids = list(request_ids)
         self._range_check(layer, rids, start, end)
         n = end - start

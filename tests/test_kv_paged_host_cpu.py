@@ -6,8 +6,10 @@ import pytest
 import torch
 
 from ferrisres_b200 import kv, paged
-from ferrisres_b200._lib import OOMError, ShapeError
+from ferrisres_b200._lib import OOMError, ShapeError, UnsupportedError
 from ferrisres_b200.paged import PAGE_POSITIONS, PagedAttentionManager, PagedKv3Cache
+
+NOT_CAPTURED = PagedKv3Cache._not_captured
 
 
 @pytest.fixture
@@ -268,3 +270,32 @@ def check_ordered(seen, side):
     held = {t.untyped_storage().data_ptr() for _, ts, _ in seen.ordered for t in ts}
     for t in seen.used:
         assert t.numel() == 0 or t.untyped_storage().data_ptr() in held, tuple(t.shape)
+
+
+# ----------------------------------------------------------- captured streams --
+@pytest.mark.parametrize("current,given", [(True, None), (True, False), (False, True)])
+@pytest.mark.parametrize("name", ["append", "append_packed", "keep", "tree_decode", "flash_decode", "weights",
+                                  "get_range", "export_range", "evict_heavy"])
+def test_calls_refuse_a_captured_stream(host, monkeypatch, name, current, given):
+    """The current stream or the one given is being captured: refused before anything changes or runs."""
+    c = host(16)
+    go = {**pool_calls(c), "evict_heavy": lambda s: c.evict_heavy(0, [0], torch.zeros((1, 2, 70)), 40, stream=s)}[name]
+    monkeypatch.setattr(PagedKv3Cache, "_not_captured", staticmethod(NOT_CAPTURED))
+    now = [current]
+
+    class On:
+        def __init__(self, s):
+            self.to, self.was = s, now[0]
+
+        def __enter__(self):
+            now[0] = self.to
+
+        def __exit__(self, *a):
+            now[0] = self.was
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    before, calls = state(c, [0, 1]), len(host.seen.calls)
+    with pytest.raises(UnsupportedError):
+        go(given)
+    assert state(c, [0, 1]) == before and len(host.seen.calls) == calls and now == [current]
