@@ -522,7 +522,8 @@ __global__ void __launch_bounds__(32 * kExportHeads)
   extern __shared__ __align__(16) uint8_t export_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = blockDim.x >> 5;
   const int groups = (int)((p.Hkv + heads - 1) / heads);
-  const int64_t x = blockIdx.x / groups, b = blockIdx.y, h0 = blockIdx.x % groups * (int64_t)heads;
+  const int64_t unit = blockIdx.x / groups, x = unit % nblk, b = unit / nblk;
+  const int64_t h0 = blockIdx.x % groups * (int64_t)heads;
   const int nh = p.Hkv - h0 < heads ? (int)(p.Hkv - h0) : heads;
   const int64_t off = p.table ? 0 : p.head % kBlk;
   const int64_t lb = (p.start + off) / kBlk + x;    // logical block
@@ -650,8 +651,8 @@ int launch_export(const RangeParams& p, uint8_t* k, float* kmm, uint8_t* v, floa
   const int64_t off = p.table ? 0 : p.head % kBlk;
   const int64_t nblk = (p.start + p.n + off + kBlk - 1) / kBlk - (p.start + off) / kBlk;
   const int heads = p.Hkv < kExportHeads ? (int)p.Hkv : kExportHeads;
-  const int64_t grid = nblk * ceil_div(p.Hkv, (int64_t)heads);
-  FT_CHECK(grid < INT32_MAX && p.B <= 65535, FT_ERR_UNSUPPORTED, "range too long");
+  const int64_t grid = p.B * nblk * ceil_div(p.Hkv, (int64_t)heads);
+  FT_CHECK(grid < INT32_MAX, FT_ERR_UNSUPPORTED, "range too long");
   static bool opted[64] = {false};  // once per device
   int dev = 0;
   FT_CUDA(cudaGetDevice(&dev));
@@ -660,8 +661,7 @@ int launch_export(const RangeParams& p, uint8_t* k, float* kmm, uint8_t* v, floa
                                  export_smem(kExportHeads)));
     if (dev < 64) opted[dev] = true;
   }
-  kv3_export_kernel<<<dim3((unsigned)grid, (unsigned)p.B), 32 * heads, export_smem(heads), s>>>(
-      p, nblk, k, kmm, v, vmm);
+  kv3_export_kernel<<<(unsigned)grid, 32 * heads, export_smem(heads), s>>>(p, nblk, k, kmm, v, vmm);
   FT_LAUNCH_CHECK();
   return FT_OK;
 }
