@@ -525,17 +525,18 @@ int ft_kv_select_heavy(ft_ctx* ctx, int64_t batch, int64_t kv_heads, const float
            "weight rows of %lld entries do not hold %lld positions", (long long)weights_stride,
            (long long)max_seq_len);
   const int64_t kept = max_seq_len < n_keep ? max_seq_len : n_keep;
+  FT_CHECK(!weights_out_dev || weights_out_stride >= kept, FT_ERR_SHAPE,
+           "weight rows of %lld entries do not hold %lld kept positions",
+           (long long)weights_out_stride, (long long)kept);
+  if (batch == 0) return FT_OK;
   if (weights_out_dev) {
-    FT_CHECK(weights_out_stride >= kept, FT_ERR_SHAPE,
-             "weight rows of %lld entries do not hold %lld kept positions",
-             (long long)weights_out_stride, (long long)kept);
+    // the last row is read up to its last position, not to the pitch
     const int64_t rows = batch * kv_heads;
     const uintptr_t a = (uintptr_t)weights_dev, o = (uintptr_t)weights_out_dev;
     FT_CHECK(o + (size_t)(rows * weights_out_stride) * 4 <= a ||
-                 a + (size_t)(rows * weights_stride) * 4 <= o,
+                 a + (size_t)((rows - 1) * weights_stride + max_seq_len) * 4 <= o,
              FT_ERR_SHAPE, "weights_out must not overlap weights");
   }
-  if (batch == 0) return FT_OK;
   DeviceScope scope(ctx->device);
   SelectParams p{};
   p.w = weights_dev;

@@ -29,3 +29,30 @@ def test_export_of_many_sequences():
         assert b.shape[0] == 80000 and torch.equal(b.view(40000, 2, *a.shape[1:]), a.expand(40000, *a.shape))
     c.ctx.check()
     c.close()
+
+
+def test_select_beside_other_memory():
+    """Weight rows that are a part of wider ones end before the last row's pitch does: what lies there
+    may be the output."""
+    from ferrisres_b200 import kv
+    from ferrisres_b200._lib import ShapeError, call
+    from ferrisres_b200.gpu import _stream_ptr, get_context
+    g = generator(2)
+    n, pitch, keep = 63, 128, 20
+    buf = torch.zeros(1024, device="cuda")
+    w = buf[37:37 + 2 * pitch].view(1, 2, pitch)[:, :, :n]
+    w.copy_(torch.rand((1, 2, n), generator=g, device="cuda"))
+    idx = torch.empty((1, 2, keep), dtype=torch.int32, device="cuda")
+    want_idx, want = kv.select_heavy(w.clone(), keep, 4)
+
+    def go(at):
+        call("ft_kv_select_heavy", get_context().handle, 1, 2, C.c_void_p(w.data_ptr()), pitch, None, n, keep, 4,
+             C.c_void_p(idx.data_ptr()), C.c_void_p(buf.data_ptr() + 4 * at), keep, _stream_ptr())
+
+    behind = 37 + pitch + n  # the first entry behind the last row
+    go(behind)
+    assert torch.equal(idx, want_idx)
+    assert torch.equal(buf[behind:behind + 2 * keep].view(1, 2, keep), want[:, :, :keep])
+    for at in (behind - 1, 37 - 2 * keep + 1):
+        with pytest.raises(ShapeError):
+            go(at)
