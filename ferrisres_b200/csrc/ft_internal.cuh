@@ -230,6 +230,7 @@ static __device__ __noinline__ float nonfinite_row(float y_finite, const uint8_t
 struct Workspace {
   void* ptr = nullptr;
   size_t bytes = 0;
+  bool captured = false;  // a graph may use it (the cache's workspaces)
 };
 
 }  // namespace ft

@@ -2,6 +2,7 @@
 // structures, the record layout (described in ft_kv3.cu) and the layout maps.
 #pragma once
 
+#include <algorithm>
 #include <vector>
 
 #include "ft_internal.cuh"
@@ -118,27 +119,46 @@ class DeviceScope {
   int dev_ = 0, prev_ = -1;
 };
 
-// Grows a workspace outside stream capture (a capture may only reuse it).  The
-// outgrown buffer is kept in `retired` until the cache is destroyed: a graph
-// captured earlier, or work in flight on another stream, may still use it.
-// Sizes at least double, so the kept buffers add up to less than the last one.
+// Grows a workspace outside stream capture (a capture may only reuse it).  A buffer
+// that a capture has used is kept in `retired` until the cache is destroyed, since the
+// graph still uses it, and the next one is at least twice as large, so that the kept
+// ones add up to less than the last.  Any other is freed first (cudaFree waits for the
+// work in flight), and the next has an eighth to spare, or what is needed where that
+// does not fit.
 inline int ensure_ws(Workspace& w, size_t need, cudaStream_t s, const char* what,
                      std::vector<void*>& retired) {
-  if (w.bytes >= need) return FT_OK;
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   if (s) cudaStreamIsCapturing(s, &cs);
+  if (w.bytes >= need) {
+    if (cs != cudaStreamCaptureStatusNone) w.captured = true;
+    return FT_OK;
+  }
   FT_CHECK(cs == cudaStreamCaptureStatusNone, FT_ERR_UNSUPPORTED,
            "the %s buffer must grow but the stream is being captured", what);
-  const size_t size = need > 2 * w.bytes ? need : 2 * w.bytes;
-  void* ptr = nullptr;
-  FT_CUDA(cudaMalloc(&ptr, size));
-  try {
-    if (w.ptr) retired.push_back(w.ptr);
-  } catch (...) {  // no exception crosses the C boundary
-    cudaFree(ptr);
-    return fail(FT_ERR_OOM, "out of host memory");
+  size_t size = w.bytes ? need + need / 8 : need;
+  if (w.captured) {
+    size = std::max(size, 2 * w.bytes);
+    try {
+      retired.push_back(w.ptr);
+    } catch (...) {  // no exception crosses the C boundary
+      return fail(FT_ERR_OOM, "out of host memory");
+    }
+  } else if (w.ptr) {
+    FT_CUDA(cudaFree(w.ptr));
   }
-  w.ptr = ptr;
+  w = Workspace{};
+  cudaError_t e = cudaMalloc(&w.ptr, size);
+  if (e == cudaErrorMemoryAllocation && size > need) {
+    cudaGetLastError();
+    size = need;
+    e = cudaMalloc(&w.ptr, size);
+  }
+  if (e != cudaSuccess) {
+    w.ptr = nullptr;
+    cudaGetLastError();
+    return fail(e == cudaErrorMemoryAllocation ? FT_ERR_OOM : FT_ERR_GPU,
+                "the %s buffer of %zu bytes: %s", what, size, cudaGetErrorString(e));
+  }
   w.bytes = size;
   return FT_OK;
 }
