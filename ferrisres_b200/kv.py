@@ -140,6 +140,17 @@ def _tree_args(q: torch.Tensor, mask, batch: int, device, out):
     return q, mask, out
 
 
+def _decode_out(q: torch.Tensor, out) -> torch.Tensor:
+    """The output of a single-token decode of ``q``: a new tensor, or ``out`` if it is
+    contiguous and like q."""
+    if out is None:
+        return torch.empty_like(q)
+    if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or \
+            out.device != q.device or not out.is_contiguous():
+        raise ShapeError("out must be contiguous and like q")
+    return out
+
+
 class Kv3Cache:
     """One layer's 3-bit KV cache for ``batch`` sequences on one GPU."""
 
@@ -258,10 +269,9 @@ class Kv3Cache:
                 q.shape[2] != HEAD_DIM:
             raise ShapeError("q must be fp32 [batch, q_heads, 128]")
         q = q.contiguous()
+        out = _decode_out(q, out)
         if weights is not None:
             return self._decode_weights(q, scale, out, stream, weights)
-        if out is None:
-            out = torch.empty_like(q)
         call("ft_flash_decode_3bit", self.ctx.handle, self.handle, _dptr(q), int(q.shape[1]),
              float(scale), _dptr(out), _call_stream(self.device, stream, q, out))
         return out
@@ -270,10 +280,6 @@ class Kv3Cache:
         if q.device != self.device:
             raise ShapeError(f"q must be on {self.device}")
         step = _row_stride(weights, (self.batch, self.kv_heads), len(self), "weights", self.device)
-        if out is None:
-            out = torch.empty_like(q)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
-            raise ShapeError("out must be like q")
         call("ft_flash_decode_3bit_weights", self.ctx.handle, self.handle, _dptr(q),
              int(q.shape[1]), float(scale), _dptr(out), C.c_void_p(weights.data_ptr()), step,
              _call_stream(self.device, stream, q, out, weights))

@@ -25,7 +25,7 @@ import torch
 
 from ._lib import OOMError, ShapeError, UnsupportedError, call
 from .gpu import _call_stream, _dptr, get_context
-from .kv import _index_list, _row_stride, _tree_args, select_heavy
+from .kv import _decode_out, _index_list, _row_stride, _tree_args, select_heavy
 
 DEFAULT_BLOCK_SIZE = 16   # the reference's default (paged_attention.rs:21)
 PAGE_POSITIONS = 32       # positions per device page
@@ -615,13 +615,10 @@ class PagedKv3Cache:
         lens = np.array([self.seq_len(r, layer) for r in rids], np.int32)
         if lens.max(initial=0) == 0:
             raise ShapeError("flash decode over empty requests")
-        if out is None:
-            out = torch.empty_like(q)
+        out = _decode_out(q, out)
         if weights is not None:
             step = _row_stride(weights, (len(rids), self.kv_heads), int(lens.max()), "weights",
                                self.device)
-            if out.shape != q.shape or out.dtype != q.dtype or out.device != self.device:
-                raise ShapeError("out must be like q")
         tables, stride, lens_dev = self._upload(layer, rids, lens)
         args = (self.ctx.handle, self.handle, len(rids), _dptr(tables), stride, _dptr(lens_dev),
                 int(lens.max()), _dptr(q), int(q.shape[1]), float(scale), _dptr(out))

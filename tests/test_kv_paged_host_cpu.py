@@ -299,3 +299,28 @@ def test_calls_refuse_a_captured_stream(host, monkeypatch, name, current, given)
     with pytest.raises(UnsupportedError):
         go(given)
     assert state(c, [0, 1]) == before and len(host.seen.calls) == calls and now == [current]
+
+
+# -------------------------------------------------------------------- outputs --
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("pool", [False, True])
+def test_decode_refuses_an_output_that_is_not_like_q(host, monkeypatch, pool, weighted):
+    """Smaller, of another type, or strided: the kernel writes [batch, q_heads, 128] adjacent floats."""
+    if pool:
+        c = host(8)
+        rids = [fill(c, 40), fill(c, 33)]
+        go = lambda q, **k: c.flash_decode(0, rids, q, **k)  # noqa: E731
+    else:
+        c = ring(host)
+        monkeypatch.setattr(kv.Kv3Cache, "__len__", lambda self: 40)
+        go = c.flash_decode
+    q = torch.zeros((2, 4, 128))
+    more = {"weights": torch.zeros((2, 2, 40))} if weighted else {}
+    out = torch.empty_like(q)
+    assert go(q, out=out, **more) is out and go(q, **more).shape == q.shape
+    calls = len(host.seen.calls)
+    for bad in (torch.zeros((2, 4, 64)), torch.zeros((1, 4, 128)), q.double(), q.bfloat16(), [0.0],
+                torch.zeros((2, 4, 256))[:, :, :128], torch.zeros((4, 2, 128)).transpose(0, 1)):
+        with pytest.raises(ShapeError):
+            go(q, out=bad, **more)
+    assert len(host.seen.calls) == calls
