@@ -12,7 +12,8 @@ Bounds, each an upper limit of the roundings that the formula needs:
 import pytest
 import torch
 
-from test_kv_tree_gpu import D, causal_bits, exact, generator, kv, paged, rand  # noqa: F401
+from test_kv_tree_gpu import (D, causal_bits, check, exact, generator, kv, paged, rand,  # noqa: F401
+                              rand_mask)
 
 pytestmark = pytest.mark.gpu
 
@@ -228,4 +229,25 @@ def test_references_that_move_fp32(kv, kind):
     out, X, V = exact(q[0], kk[0], vv[0], causal_bits(1, T)[0])
     tol = V * (6 * X * 2.0 ** -20 + 2.0 ** -18 + 2.0 ** -21 + 3 * (n / 32 + 16) * 2.0 ** -24)
     assert bool(((got - out).abs() <= tol).all())
+    c.close()
+
+
+@pytest.mark.parametrize("mode", ["R", "T"])
+@pytest.mark.parametrize("case", [(1, 128 + 1, 1, 1, 1), (1, 256 + 3, 2, 8, 2), (2, 385, 1, 16, 2), (1, 1100, 4, 32, 8),
+                                  (1, 2100, 64, 2, 1), (2, 1500, 64, 4, 1), (1, 3000, 33, 20, 4), (3, 900, 64, 15, 3),
+                                  (1, 20000, 8, 8, 2), (8, 640, 17, 8, 8)])
+def test_whole_prefix_tiles_fp32(kv, case, mode):
+    """fp32 queries, the cases that test_kv_tree_gpu has for bf16 ones: one and many tiles, few and many rows,
+    heads and channels of unequal spread.  Bounds: test_kv_tree_gpu."""
+    B, n, T, Hq, H = case
+    g = generator(n + T)
+    spread = 0.2 + 2 * torch.rand((H, D), generator=g, device="cuda")
+    c = ring(kv, rand(g, B, n, H, D) * spread, rand(g, B, n, H, D) * spread, mode=mode)
+    q = 2 * rand(g, B, T, Hq, D)
+    mask, bits = rand_mask(g, B, T)
+    out = c.tree_decode(q, mask)
+    c.ctx.check()
+    k, v = c.get_range(0, n)
+    for b in range(B):
+        check(out[b], exact(q[b], k[b], v[b], bits[b]), torch.float32, mode, n)
     c.close()
