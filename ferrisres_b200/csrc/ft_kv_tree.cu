@@ -17,7 +17,7 @@
 // absmax in [2^14, 2^15)): hi alone holds a bf16 q exactly down to 2^-29 of the
 // absmax, hi + lo hold 22 bits of an fp32 q or of a rotated one (mode T), which is
 // no bf16 value.  p . v likewise: w = p st as fp16 hi + lo, 22 bits.  (hi alone, 11
-// bits, took 532 us where 64 drafts over 8 x 32768 positions now take 604, but one
+// bits, took 532 us where 64 drafts over 8 x 32768 positions now take 616, but one
 // bf16 output in twenty came out a step off.)  The centred form keeps the products'
 // sums near zero, where the two parts of v do not cancel; the scores of a bf16 q do
 // without it.  (As
@@ -26,8 +26,8 @@
 // the result were lost.)  Softmax statistics, the sum terms and the merge of the
 // splits are fp32; the tensor core's sums are fp32 that it truncates, see below.
 // With mma.sync instead (16 rows a warp, the codes unpacked by every warp) 16
-// drafts over 32768 positions took 86 us where this takes 44 (32 q and 8 kv heads,
-// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 604.
+// drafts over 32768 positions took 86 us where this takes 47 (32 q and 8 kv heads,
+// bf16), and 64 drafts over 8 x 32768 positions 1868 us where it takes 616.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -202,7 +202,7 @@ constexpr float kValueScale = 0x1p-16f;
 // softmax warps (16 rows each) take the even and the odd tiles, each with its own S
 // and O in TMEM and its own running statistics, and merge at the end.  P overwrites S.
 // The waits of the chain S -> P -> O poll, all others suspend the warp: 64 drafts over
-// 8 x 32768 positions take 535 us, 543 when these suspend it too.
+// 8 x 32768 positions take 616 us, 625 when these suspend it too.
 // The K index of the first product is dims in the order 32 (Q/2) + 8r + 4 (Q%2)
 // + (0 2 1 3)[b] of dim 16Q + 4r + b; positions run as 32 w + 8 (s%4) + 4 (s/4%2)
 // + (0 2 1 3)[s/8] of slot s of record w; both so that a converter lane writes the
@@ -218,10 +218,11 @@ constexpr float kValueScale = 0x1p-16f;
 // e of its largest range first; only where one passes that does each position's own e
 // count.
 // kTerms 1: bf16 queries (mode R), q as one fp16; 2: fp32 or rotated queries, hi and lo.
-// P's hi and lo of a record take the columns of its scores.  O is summed in TMEM over the whole split, where the tensor core
-// truncates, 2^-25 of O a product on average: 2^-14 after 2048 products, against
-// 2^-9 of the bf16 output; for fp32 a split has at most 8 tiles (64 products a
-// group: 2^-19 expected, 1e-6 as measured), the splits being merged in fp32.
+// P's hi and lo of a record take the columns of its scores.  O is summed in TMEM over
+// the whole split, where the tensor core truncates, 2^-25 of O a product on average:
+// 2^-14 after 2048 products, against 2^-9 of the bf16 output; for fp32 a split has at
+// most 8 tiles (64 products a group: 2^-19 expected, 1e-6 as measured), the splits being
+// merged in fp32.
 constexpr int kPreRows = 128;
 constexpr int kPreWarps = 28;
 constexpr int kPreRaw = 3;
@@ -293,8 +294,8 @@ __device__ __forceinline__ int row_lane(int i) {
 // first takes the first two records of each tile, the second the others, so that all
 // softmax warps work and each for half as long.  Their weights are 0 in the records
 // that the other takes, their sums are merged like those of the two groups.  (5 drafts
-// over 517 positions, 2 kv heads: 18.4 -> 16.4 us; 16 over 32768, 8 kv heads: 43.0 ->
-// 41.1.  Without the rows' second copies half the softmax warps have nothing to do.)
+// over 517 positions, 2 kv heads: 18.6 -> 16.6 us; 16 over 32768, 8 kv heads: 47.7 ->
+// 46.7.  Without the rows' second copies half the softmax warps have nothing to do.)
 __host__ __device__ constexpr bool twice(int rows) { return rows <= kPreRows / 2; }
 
 // The query operand of tree_tile_kernel, 32 rows a CTA, four a warp: fp16 in the
@@ -939,8 +940,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1)
 }
 
 // Merges the split partials of a row: one CTA a row, its warps share the splits
-// (so that more loads are in flight at once: with a warp a row the decode of 16 drafts
-// over 32768 positions takes 49.5 us, so 45.5), 4 dims a lane; mode T: the output is rotated back.
+// (so that more loads are in flight at once: with one warp the decode of 16 drafts
+// over 32768 positions takes 51.2 us, so 46.7), 4 dims a lane; mode T: the output is rotated back.
 constexpr int kCombineWarps = 4;
 __global__ void __launch_bounds__(32 * kCombineWarps)
     tree_combine_kernel(const __grid_constant__ TreeParams p, void* __restrict__ out) {
@@ -1026,15 +1027,15 @@ void tree_opt_in(int device) {
 
 // Tiles per split, at most `most`: fewest waves of `resident` CTAs x (tiles + a CTA's
 // own cost, which is about three tiles' time: counted as 1 or 6 of them, 64 drafts over
-// 8 x 32768 positions took 547 or 556 us, as 3 they took 544, all measured in one run).
+// 8 x 32768 positions take 616 or 627 us, as 3 they take 616, all measured in one run).
 // `rows` row tiles a sequence; `all` tiles of the batch's sequences together, of which
 // the longest has ntiles.  Unequal sequences: CTAs that would start behind a sequence's
 // end return at once and are not counted (each sequence's last split is taken as half
 // full), and where more CTAs work than are resident the time is their work evenly
 // shared and a quarter of a split.  24 drafts over 6 sequences of 2006 to 8191
-// positions, 4 kv heads: 66 us, 77 with splits for equal lengths; 64 drafts over 8
-// sequences of 500 to 11469, 8 kv heads: 162 and 235 (half a split: 171, an eighth: 181);
-// over 24 of 200 to 29352: 429 and 431 (443, 417).
+// positions, 4 kv heads: 70 us, 78 with splits for equal lengths; 64 drafts over 8
+// sequences of 500 to 11469, 8 kv heads: 179 and 257 (half a split: 188, an eighth: 200);
+// over 24 of 200 to 29352: 475 and 468 (486, 465), the one where others are better.
 constexpr int64_t kPreOverhead = 3;
 constexpr int64_t kTailParts = 4;  // of a split
 constexpr int64_t kTermTiles = 8;  // fp32 queries: most tiles of a split

@@ -152,7 +152,11 @@ def _decode_out(q: torch.Tensor, out) -> torch.Tensor:
 
 
 class Kv3Cache:
-    """One layer's 3-bit KV cache for ``batch`` sequences on one GPU."""
+    """One layer's 3-bit KV cache for ``batch`` sequences on one GPU.
+
+    ``stream``: a call runs there, behind what the current stream holds so far.  Calls on
+    one cache share its scratch: they, and replays of graphs that hold them, follow one
+    another."""
 
     def __init__(self, batch: int, kv_heads: int, max_seq: int, head_dim: int = HEAD_DIM,
                  device=None, mode: str = "R", seed: int = 0):
