@@ -160,11 +160,16 @@ class PrefixSharingManager:
 
     def __init__(self, allocator: BlockAllocator, block_size: int):
         self._prefixes: dict[tuple, list[list[int]]] = {}
+        self._named: dict[int, set[tuple]] = {}  # block -> prefixes that name it
         self._alloc = allocator
         self._bs = int(block_size)
 
     def register_prefix(self, prefix_tokens, layer_blocks) -> None:
-        self._prefixes[tuple(prefix_tokens)] = [list(b) for b in layer_blocks]
+        key = tuple(prefix_tokens)
+        self.remove_prefix(key)
+        self._prefixes[key] = [list(b) for b in layer_blocks]
+        for b in set().union(*self._prefixes[key]):
+            self._named.setdefault(b, set()).add(key)
 
     def lookup_prefix(self, prefix_tokens):
         """The blocks of a registered prefix, one more reference on each; None if absent."""
@@ -183,20 +188,23 @@ class PrefixSharingManager:
         return tuple(tokens) in self._prefixes
 
     def remove_prefix(self, tokens) -> None:
-        self._prefixes.pop(tuple(tokens), None)
+        key = tuple(tokens)
+        for b in set().union(*self._prefixes.pop(key, ())):
+            self._named[b].discard(key)
+            if not self._named[b]:
+                del self._named[b]
 
     def forget_blocks(self, changed: dict, freed=()) -> None:
         """Drops the registrations that blocks no longer fit (no counterpart in the
         reference, where a block's positions never change): those that name a block of
         ``freed``, or one of ``changed`` (block -> its first slot that holds another
         position now) with that slot among the prefix's tokens."""
-        def stale(n_tokens, layer_blocks):
-            return any(b in freed or j * self._bs + changed.get(b, n_tokens) < n_tokens
-                       for j, b in enumerate(layer_blocks))
-
-        for key in [k for k, blocks in self._prefixes.items()
-                    if any(stale(len(k), lb) for lb in blocks)]:
-            del self._prefixes[key]
+        for b in {*changed, *freed} & self._named.keys():
+            for key in list(self._named.get(b, ())):
+                if b in freed or any(x == b and j * self._bs + changed[b] < len(key)
+                                     for blocks in self._prefixes[key]
+                                     for j, x in enumerate(blocks)):
+                    self.remove_prefix(key)
 
 
 class PagedAttentionManager:

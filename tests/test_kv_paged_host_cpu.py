@@ -147,6 +147,27 @@ def test_evict_forgets_a_prefix(host, monkeypatch):
     assert pm.lookup_prefix(range(32)) is None
 
 
+def test_forgetting_looks_at_the_pages_of_the_call_only(host):
+    """Registrations anew, removed, of several layers and in large numbers."""
+    c = host(8)
+    r, other = fill(c, 64), fill(c, 64)
+    pm = c.manager.prefix_manager()
+    a, b = c.block_table(r), c.block_table(other)
+    for i in range(500):
+        pm.register_prefix([i] * 64, [b])
+    pm.register_prefix(range(64), [a])
+    pm.register_prefix(range(64), [b])  # the same tokens, now elsewhere
+    pm.register_prefix(range(32), [b[:1], a[:1]])  # the second layer's page
+    pm.register_prefix(range(33), [a])
+    pm.remove_prefix(range(33))
+    pm.remove_prefix(range(33))
+    c.keep(0, [r], idx(10, 5))
+    assert not pm.has_prefix(range(32)) and not pm.has_prefix(range(33))
+    assert pm.has_prefix(range(64)) and pm.num_prefixes() == 501
+    c.keep(0, [other], idx(10, 5))
+    assert pm.num_prefixes() == 0 and not pm._named
+
+
 # ------------------------------------------------------------- free pages --
 def test_keep_needs_no_copy_for_the_last_owner(host):
     """A request and its fork, both rewritten: half of their pages have to be copied."""
