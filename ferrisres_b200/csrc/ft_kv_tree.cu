@@ -188,7 +188,7 @@ __device__ __forceinline__ float scale2(float v, float half_pow) { return v * ha
 
 // The tile kernel takes V as V * 2^-16, so that with the largest ranges (e = 112) exp2(x - M)
 // is at least 2^-107 for the heaviest position, 2^19 above the smallest normal float;
-// the combine kernel scales back.
+// the combine kernel scales back.  (Values below 2^-110 lose low bits to it: 2^-133.)
 constexpr float kValueScale = 0x1p-16f;
 
 // ---------------------------------------------------------------- tiles --
